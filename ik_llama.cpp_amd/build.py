@@ -18,7 +18,8 @@ GEMV_ONLY_TYPES = [153, 154, 155, 158]   # IQ2_KT IQ3_KT IQ4_KT IQ1_KT (trellis)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",
          "-Wall", "-Wno-unused-function", "-I/opt/rocm/include",
          "--offload-compress",    # compressed code objects: the library is ~100 translation units of template instantiations (96 MB plain); every gpurun call pushes it
-         "-fno-slp-vectorize"]    # keep scalar v_fma_f32: v_pk_fma_f32 beside MFMAs is slower (MI355X guide, "price of one filler")
+         "-fno-slp-vectorize",    # keep scalar v_fma_f32: v_pk_fma_f32 beside MFMAs is slower (MI355X guide, "price of one filler")
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]    # no packed f32 arithmetic at all: some forms of it have given wrong results on this hardware (the host pass does not know the feature and says so)
 EXTRA_FLAGS = os.environ.get("CDNA4_BUILD_FLAGS", "").split()     # developer knob: e.g. -DGEMV_EXP_TIMELINE
 
 COMMON = ["api_internal.h", "cdna4_common.cuh", os.path.join("..", "..", "include", "ggml_hip_cdna4.h")]
