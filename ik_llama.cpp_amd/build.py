@@ -38,6 +38,8 @@ def translation_units():
         tus.append(("ops", "ops.hip", [], COMMON + ["fa_decode.cuh"]))
     if os.path.exists(os.path.join(CSRC, "flash_attn.hip")):
         tus.append(("flash_attn", "flash_attn.hip", [], COMMON))
+    for name in ("paged", "paged_attn", "beam"):
+        tus.append((name, name + ".hip", [], COMMON + ["paged.cuh", "fa_decode.cuh"]))
     for t in BASE_TYPES:
         for up in (0, 1):
             tus.append(("gemv_%d_%s" % (t, "upgate" if up else "plain"), "gemv_inst.hip", ["-DINST_TYPE=%d" % t, "-DINST_UPGATE=%d" % up], GEMV_DEPS))

@@ -121,6 +121,14 @@ SIGNATURES = {
     "cdna4_window_all_reduce_sum_wire": (_I, [_P, _P, _I64, _I, _I, _I, _P]),
     "cdna4_window_free": (None, [_P]),
     "cdna4_op_mul_mat_dense": (_I, [_P, _P, _P, _P, _P]),
+    "cdna4_op_paged_store": (_I, [_P] * 13),
+    "cdna4_op_paged_attn": (_I, [_P] * 8 + [C.c_float, C.c_float, _P]),
+    "cdna4_paged_attn_workspace": (_I64, [_P] * 6),
+    "cdna4_op_paged_evict": (_I, [_P] * 8 + [_I] * 3 + [_P] * 4),
+    "cdna4_paged_evict_workspace": (_I64, [_P] * 5 + [_I] * 3 + [_P] * 2),
+    "cdna4_op_beam_select": (_I, [_P] * 4 + [_I] * 3 + [_P] * 4),
+    "cdna4_beam_select_workspace": (_I64, [_P] + [_I] * 3),
+    "cdna4_op_paged_fork": (_I, [_P] * 10),
     "cdna4_repack_r4": (_I, [_P, _I, _P, _I64, _I64, _P, _P]),
     "cdna4_unrepack_r4": (_I, [_P, _I, _P, _I64, _I64, _P, _P]),
     "cdna4_invalidate_weight_cache": (_I, [_P, _P]),
@@ -164,6 +172,10 @@ def load_library(path=None):
     if path is None:
         _lib = lib
     return lib
+
+
+class _Tensor(C.Structure):      # cdna4_tensor {data, type, ne[4], nb[4]} (include/ggml_hip_cdna4.h)
+    _fields_ = [("data", C.c_void_p), ("type", C.c_int), ("ne", C.c_int64 * 4), ("nb", C.c_int64 * 4)]
 
 
 class _Fusion(C.Structure):      # cdna4_fusion {norm_w, norm_eps, residual, qkv, add_b, add_dst} (include/ggml_hip_cdna4.h)
@@ -417,6 +429,115 @@ class Cdna4Backend:
 
     def invalidate_weight_cache(self, w=None):
         self._check(self.lib.cdna4_invalidate_weight_cache(self.ctx, w.data_ptr() if w is not None else None))
+
+    # ---- decoding over a paged key / value cache
+    # Caches are torch.float16 / torch.bfloat16 [n_pages, n_head_kv, page, D] views of any strides with dense rows (token-major pages: x.transpose(1, 2)), tables int32 [n_seq, W]; n_kv,
+    # n_past, start, parent, fresh and done are dense int32 vectors, weight / pos float32 / int32 [n_seq, n_head_kv, >= W * page], all on the backend's device.  What the library refuses
+    # raises Cdna4Error before anything is launched.
+    def _desc(self, x, name):
+        """the ggml descriptor (sizes and byte strides from the innermost dimension out) of a torch tensor of at most 4 dimensions"""
+        types = {self.torch.float32: T["F32"], self.torch.float16: T["F16"], self.torch.bfloat16: T["BF16"], self.torch.int32: 26}
+        if not self.torch.is_tensor(x) or x.device != self.device or x.dtype not in types or not 1 <= x.dim() <= 4:
+            raise Cdna4Error(-2, "%s: a float32 / float16 / bfloat16 / int32 tensor of 1 to 4 dimensions on %s" % (name, self.device))
+        ne, nb = list(x.shape)[::-1], [s * x.element_size() for s in x.stride()][::-1]
+        for i, n in enumerate(ne):          # (torch gives dimensions of one element arbitrary strides: a dense one says the same)
+            if n == 1:
+                nb[i] = nb[i - 1] * ne[i - 1] if i else x.element_size()
+        while len(ne) < 4:
+            nb.append(nb[-1] * ne[-1]); ne.append(1)
+        return C.byref(_Tensor(x.data_ptr(), types[x.dtype], (C.c_int64 * 4)(*ne), (C.c_int64 * 4)(*nb)))
+
+    def _vec(self, x, name, n, dtype=None):
+        """address of a dense vector of n elements (int32 unless said), None for None"""
+        dtype = dtype or self.torch.int32
+        if x is None:
+            return None
+        if not self.torch.is_tensor(x) or x.device != self.device or x.dtype != dtype or x.dim() < 1 or x.numel() != n or not x.is_contiguous():
+            raise Cdna4Error(-2, "%s: a dense %s vector of %d elements on %s" % (name, dtype, n, self.device))
+        return x.data_ptr()
+
+    def _table_rows(self, table, name="table"):
+        if not self.torch.is_tensor(table) or table.dim() != 2:
+            raise Cdna4Error(-2, "%s: int32 [n_seq, W]" % name)
+        return table.shape[0]
+
+    def _ints(self, *shape):
+        return self.torch.empty(shape, dtype=self.torch.int32, device=self.device)
+
+    def paged_store(self, k, v, k_cache, v_cache, table, n_kv, start=None, n_past=None, weight=None, pos=None, n_kv_out=None):
+        """cdna4_op_paged_store: k, v f32 [n_tok, n_head_kv, D] into the slots behind n_kv (start int32 [n_seq + 1]: token ranges of the sequences, None: one token each); returns the new n_kv."""
+        n = self._table_rows(table)
+        if n_kv_out is None:
+            n_kv_out = self._ints(n)
+        self._check(self.lib.cdna4_op_paged_store(self.ctx, self._desc(k, "k"), self._desc(v, "v"), self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), self._desc(table, "table"),
+                                                  self._vec(n_kv, "n_kv", n), self._vec(start, "start", n + 1), self._vec(n_past, "n_past", n),
+                                                  None if weight is None else self._desc(weight, "weight"), None if pos is None else self._desc(pos, "pos"),
+                                                  self._vec(n_kv_out, "n_kv_out", n), self._stream()))
+        return n_kv_out
+
+    def paged_attn(self, q, k_cache, v_cache, table, n_kv, scale=None, softcap=0.0, weight=None, out=None):
+        """cdna4_op_paged_attn: q f32 [n_seq, n_head, D] -> f32 [n_seq, n_head, D]; scale None: 1 / sqrt(D); weight: += the attention weight that every slot gathers, in place."""
+        qd = self._desc(q, "q")
+        if out is None:
+            out = self.torch.empty(q.shape, dtype=self.torch.float32, device=self.device)
+        self._check(self.lib.cdna4_op_paged_attn(self.ctx, qd, self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), self._desc(table, "table"),
+                                                 self._vec(n_kv, "n_kv", self._table_rows(table)), None if weight is None else self._desc(weight, "weight"), self._desc(out, "out"),
+                                                 float(q.shape[-1] ** -0.5 if scale is None else scale), float(softcap), self._stream()))
+        return out
+
+    def paged_evict(self, k_cache, v_cache, table, n_kv, weight, pos, n_past, budget, n_sink=0, n_recent=0, weight_out=None, pos_out=None, n_kv_out=None):
+        """cdna4_op_paged_evict: every (sequence, KV head) keeps `budget` slots, by position and gathered weight; weight_out / pos_out None: in place.  Returns the new n_kv."""
+        n = self._table_rows(table)
+        if n_kv_out is None:
+            n_kv_out = self._ints(n)
+        self._check(self.lib.cdna4_op_paged_evict(self.ctx, self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), self._desc(table, "table"), self._vec(n_kv, "n_kv", n),
+                                                  self._desc(weight, "weight"), self._desc(pos, "pos"), self._vec(n_past, "n_past", n), budget, n_sink, n_recent,
+                                                  self._desc(weight if weight_out is None else weight_out, "weight_out"), self._desc(pos if pos_out is None else pos_out, "pos_out"),
+                                                  self._vec(n_kv_out, "n_kv_out", n), self._stream()))
+        return n_kv_out
+
+    def beam_select(self, logits, score, n_beam, n_out, done=None, pad=0, outs=None):
+        """cdna4_op_beam_select: logits f32 [n_group * n_beam, n_vocab], score f32 [n_group * n_beam] -> (score f32, parent row int32, token int32), each [n_group, n_out]."""
+        d = self._desc(logits, "logits")
+        rows = logits.shape[0]; n_group = rows // n_beam if n_beam > 0 else 0
+        if outs is None:
+            shape = (n_group, max(n_out, 0))
+            outs = (self.torch.empty(shape, dtype=self.torch.float32, device=self.device), self._ints(*shape), self._ints(*shape))
+        ptr = [self._vec(x, name, n_group * n_out, want) for x, name, want in
+               zip(outs, ("score_out", "parent", "token"), (self.torch.float32, self.torch.int32, self.torch.int32))]
+        self._check(self.lib.cdna4_op_beam_select(self.ctx, d, self._vec(score, "score", rows, self.torch.float32), self._vec(done, "done", rows), n_beam, n_out, pad, *ptr, self._stream()))
+        return outs
+
+    def paged_fork(self, k_cache, v_cache, table, n_kv, parent, fresh, table_out=None, n_kv_out=None):
+        """cdna4_op_paged_fork: rows that go on from row parent[i] (full pages shared, a cut last page copied into page fresh[i]); returns (table int32 [n_out, W], n_kv int32 [n_out])."""
+        n = self._table_rows(table); n_out = parent.numel() if self.torch.is_tensor(parent) else 0
+        if table_out is None:
+            table_out = self._ints(n_out, table.shape[1])
+        if n_kv_out is None:
+            n_kv_out = self._ints(n_out)
+        self._check(self.lib.cdna4_op_paged_fork(self.ctx, self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), self._desc(table, "table"), self._vec(n_kv, "n_kv", n),
+                                                 self._vec(parent, "parent", n_out), self._vec(fresh, "fresh", n_out), self._desc(table_out, "table_out"),
+                                                 self._vec(n_kv_out, "n_kv_out", n_out), self._stream()))
+        return table_out, n_kv_out
+
+    def paged_workspace(self, q, k_cache, v_cache, table, weight=None, out=None):
+        """bytes of scratch that paged_attn takes for these tensors (reserve_workspace them before a capture)"""
+        return self._bytes(self.lib.cdna4_paged_attn_workspace(self._desc(q, "q"), self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), self._desc(table, "table"),
+                                                               None if weight is None else self._desc(weight, "weight"), self._desc(q if out is None else out, "out")))
+
+    def evict_workspace(self, k_cache, v_cache, table, weight, pos, budget, n_sink=0, n_recent=0):
+        """bytes of scratch that paged_evict takes"""
+        w, p = self._desc(weight, "weight"), self._desc(pos, "pos")
+        return self._bytes(self.lib.cdna4_paged_evict_workspace(self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), self._desc(table, "table"), w, p, budget, n_sink, n_recent, w, p))
+
+    def beam_workspace(self, logits, n_beam, n_out, pad=0):
+        """bytes of scratch that beam_select takes"""
+        return self._bytes(self.lib.cdna4_beam_select_workspace(self._desc(logits, "logits"), n_beam, n_out, pad))
+
+    def _bytes(self, n):
+        if n < 0:
+            self._check(int(n))
+        return int(n)
 
     # ---- tensor parallel reduce (GGML_OP_REDUCE)
     def comm_unique_id(self):

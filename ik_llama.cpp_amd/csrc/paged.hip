@@ -1,0 +1,292 @@
+// paged.hip -- storing into, evicting from and forking a paged key / value cache (the attention that reads it: paged_attn.hip).
+#include "paged.cuh"
+#include <algorithm>
+
+struct SlotView { char *p; long head, seq; };           // weight / pos: bytes between KV heads and sequences
+static SlotView slot_view(const cdna4_tensor *t) { SlotView s = {nullptr, 0, 0}; if (t) { s.p = (char *)t->data; s.head = t->nb[1]; s.seq = t->nb[2]; } return s; }
+template <typename X> static __device__ __forceinline__ X *slot_row(const SlotView &v, int s, int h) { return reinterpret_cast<X *>(v.p + (long)s * v.seq + (long)h * v.head); }
+
+// ------------------------------------------------------------------------------------------------ store
+struct StoreArgs {
+    PagedCache c; const char *k, *v; long k_head, v_head, k_tok, v_tok;
+    const int *start, *n_past; SlotView weight, pos; int *n_kv_out; int n_tok; int bf16;
+};
+// two f32 -> two 16-bit values of the cache type, rounded to nearest even (the one rounding of K and V)
+template <bool BF16> static __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (BF16) return float_to_bf16_bits(a) | (float_to_bf16_bits(b) << 16);
+    else { typedef _Float16 h2 __attribute__((ext_vector_type(2))); const h2 h = {(_Float16)a, (_Float16)b}; return __builtin_bit_cast(uint32_t, h); }
+}
+// the sequence of token i: the last s with start[s] <= i (a wave reads the whole vector at once: one memory latency instead of a binary search's chain of them)
+static __device__ __forceinline__ int token_seq(const int *start, int n_seq, int i) {
+    if (!start) return i;
+    int n = 0;
+    for (int b = 0; b < n_seq; b += 64) {
+        const int s = b + (int)(threadIdx.x & 63);
+        n += __popcll(__ballot(s < n_seq && start[min(s, n_seq - 1)] <= i));
+    }
+    return i < start[n_seq] ? n - 1 : -1;
+}
+// One workgroup per token; a thread moves 8 values of K or V at a time.  The f32 rows do not depend on where they go: the first load of every thread runs under the lookups of sequence,
+// length and page (unconditional, on a clamped unit: loaded under a branch and carried into the loop, this compiler reuses three of the four registers before they are read).
+template <bool BF16> __global__ void __launch_bounds__(256) paged_store_kernel(StoreArgs a) {
+    const int tok = blockIdx.x;
+    if (tok >= a.n_tok) {          // the workgroups behind the tokens: the new lengths
+        const int s = (tok - a.n_tok) * 256 + (int)threadIdx.x;
+        if (s < a.c.n_seq) {
+            const int n = a.c.n_kv[s], add = a.start ? max(a.start[s + 1] - a.start[s], 0) : 1;
+            a.n_kv_out[s] = n < 0 ? n : (int)min((long)n + add, (long)a.c.W << a.c.page_shift);
+        }
+        return;
+    }
+    const int lg = a.c.D == 64 ? 3 : a.c.D == 128 ? 4 : 5, half = a.c.n_head_kv << lg, units = 2 * half;        // units of 8 values: all of K, then all of V
+    auto source = [&](int u) {
+        const int w = u >= half ? u - half : u, h = w >> lg, d = (w - (h << lg)) * 8;
+        return reinterpret_cast<const float4 *>((u >= half ? a.v + (long)tok * a.v_tok + (long)h * a.v_head : a.k + (long)tok * a.k_tok + (long)h * a.k_head) + d * 4);
+    };
+    int u = threadIdx.x;
+    const float4 *src = source(min(u, units - 1));
+    const float4 f0 = src[0], f1 = src[1];
+    const int s = token_seq(a.start, a.c.n_seq, tok);
+    if (s < 0 || s >= a.c.n_seq) return;
+    const int n = a.c.n_kv[s], nth = a.start ? tok - a.start[s] : 0;
+    const long slot = (long)n + nth;
+    if (n < 0 || nth < 0 || slot >= ((long)a.c.W << a.c.page_shift)) return;
+    const int page = paged_page(a.c, s, (int)slot);
+    if (page < 0) return;
+    const int in = (int)slot & ((1 << a.c.page_shift) - 1);
+    char *kp = a.c.k + (long)page * a.c.k_page + (long)in * a.c.k_row, *vp = a.c.v + (long)page * a.c.v_page + (long)in * a.c.v_row;
+    auto store = [&](int unit, const float4 &x, const float4 &y) {
+        const int w = unit >= half ? unit - half : unit, h = w >> lg, d = (w - (h << lg)) * 8;
+        char *p = unit >= half ? vp + (long)h * a.c.v_head : kp + (long)h * a.c.k_head;
+        *reinterpret_cast<uint4 *>(p + d * 2) = make_uint4(pack2<BF16>(x.x, x.y), pack2<BF16>(x.z, x.w), pack2<BF16>(y.x, y.y), pack2<BF16>(y.z, y.w));
+    };
+    if (u < units) store(u, f0, f1);
+    for (u += 256; u < units; u += 256) { const float4 *p = source(u); const float4 x = p[0], y = p[1]; store(u, x, y); }
+    for (int h = threadIdx.x; h < a.c.n_head_kv; h += 256) {
+        if (a.weight.p) slot_row<float>(a.weight, s, h)[slot] = 0.0f;
+        if (a.pos.p) slot_row<int>(a.pos, s, h)[slot] = a.n_past[s] + nth;
+    }
+}
+static int new_rows_check(const char *name, const cdna4_tensor *t, const PagedCache &c) {
+    ARG_CHECK(pg_sizes_ok(t) && t->type == CDNA4_TYPE_F32 && t->ne[0] == c.D && t->ne[1] == c.n_head_kv && t->ne[3] == 1, "paged_store: %s f32 [D, n_head_kv, n_tok]", name);
+    OP_CHECK(t->nb[0] == 4 && t->nb[1] % 16 == 0 && t->nb[2] % 16 == 0 && (uintptr_t)t->data % 16 == 0, "paged_store: %s rows dense and 16-byte aligned", name);
+    return CDNA4_OK;
+}
+int cdna4_op_paged_store(cdna4_context *ctx, const cdna4_tensor *k, const cdna4_tensor *v, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table,
+                         const int32_t *n_kv, const int32_t *start, const int32_t *n_past, const cdna4_tensor *weight, const cdna4_tensor *pos, int32_t *n_kv_out, void *stream) {
+    ARG_CHECK(ctx && k && v, "paged_store: null argument");
+    StoreArgs a; int rc = pg_cache_check("paged_store", k_cache, v_cache, table, true, &a.c); if (rc) return rc;
+    if ((rc = new_rows_check("k", k, a.c)) || (rc = new_rows_check("v", v, a.c))) return rc;
+    ARG_CHECK(k->ne[2] == v->ne[2], "paged_store: as many rows of k as of v");
+    const long n_tok = k->ne[2], n_seq = a.c.n_seq;
+    OP_CHECK(n_tok <= 0x7fffffff - PAGED_MAX_SEQ, "paged_store: too many tokens");
+    ARG_CHECK(start || n_tok == n_seq, "paged_store: without start, one token per sequence");
+    if (weight && (rc = pg_slots_check("paged_store", "weight", weight, CDNA4_TYPE_F32, a.c, true))) return rc;
+    if (pos && (rc = pg_slots_check("paged_store", "pos", pos, CDNA4_TYPE_I32, a.c, true))) return rc;
+    if (n_seq == 0) return CDNA4_OK;
+    ARG_CHECK(n_kv && (a.c.table || a.c.W == 0) && (n_tok == 0 || (k->data && v->data)) && (!pos || n_past), "paged_store: null data");
+    ARG_CHECK((!weight || weight->data || a.c.W == 0) && (!pos || pos->data || a.c.W == 0), "paged_store: null data");
+    ARG_CHECK(!n_kv_out || !pg_overlap(n_kv_out, n_seq * 4, n_kv, n_seq * 4), "paged_store: n_kv_out overlaps n_kv");
+    a.k = (const char *)k->data; a.v = (const char *)v->data; a.k_head = k->nb[1]; a.v_head = v->nb[1]; a.k_tok = k->nb[2]; a.v_tok = v->nb[2];
+    a.c.n_kv = n_kv; a.start = start; a.n_past = n_past; a.weight = slot_view(weight); a.pos = slot_view(pos); a.n_kv_out = n_kv_out; a.n_tok = (int)n_tok;
+    const long blocks = n_tok + (n_kv_out ? (n_seq + 255) / 256 : 0);
+    if (blocks == 0) return CDNA4_OK;
+    DEVICE_SCOPE(ctx);
+    if (k_cache->type == CDNA4_TYPE_BF16) hipLaunchKernelGGL(paged_store_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL(paged_store_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
+    HIP_TRY(hipGetLastError()); return CDNA4_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ fork
+struct ForkArgs { PagedCache c; const int *parent, *fresh; int *table_out, *n_kv_out; long out_row; };
+// grid (KV heads, rows): a workgroup copies the cut page's used slots of one head, K and V; the first head's workgroup also writes the row of the table.
+__global__ void __launch_bounds__(256) paged_fork_kernel(ForkArgs a) {
+    const int h = blockIdx.x, i = blockIdx.y, p = a.parent[i];
+    const bool live = (unsigned)p < (unsigned)a.c.n_seq && a.c.n_kv[(unsigned)p < (unsigned)a.c.n_seq ? p : 0] >= 0;
+    const int n = live ? paged_len(a.c, p) : -1;
+    const int full = live ? n >> a.c.page_shift : 0, used = live ? n & ((1 << a.c.page_shift) - 1) : 0;
+    const int fresh = a.fresh[i], to = (unsigned)fresh < (unsigned)a.c.n_pages ? fresh : -1;
+    if (h == 0) {
+        int *row = a.table_out + (long)i * a.out_row;
+        for (int w = threadIdx.x; w < a.c.W; w += 256) row[w] = w < full ? a.c.table[(long)p * a.c.table_row + w] : w == full && used ? to : -1;
+        if (threadIdx.x == 0) a.n_kv_out[i] = n;
+    }
+    if (!used || to < 0) return;
+    const int from = paged_page(a.c, p, full << a.c.page_shift);
+    if (from < 0) return;
+    const int per_row = a.c.D / 8, units = used * per_row;
+    const char *ks = a.c.k + (long)from * a.c.k_page + (long)h * a.c.k_head, *vs = a.c.v + (long)from * a.c.v_page + (long)h * a.c.v_head;
+    char *kd = a.c.k + (long)to * a.c.k_page + (long)h * a.c.k_head, *vd = a.c.v + (long)to * a.c.v_page + (long)h * a.c.v_head;
+    for (int u = threadIdx.x; u < units; u += 256) {
+        const int r = u / per_row, d = (u - r * per_row) * 16;
+        const uint4 x = *reinterpret_cast<const uint4 *>(ks + r * a.c.k_row + d), y = *reinterpret_cast<const uint4 *>(vs + r * a.c.v_row + d);
+        *reinterpret_cast<uint4 *>(kd + r * a.c.k_row + d) = x; *reinterpret_cast<uint4 *>(vd + r * a.c.v_row + d) = y;
+    }
+}
+int cdna4_op_paged_fork(cdna4_context *ctx, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const int32_t *n_kv, const int32_t *parent,
+                        const int32_t *fresh, const cdna4_tensor *table_out, int32_t *n_kv_out, void *stream) {
+    ARG_CHECK(ctx && table_out, "paged_fork: null argument");
+    ForkArgs a; int rc = pg_cache_check("paged_fork", k_cache, v_cache, table, true, &a.c); if (rc) return rc;
+    ARG_CHECK(pg_sizes_ok(table_out) && table_out->type == CDNA4_TYPE_I32 && table_out->nb[0] == 4 && table_out->nb[1] % 4 == 0 && table_out->ne[0] == a.c.W && table_out->ne[2] == 1 &&
+              table_out->ne[3] == 1 && pg_disjoint_elems(table_out, 4), "paged_fork: table_out i32 [W, n_out]");
+    const long n_out = table_out->ne[1], n_seq = a.c.n_seq;
+    OP_CHECK(n_out <= PAGED_MAX_SEQ, "paged_fork: at most %ld rows", PAGED_MAX_SEQ);
+    if (n_out == 0) return CDNA4_OK;
+    ARG_CHECK(n_seq > 0 && n_kv && parent && fresh && n_kv_out && ((a.c.table && table_out->data) || a.c.W == 0), "paged_fork: null data");
+    ARG_CHECK(!pg_overlap(n_kv_out, n_out * 4, n_kv, n_seq * 4) && !pg_overlap(n_kv_out, n_out * 4, parent, n_out * 4) && !pg_overlap(n_kv_out, n_out * 4, fresh, n_out * 4),
+              "paged_fork: n_kv_out overlaps an input");
+    if (a.c.W) {
+        ARG_CHECK(!pg_overlap(table_out, 4, table, 4) && !pg_overlap(table_out->data, pg_extent(table_out, 4), parent, n_out * 4) && !pg_overlap(table_out->data, pg_extent(table_out, 4), fresh, n_out * 4) &&
+                  !pg_overlap(table_out->data, pg_extent(table_out, 4), n_kv, n_seq * 4) && !pg_overlap(table_out->data, pg_extent(table_out, 4), n_kv_out, n_out * 4), "paged_fork: table_out overlaps another argument");
+    }
+    a.c.n_kv = n_kv; a.parent = parent; a.fresh = fresh; a.table_out = (int *)table_out->data; a.n_kv_out = n_kv_out; a.out_row = table_out->nb[1] / 4;
+    DEVICE_SCOPE(ctx);
+    hipLaunchKernelGGL(paged_fork_kernel, dim3((unsigned)a.c.n_head_kv, (unsigned)n_out), dim3(256), 0, (hipStream_t)stream, a);
+    HIP_TRY(hipGetLastError()); return CDNA4_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ evict
+struct EvictArgs {
+    PagedCache c; SlotView weight, pos, weight_out, pos_out; const int *n_past; int *n_kv_out; int budget, sink, recent, in_place, list;        // list: ints per (sequence, head) in `moves`
+    int *moves;                                                                                                                           // [count, from[max], to[max]]
+};
+// sort key of a slot: larger = kept first.  Held slots above everything, then the order of the floats (-0 as 0, NaN as -inf)
+static __device__ __forceinline__ uint32_t evict_key(float w, int p, int sink, long recent_from) {
+    if (p < sink || (long)p >= recent_from) return 0xffffffffu;
+    if (w != w) w = -INFINITY;
+    const uint32_t b = __float_as_uint(w + 0.0f);
+    return b ^ ((b & 0x80000000u) ? 0xffffffffu : 0x80000000u);
+}
+// One workgroup per (sequence, KV head).  The budget-th largest key by four passes over 8-bit digits, then the slots in order: which kept ones lie behind the budget, which freed
+// ones before it.  Each wave owns a contiguous range of slots, so that a prefix sum over 16 wave totals is all the order takes.
+constexpr int EVICT_THREADS = 1024, EVICT_WAVES = 16;
+__global__ void __launch_bounds__(EVICT_THREADS) paged_evict_select_kernel(EvictArgs a) {
+    __shared__ unsigned hist[256], tot[3][EVICT_WAVES]; __shared__ unsigned s_digit, s_rest;
+    const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int raw = a.c.n_kv[s], n = paged_len(a.c, s);
+    int *moves = a.moves + ((long)s * a.c.n_head_kv + h) * a.list; const int most = (a.list - 1) / 2;
+    const float *w = slot_row<const float>(a.weight, s, h); const int *p = slot_row<const int>(a.pos, s, h);
+    float *wo = slot_row<float>(a.weight_out, s, h); int *po = slot_row<int>(a.pos_out, s, h);
+    if (h == 0 && tid == 0) a.n_kv_out[s] = raw < 0 ? raw : min(n, a.budget);
+    if (n <= a.budget) {
+        if (tid == 0) moves[0] = 0;
+        if (!a.in_place) for (int j = tid; j < n; j += EVICT_THREADS) { wo[j] = w[j]; po[j] = p[j]; }
+        return;
+    }
+    const long recent_from = (long)a.n_past[s] - a.recent;
+    auto key = [&](int j) { return evict_key(w[j], p[j], a.sink, recent_from); };
+    uint32_t prefix = 0, rest = (uint32_t)a.budget;         // the budget-th largest key lies among those whose digits so far equal `prefix`; `rest` of them are kept
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (tid < 256) hist[tid] = 0;
+        __syncthreads();
+        for (int j = tid; j < n; j += EVICT_THREADS) {
+            const uint32_t x = key(j);
+            if (shift == 24 || (x >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(x >> shift) & 255], 1u);
+        }
+        __syncthreads();
+        if (wave == 0) {                                    // the digit at which the count from above reaches `rest`
+            unsigned c[4], sum = 0;
+            for (int i = 0; i < 4; ++i) { c[i] = hist[255 - (4 * lane + i)]; sum += c[i]; }
+            unsigned above = sum;
+            for (int o = 1; o < 64; o <<= 1) { const unsigned y = __shfl_up(above, o, 64); if (lane >= o) above += y; }
+            above -= sum;
+            for (int i = 0; i < 4; ++i) { if (above < rest && above + c[i] >= rest) { s_digit = 255 - (4 * lane + i); s_rest = rest - above; } above += c[i]; }
+        }
+        __syncthreads();
+        prefix |= s_digit << shift; rest = s_rest;
+        __syncthreads();
+    }
+    const int span = ((n + EVICT_WAVES - 1) / EVICT_WAVES + 63) & ~63, j0 = min(wave * span, n), j1 = min(j0 + span, n);
+    const unsigned long long below = (1ull << lane) - 1;
+    unsigned ties = 0;
+    for (int b = j0; b < j1; b += 64) { const int j = b + lane; ties += __popcll(__ballot(j < j1 && key(min(j, n - 1)) == prefix)); }
+    if (lane == 0) tot[0][wave] = ties;
+    __syncthreads();
+    unsigned tie0 = 0; for (int i = 0; i < wave; ++i) tie0 += tot[0][i];
+    // two rounds over the wave's slots: count holes and movers, then list them
+    unsigned holes = 0, movers = 0, nh = 0, nm = 0;
+    for (int round = 0; round < 2; ++round) {
+        unsigned t = tie0; nh = holes; nm = movers;
+        for (int b = j0; b < j1; b += 64) {
+            const int j = b + lane; const bool in = j < j1; const uint32_t x = in ? key(j) : 0u;
+            const unsigned long long tie = __ballot(in && x == prefix);
+            const bool keep = in && (x > prefix || (x == prefix && t + __popcll(tie & below) < rest));
+            t += __popcll(tie);
+            const unsigned long long hole = __ballot(in && !keep && j < a.budget), mover = __ballot(keep && j >= a.budget);
+            if (round) {
+                if ((hole >> lane) & 1) moves[1 + most + nh + __popcll(hole & below)] = j;
+                if ((mover >> lane) & 1) moves[1 + nm + __popcll(mover & below)] = j;
+                if (!a.in_place && keep && j < a.budget) { wo[j] = w[j]; po[j] = p[j]; }
+            }
+            nh += __popcll(hole); nm += __popcll(mover);
+        }
+        if (!round) {
+            if (lane == 0) { tot[1][wave] = nh; tot[2][wave] = nm; }
+            __syncthreads();
+            for (int i = 0; i < wave; ++i) { holes += tot[1][i]; movers += tot[2][i]; }
+        }
+    }
+    if (tid == EVICT_THREADS - 1) moves[0] = (int)nm;       // the last wave's running count is the total
+}
+// grid (chunks of moves, KV heads, sequences): a 16th of a workgroup per row, K and V; weight and pos of the row ride along
+__global__ void __launch_bounds__(256) paged_evict_move_kernel(EvictArgs a) {
+    const int h = blockIdx.y, s = blockIdx.z;
+    const int *moves = a.moves + ((long)s * a.c.n_head_kv + h) * a.list; const int count = moves[0], most = (a.list - 1) / 2;
+    const int sub = threadIdx.x & 15;
+    for (int m = blockIdx.x * 16 + (threadIdx.x >> 4); m < count; m += gridDim.x * 16) {
+        const int from = moves[1 + m], to = moves[1 + most + m];
+        if (sub == 0) {
+            slot_row<float>(a.weight_out, s, h)[to] = slot_row<const float>(a.weight, s, h)[from];
+            slot_row<int>(a.pos_out, s, h)[to] = slot_row<const int>(a.pos, s, h)[from];
+        }
+        const int pf = paged_page(a.c, s, from), pt = paged_page(a.c, s, to);
+        if (pf < 0 || pt < 0) continue;
+        const int mask = (1 << a.c.page_shift) - 1;
+        const char *ks = a.c.k + (long)pf * a.c.k_page + (long)h * a.c.k_head + (long)(from & mask) * a.c.k_row, *vs = a.c.v + (long)pf * a.c.v_page + (long)h * a.c.v_head + (long)(from & mask) * a.c.v_row;
+        char *kd = a.c.k + (long)pt * a.c.k_page + (long)h * a.c.k_head + (long)(to & mask) * a.c.k_row, *vd = a.c.v + (long)pt * a.c.v_page + (long)h * a.c.v_head + (long)(to & mask) * a.c.v_row;
+        for (int d = sub * 16; d < a.c.D * 2; d += 256) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(ks + d), y = *reinterpret_cast<const uint4 *>(vs + d);
+            *reinterpret_cast<uint4 *>(kd + d) = x; *reinterpret_cast<uint4 *>(vd + d) = y;
+        }
+    }
+}
+// at most this many rows of a (sequence, head) move: a mover lies behind the budget, a hole before it
+static long evict_most(const PagedCache &c, int budget) { return std::min<long>(budget, std::max<long>(((long)c.W << c.page_shift) - budget, 0)); }
+static int64_t evict_check(const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const cdna4_tensor *weight, const cdna4_tensor *pos, int budget, int n_sink,
+                           int n_recent, const cdna4_tensor *weight_out, const cdna4_tensor *pos_out, EvictArgs *a) {
+    ARG_CHECK(weight && pos && weight_out && pos_out, "paged_evict: null argument");
+    int rc = pg_cache_check("paged_evict", k_cache, v_cache, table, true, &a->c); if (rc) return rc;
+    if ((rc = pg_slots_check("paged_evict", "weight", weight, CDNA4_TYPE_F32, a->c, false)) || (rc = pg_slots_check("paged_evict", "pos", pos, CDNA4_TYPE_I32, a->c, false)) ||
+        (rc = pg_slots_check("paged_evict", "weight_out", weight_out, CDNA4_TYPE_F32, a->c, true)) || (rc = pg_slots_check("paged_evict", "pos_out", pos_out, CDNA4_TYPE_I32, a->c, true))) return rc;
+    ARG_CHECK(budget >= 1 && n_sink >= 0 && n_recent >= 0 && (long)n_sink + n_recent <= budget, "paged_evict: 1 <= budget, 0 <= n_sink + n_recent <= budget");
+    const bool ws = pg_same(weight, weight_out), ps = pg_same(pos, pos_out);
+    ARG_CHECK(pg_empty(weight) || (ws == ps && (ws || (!pg_overlap(weight, 4, weight_out, 4) && !pg_overlap(pos, 4, pos_out, 4))) && !pg_overlap(weight_out, 4, pos, 4) &&
+              !pg_overlap(pos_out, 4, weight, 4) && !pg_overlap(weight_out, 4, pos_out, 4)), "paged_evict: weight_out and pos_out are weight and pos themselves, or memory apart from both");
+    a->in_place = ws; a->budget = budget; a->sink = n_sink; a->recent = n_recent; a->list = (int)(1 + 2 * evict_most(a->c, budget));
+    return (int64_t)a->c.n_seq * a->c.n_head_kv * a->list * 4;
+}
+int64_t cdna4_paged_evict_workspace(const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const cdna4_tensor *weight, const cdna4_tensor *pos, int budget, int n_sink,
+                                    int n_recent, const cdna4_tensor *weight_out, const cdna4_tensor *pos_out) {
+    EvictArgs a; return evict_check(k_cache, v_cache, table, weight, pos, budget, n_sink, n_recent, weight_out, pos_out, &a);
+}
+int cdna4_op_paged_evict(cdna4_context *ctx, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const int32_t *n_kv, const cdna4_tensor *weight,
+                         const cdna4_tensor *pos, const int32_t *n_past, int budget, int n_sink, int n_recent, const cdna4_tensor *weight_out, const cdna4_tensor *pos_out, int32_t *n_kv_out, void *stream) {
+    ARG_CHECK(ctx, "paged_evict: null argument");
+    EvictArgs a; const int64_t bytes = evict_check(k_cache, v_cache, table, weight, pos, budget, n_sink, n_recent, weight_out, pos_out, &a); if (bytes < 0) return (int)bytes;
+    if (a.c.n_seq == 0) return CDNA4_OK;
+    const long n = a.c.n_seq;
+    ARG_CHECK(n_kv && n_past && n_kv_out && (a.c.W == 0 || (a.c.table && weight->data && pos->data && weight_out->data && pos_out->data)), "paged_evict: null data");
+    ARG_CHECK(!pg_overlap(n_kv_out, n * 4, n_kv, n * 4) && !pg_overlap(n_kv_out, n * 4, n_past, n * 4), "paged_evict: n_kv_out overlaps an input");
+    a.c.n_kv = n_kv; a.n_past = n_past; a.n_kv_out = n_kv_out;
+    a.weight = slot_view(weight); a.pos = slot_view(pos); a.weight_out = slot_view(weight_out); a.pos_out = slot_view(pos_out);
+    DEVICE_SCOPE(ctx);
+    const int rc = cdna4_ensure_ws(ctx, (size_t)bytes, (hipStream_t)stream); if (rc) return rc;
+    a.moves = (int *)ctx->ws;
+    hipLaunchKernelGGL(paged_evict_select_kernel, dim3((unsigned)a.c.n_head_kv, (unsigned)n), dim3(EVICT_THREADS), 0, (hipStream_t)stream, a);
+    HIP_TRY(hipGetLastError());
+    const long most = evict_most(a.c, budget);
+    if (most == 0) return CDNA4_OK;
+    const unsigned gx = (unsigned)std::min<long>((most + 15) / 16, 64);
+    hipLaunchKernelGGL(paged_evict_move_kernel, dim3(gx, (unsigned)a.c.n_head_kv, (unsigned)n), dim3(256), 0, (hipStream_t)stream, a);
+    HIP_TRY(hipGetLastError()); return CDNA4_OK;
+}

@@ -355,6 +355,59 @@ CDNA4_API int cdna4_op_moe_router(cdna4_context *ctx, const cdna4_tensor *w, con
 CDNA4_API int cdna4_op_moe_router_norm(cdna4_context *ctx, const cdna4_tensor *w, const cdna4_tensor *x, const cdna4_tensor *norm_w, float norm_eps, const cdna4_tensor *x_normed, const cdna4_tensor *logits,
                                        const cdna4_tensor *probs, const cdna4_tensor *sorted, const cdna4_tensor *wsel, const cdna4_tensor *wsum, const cdna4_tensor *wnorm, int n_used, void *stream);
 
+/* ---- decoding over a paged key / value cache ---------------------------------------------------------------
+ * Many sequences share one pool of pages; what a sequence holds is a row of a page table.  No reference counterpart (the reference keeps one contiguous cache per context and masks
+ * the cells of other sequences, llama.cpp llama_kv_cache); the arithmetic of the attention is FLASH_ATTN_EXT's (ggml.c:22874-23160) for one new token per sequence.
+ *   k_cache, v_cache : f16 or bf16 (both the same) [D, page, n_head_kv, n_pages], any strides that are multiples of 16 bytes with dense rows; D = 64, 128 or 256; page a power of two
+ *                      in 16 ... 4096.  Token-major pages ([D, n_head_kv, page, n_pages] in memory) are the same descriptor with other strides.
+ *   table            : i32 [W, n_seq]: slot j of sequence s is row j % page of page table[s][j / page].  An id outside [0, n_pages) marks an unmapped page: its slots are not read,
+ *                      written or attended to.
+ *   n_kv             : i32 [n_seq] ON THE DEVICE: slots in use, so that a captured graph serves growing sequences.  Values above W * page count as W * page; a negative value marks an
+ *                      inactive row of a padded batch (nothing is stored or moved, the attention row is 0, the value passes through to n_kv_out).
+ *   weight, pos      : f32 / i32 [>= W * page, n_head_kv, n_seq]: per slot and KV head, the attention weight that the slot has gathered and the position of its token (the heads keep
+ *                      different tokens after an eviction).
+ * Attention does not depend on the order of the slots (K is rotated before it is stored), so evictions leave the slots of a sequence in disorder and pos says which token is where.
+ * n_seq, W * page: at most 8192 and 2^30.  n_kv_out may not overlap n_kv.  Errors: CDNA4_E_INVALID null / inconsistent arguments, CDNA4_E_UNSUPPORTED shapes and types outside the
+ * above, CDNA4_E_NOMEM a workspace that would have to grow during stream capture: reserve the largest cdna4_paged_*_workspace / cdna4_beam_select_workspace beforehand.  Those
+ * functions run the same checks and return the bytes, or the error; they need no device. */
+
+/* New tokens into the cache: token i of sequence s (start[s] <= i < start[s + 1]; start NULL: token i belongs to sequence i and n_tok == n_seq) goes to slot n_kv[s] + i - start[s]; its
+ * f32 K and V rows ([D, n_head_kv, n_tok], after rope) are rounded once to the cache type, weight (or NULL) becomes 0 and pos (or NULL; needs n_past) n_past[s] + i - start[s] at the
+ * slot.  n_kv_out[s] = min(n_kv[s] + tokens of s, W * page) unless NULL.  Tokens beyond the last page, on an unmapped page or outside start are dropped.  Two sequences that append
+ * must not share the page they append to (cdna4_op_paged_fork copies it). */
+CDNA4_API int cdna4_op_paged_store(cdna4_context *ctx, const cdna4_tensor *k, const cdna4_tensor *v, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table,
+                                   const int32_t *n_kv, const int32_t *start, const int32_t *n_past, const cdna4_tensor *weight, const cdna4_tensor *pos, int32_t *n_kv_out, void *stream);
+/* Attention of one new token per sequence: q f32 [D, n_head, n_seq] -> dst f32 [D, n_head, n_seq]; n_head a multiple of n_head_kv.  scores = scale * q.k, softcap != 0:
+ * softcap * tanh(scores / softcap); softmax over the mapped slots j < n_kv[s].  A sequence with nothing to attend to gets a row of zeros.  weight (or NULL): weight[s][hk][j] += the sum of
+ * the slot's probabilities over the query heads of hk, every element by one thread in a fixed order.  Results do not depend on the run.  Slots that are not attended to may hold
+ * anything (infinities and NaN included); those that are hold finite values. */
+CDNA4_API int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const int32_t *n_kv,
+                                  const cdna4_tensor *weight, const cdna4_tensor *dst, float scale, float softcap, void *stream);
+CDNA4_API int64_t cdna4_paged_attn_workspace(const cdna4_tensor *q, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const cdna4_tensor *weight,
+                                             const cdna4_tensor *dst);
+/* Eviction by gathered attention weight: every (sequence, KV head) with more than `budget` slots keeps `budget` of them: first the held ones (pos < n_sink or
+ * pos >= n_past[s] - n_recent; all alike), then by descending weight (NaN counts as -inf), ties to the lower slot.  Kept slots at budget and above move, in ascending order, into the freed slots
+ * below, in ascending order: K and V rows in the cache, weight and pos into weight_out / pos_out (either the very tensors weight / pos, or memory apart from both; values of slots at
+ * n_kv_out[s] and above are left as they were).  n_kv_out[s] = min(n_kv[s], budget).  budget >= 1, n_sink + n_recent <= budget.  The pages must belong to their sequence alone. */
+CDNA4_API int cdna4_op_paged_evict(cdna4_context *ctx, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const int32_t *n_kv, const cdna4_tensor *weight,
+                                   const cdna4_tensor *pos, const int32_t *n_past, int budget, int n_sink, int n_recent, const cdna4_tensor *weight_out, const cdna4_tensor *pos_out,
+                                   int32_t *n_kv_out, void *stream);
+CDNA4_API int64_t cdna4_paged_evict_workspace(const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const cdna4_tensor *weight, const cdna4_tensor *pos,
+                                              int budget, int n_sink, int n_recent, const cdna4_tensor *weight_out, const cdna4_tensor *pos_out);
+/* One step of a beam search: logits f32 [n_vocab, n_group * n_beam], score f32 [n_group * n_beam].  Candidate (b, t) of a group: score[b] + logits[b][t] - log sum exp logits[b]; a
+ * beam with done[b] != 0 (done: i32 or NULL) has the one candidate (b, pad) = score[b], its others are -inf.  The n_out largest of a group in descending order, ties (and candidates
+ * of -inf; NaN counts as -inf) to the lower b * n_vocab + t; the order goes by the values in 64 bits, within a beam by the logits.  score_out f32, parent i32 (a ROW: group * n_beam + b) and token i32 are
+ * [n_out, n_group], dense.  1 <= n_out <= min(64, n_beam * n_vocab), n_beam <= 256, n_beam * n_vocab < 2^31. */
+CDNA4_API int cdna4_op_beam_select(cdna4_context *ctx, const cdna4_tensor *logits, const float *score, const int32_t *done, int n_beam, int n_out, int pad, float *score_out,
+                                   int32_t *parent, int32_t *token, void *stream);
+CDNA4_API int64_t cdna4_beam_select_workspace(const cdna4_tensor *logits, int n_beam, int n_out, int pad);
+/* Sequences go on from others: row i of table_out [W, n_out] = the pages of row parent[i] of table; if its last page is cut (n_kv % page != 0) the rows in use are copied into page
+ * fresh[i], which takes its place, so that the rows that share a past append apart; entries behind are -1.  n_kv_out[i] = n_kv[parent[i]] (at most W * page).  A parent outside
+ * [0, n_seq) or an inactive one gives an inactive row (-1 everywhere); a fresh page outside [0, n_pages) leaves the cut page unmapped.  Fresh pages are distinct and in no row of
+ * table.  table_out may not overlap table. */
+CDNA4_API int cdna4_op_paged_fork(cdna4_context *ctx, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const int32_t *n_kv, const int32_t *parent,
+                                  const int32_t *fresh, const cdna4_tensor *table_out, int32_t *n_kv_out, void *stream);
+
 /* ---- run-time repack to the row-interleaved layouts (a8) ------------------------------------------------
  * replaces iqk_repack_tensor (iqk_quantize.cpp:8535-8582): base type -> *_R4, on the device, out of place.
  * nrows % 4 == 0; row stride is unchanged. */
