@@ -1,63 +1,341 @@
 // paged_attn.hip -- attention of one new token per sequence over a paged key / value cache.
+//
+// z[h][j] = scale q[h].k[j] (soft-capped), o[h] = sum_j softmax(z[h])[j] v[j]; the query heads of a KV head read the same rows, so the cache is read once per group of 16 heads and the
+// operator is bound by that read (4 D bytes a slot and KV head against 4 D flops a query head).  Three things follow:
+//
+// * Matrix instructions, for any group size: 32 slots are one step of v_mfma_f32_16x16x32.  S^T = K Q^T puts a query head into every lane column and four slots into every lane, which is
+//   the operand layout that O^T = V^T P^T wants for P: the probabilities never leave their registers, and the running maximum and sum of a head are scalars of a lane.  V arrives as rows
+//   (16 bytes a lane, a row per 16 lanes) and becomes the other operand by v_perm, so the loop touches no LDS at all.
+// * f32 results from 16-bit operands: q and p are split into two f16 (2^-22; q scaled by a power of two, p by 2^8) or three bf16 (exactly 24 bits) terms, K and V are what the cache
+//   holds; products and sums are f32.  The extra matrix instructions stay far below the load time (32 or 48 of 16 clk per 16 KB and SIMD).
+// * Equal shares: all tiles of 128 slots of all (sequence, KV head, 16 query heads) units are numbered through, and every workgroup takes an equal contiguous range of the numbers, from
+//   the lengths as they are on the device.  A long sequence in a batch of short ones spreads over the chip by itself; a workgroup that covers a unit alone writes its result, the others
+//   leave (max, sum, accumulator) for the join.
 #include "paged.cuh"
 #include "fa_decode.cuh"
+#include <algorithm>
 #include <cmath>
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr int TILE = 128, WAVES = 4, QH = 16;         // slots of a workgroup's tile (32 a wave), waves, query heads of a unit
 
 struct AttnArgs {
     PagedCache c; const char *q; long q_head, q_seq; char *dst; long d_head, d_seq; char *weight; long w_head, w_seq;
-    int group; float scale, softcap;
+    int group, n_head, n_unit, n_wg; float scale, softcap;          // n_unit: (KV head, 16 query heads) pairs of a sequence; n_wg: workgroups that share the tiles
+    int *prefix;                // [n_seq + 1] tiles of a unit before sequence s
+    float *part;                // [n_wg][2][QH][D + 2]: what a workgroup leaves of its first / last unit (max, sum, accumulator of every head)
+    float2 *stat;               // [n_seq][n_head] max and sum of a row (weight only)
+    float *score; long score_row;   // [n_seq][n_head][score_row] scores in units of log 2 (weight only)
 };
-template <bool BF16> static __device__ __forceinline__ float cache_f32(const char *p) {
-    const uint32_t b = *reinterpret_cast<const uint16_t *>(p);
-    return BF16 ? bf16_bits_to_float(b) : half_bits_to_float(b);
+
+template <bool BF16> static __device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
+    if constexpr (BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
-// One workgroup per (KV head, sequence), its query heads one after the other; a wave takes every fourth slot, a lane D / 64 elements of the row.
-template <bool BF16> __global__ void __launch_bounds__(256) paged_attn_kernel(AttnArgs a) {
-    __shared__ float s_m[4], s_l[4], s_o[4][256];
-    const int hk = blockIdx.x, s = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, E = a.c.D / 64;
-    const int n = paged_len(a.c, s), mask = (1 << a.c.page_shift) - 1;
-    auto score = [&](const float *q, int j, int page) {
-        const char *kr = a.c.k + (long)page * a.c.k_page + (long)hk * a.c.k_head + (long)(j & mask) * a.c.k_row;
-        float d = 0.f;
-        for (int e = 0; e < E; ++e) d = fmaf(q[e], cache_f32<BF16>(kr + 2 * (lane * E + e)), d);
-        d = wave_sum_dpp(d) * a.scale;
-        return a.softcap != 0.f ? a.softcap * tanhf(d / a.softcap) : d;
-    };
-    for (int g = 0; g < a.group; ++g) {
-        const int h = hk * a.group + g;
-        float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-        for (int e = 0; e < E; ++e) q[e] = reinterpret_cast<const float *>(a.q + (long)s * a.q_seq + (long)h * a.q_head)[lane * E + e];
-        for (int j = wave; j < n; j += 4) {
-            const int page = paged_page(a.c, s, j); if (page < 0) continue;
-            const float x = score(q, j, page), mn = fmaxf(m, x), f = expf(m - mn), p = expf(x - mn);
-            const char *vr = a.c.v + (long)page * a.c.v_page + (long)hk * a.c.v_head + (long)(j & mask) * a.c.v_row;
-            l = l * f + p; m = mn;
-            for (int e = 0; e < E; ++e) o[e] = fmaf(p, cache_f32<BF16>(vr + 2 * (lane * E + e)), o[e] * f);
+// max / sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48 (the slots of one query head)
+template <typename F> static __device__ __forceinline__ float over_rows(float v, F f) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+// the two / three 16-bit terms of a pair of f32 values, packed (first value in the low half)
+template <bool BF16> struct Split;
+template <> struct Split<false> {
+    static constexpr int N = 2;
+    static __device__ __forceinline__ void of(float a, float b, uint32_t (&t)[2]) {
+        t[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));          // towards zero: the remainders are exact and of the values' sign
+        const float ra = a - half_bits_to_float(t[0] & 0xffffu), rb = b - half_bits_to_float(t[0] >> 16);
+        t[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
+    }
+};
+template <> struct Split<true> {
+    static constexpr int N = 3;
+    static __device__ __forceinline__ void of(float a, float b, uint32_t (&t)[3]) {      // 24 significant bits = three times 8: exact
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+            t[i] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+            a -= __uint_as_float(x & 0xffff0000u); b -= __uint_as_float(y & 0xffff0000u);
+        }
+    }
+};
+
+// prefix sums of the sequences' tiles into LDS (pre[0] = 0 ... pre[n_seq]); 256 threads
+static __device__ __forceinline__ void scan_tiles(const AttnArgs &a, int *pre, int *tot) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int run = 0;
+    if (threadIdx.x == 0) pre[0] = 0;
+    for (int b = 0; b < a.c.n_seq; b += 256) {
+        const int s = b + (int)threadIdx.x;
+        int v = s < a.c.n_seq ? (paged_len(a.c, s) + TILE - 1) / TILE : 0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int y = __shfl_up(v, o, 64); if (lane >= o) v += y; }
+        if (lane == 63) tot[wave] = v;
+        __syncthreads();
+        int before = run;
+        for (int w = 0; w < wave; ++w) before += tot[w];
+        if (s < a.c.n_seq) pre[s + 1] = before + v;
+        run += tot[0] + tot[1] + tot[2] + tot[3];
+        __syncthreads();
+    }
+}
+static __device__ __forceinline__ long share_of(int w, long total, int n_wg) { return (long)((unsigned long)w * (unsigned long)total / (unsigned)n_wg); }
+
+template <int D, bool BF16, bool CAP> __global__ void __launch_bounds__(256) paged_attn_kernel(AttnArgs a) {
+    constexpr int KC = D / 32, VW = D == 64 ? 4 : 8, VH = D == 256 ? 2 : 1, NS = Split<BF16>::N;      // K chunks of 32 elements; V elements of a lane and half; halves of 128
+    extern __shared__ int s_mem[];
+    int *pre = s_mem;
+    __shared__ int s_tot[4]; __shared__ float s_m[WAVES][QH], s_l[WAVES][QH];
+    float *s_o = reinterpret_cast<float *>(s_mem + ((a.c.n_seq + 4) & ~3));       // [WAVES][heads][D + 4]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+    scan_tiles(a, pre, s_tot);
+    const long total = (long)pre[a.c.n_seq] * a.n_unit;
+    if (blockIdx.x == 0) for (int s = threadIdx.x; s <= a.c.n_seq; s += 256) a.prefix[s] = pre[s];
+    long x = share_of(blockIdx.x, total, a.n_wg); const long x_end = share_of(blockIdx.x + 1, total, a.n_wg);
+    if (x >= x_end) return;
+    int s = 0;
+    for (int b = 0; b < a.c.n_seq; b += 64) { const int i = b + lane; s += __popcll(__ballot(i < a.c.n_seq && (long)pre[min(i, a.c.n_seq - 1) + 1] * a.n_unit <= x)); }
+    s = __builtin_amdgcn_readfirstlane(s);
+    for (bool first = true; x < x_end; first = false) {
+        while ((long)pre[s + 1] * a.n_unit <= x) ++s;
+        s = __builtin_amdgcn_readfirstlane(s);
+        const int tiles = __builtin_amdgcn_readfirstlane(pre[s + 1] - pre[s]), n = __builtin_amdgcn_readfirstlane(paged_len(a.c, s));
+        const int rem = __builtin_amdgcn_readfirstlane((int)(x - (long)pre[s] * a.n_unit)), unit = rem / tiles, tile0 = rem - unit * tiles;
+        const int ntile = (int)min((long)(tiles - tile0), x_end - x);
+        x += ntile;
+        const int blocks = (a.group + QH - 1) / QH, hk = unit / blocks, h0 = hk * a.group + (unit - hk * blocks) * QH, heads = min(QH, (hk + 1) * a.group - h0);
+        // the queries: chunk c holds elements 32 c + 8 g ... + 7 of head `col`
+        u4 q[NS][KC]; float unscale = 1.0f;
+        {
+            const float *qr = reinterpret_cast<const float *>(a.q + (long)s * a.q_seq + (long)(h0 + min(col, heads - 1)) * a.q_head) + 8 * g;
+            float4 x0[KC], x1[KC]; float top = 0.f;
+            const float pre_scale = CAP ? a.scale : a.scale * 1.44269504088896341f;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) { x0[c] = reinterpret_cast<const float4 *>(qr + 32 * c)[0]; x1[c] = reinterpret_cast<const float4 *>(qr + 32 * c)[1]; }
+            float up = 1.0f;
+            if constexpr (!BF16) {          // a power of two that puts the largest element into [2^10, 2^11): the f16 terms neither overflow nor lose bits to the smallest exponent
+#pragma unroll
+                for (int c = 0; c < KC; ++c) top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(x0[c].x), fabsf(x0[c].y)), fmaxf(fabsf(x0[c].z), fabsf(x0[c].w))),
+                                                                   fmaxf(fmaxf(fabsf(x1[c].x), fabsf(x1[c].y)), fmaxf(fabsf(x1[c].z), fabsf(x1[c].w)))));
+                top = over_rows(top, [](float p, float r) { return fmaxf(p, r); });
+                const int e = top > 0.f ? min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100), 110) : 0;
+                up = __uint_as_float((uint32_t)(127 + 10 - e) << 23); unscale = __uint_as_float((uint32_t)(127 - 10 + e) << 23);
+            }
+            unscale *= pre_scale;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const float e[8] = {x0[c].x, x0[c].y, x0[c].z, x0[c].w, x1[c].x, x1[c].y, x1[c].z, x1[c].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { uint32_t t[NS]; Split<BF16>::of(e[2 * i] * up, e[2 * i + 1] * up, t);
+#pragma unroll
+                    for (int k = 0; k < NS; ++k) q[k][c][i] = t[k]; }
+            }
+        }
+        const char *kb = a.c.k + (long)hk * a.c.k_head, *vb = a.c.v + (long)hk * a.c.v_head;
+        const int *table = a.c.table + (long)s * a.c.table_row; const int in_page = (1 << a.c.page_shift) - 1;
+        // 16 slots from j on lie in one page (pages are powers of two >= 16): its id, -1 past the end or unmapped
+        auto page_of = [&](int j) { int id = -1; if (j < n) { id = table[j >> a.c.page_shift]; if ((unsigned)id >= (unsigned)a.c.n_pages) id = -1; } return id; };
+        const uint32_t k_lane = (uint32_t)col * (uint32_t)a.c.k_row + 16u * g, v_lane = 4u * g * (uint32_t)a.c.v_row + 2u * VW * col;
+        u4 kr[2][KC]; uint32_t vr[8][VH][VW / 2];
+        // (a half that is past the end or unmapped loads page 0: in bounds, and masked below)
+        auto load_k = [&](int j, int id0, int id1) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int id = t ? id1 : id0, off = id < 0 ? 0 : (j + 16 * t) & in_page;
+                const char *p = kb + (long)max(id, 0) * a.c.k_page + (long)off * a.c.k_row;
+#pragma unroll
+                for (int c = 0; c < KC; ++c) kr[t][c] = *reinterpret_cast<const u4 *>(p + k_lane + 64 * c);
+            }
+        };
+        auto load_v = [&](int j, int id0, int id1) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int id = t ? id1 : id0, off = id < 0 ? 0 : (j + 16 * t) & in_page;
+                const char *p = vb + (long)max(id, 0) * a.c.v_page + (long)off * a.c.v_row;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int hf = 0; hf < VH; ++hf) {
+                        const char *e = p + (v_lane + (uint32_t)r * (uint32_t)a.c.v_row) + 256 * hf;
+                        if constexpr (VW == 8) { const u4 w = *reinterpret_cast<const u4 *>(e);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) vr[4 * t + r][hf][i] = w[i]; }
+                        else { const uint2 w = *reinterpret_cast<const uint2 *>(e); vr[4 * t + r][hf][0] = w.x; vr[4 * t + r][hf][1] = w.y; }
+                    }
+            }
+        };
+        f4 o[VH][VW];
+#pragma unroll
+        for (int hf = 0; hf < VH; ++hf)
+#pragma unroll
+            for (int i = 0; i < VW; ++i) o[hf][i] = (f4){0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;
+        int j = (tile0 * WAVES + wave) * 32; const int j_end = min((tile0 + ntile) * TILE, n);
+        int id0 = page_of(j), id1 = page_of(j + 16), nx0 = page_of(j + TILE), nx1 = page_of(j + TILE + 16);
+        float *score = a.weight ? a.score + ((long)s * a.n_head + h0 + min(col, heads - 1)) * a.score_row : nullptr;
+        if (j < j_end) { load_k(j, id0, id1); load_v(j, id0, id1); }
+        while (j < j_end) {
+            f4 z[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                z[t] = (f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < KC; ++c)
+#pragma unroll
+                    for (int k = NS - 1; k >= 0; --k) z[t] = mfma<BF16>(kr[t][c], q[k][c], z[t]);
+            }
+            const int jn = j + TILE;
+            if (jn < j_end) load_k(jn, nx0, nx1);
+            const int nn0 = page_of(jn + TILE), nn1 = page_of(jn + TILE + 16);
+            const bool whole = id0 >= 0 && id1 >= 0 && j + 32 <= n;          // (wave-uniform)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float v = z[t][r] * unscale;
+                    if constexpr (CAP) v = a.softcap * 1.44269504088896341f * tanhf(v / a.softcap);
+                    z[t][r] = v;
+                }
+            if (!whole) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) if ((t ? id1 : id0) < 0 || j + 16 * t + 4 * g + r >= n) {
+                        z[t][r] = -INFINITY;
+#pragma unroll
+                        for (int hf = 0; hf < VH; ++hf)
+#pragma unroll
+                            for (int i = 0; i < VW / 2; ++i) vr[4 * t + r][hf][i] = 0u;          // (0 times what an unused slot holds may be NaN)
+                    }
+            }
+            if (score && col < heads) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) *reinterpret_cast<f4 *>(score + j + 16 * t + 4 * g) = z[t];
+            }
+            float top = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])), fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
+            top = over_rows(top, [](float p, float r) { return fmaxf(p, r); });
+            // the reference value of the exponentials follows the maximum only when that has grown by 2^6: 2^8 p stays below 2^14 in f16
+            if (__ballot(top > m + 6.0f)) {
+                const float to = fmaxf(m, top), f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+                m = to; l *= f;
+#pragma unroll
+                for (int hf = 0; hf < VH; ++hf)
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) o[hf][i] *= f;
+            }
+            const float ref = m == -INFINITY ? 0.f : m - 8.0f;
+            uint32_t p[NS][4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(z[t][r] - ref), p1 = __builtin_amdgcn_exp2f(z[t][r + 1] - ref);
+                    l += p0 + p1;
+                    uint32_t w[NS]; Split<BF16>::of(p0, p1, w);
+#pragma unroll
+                    for (int k = 0; k < NS; ++k) p[k][2 * t + r / 2] = w[k];
+                }
+#pragma unroll
+            for (int hf = 0; hf < VH; ++hf)
+#pragma unroll
+                for (int i = 0; i < VW; ++i) {          // column i of every lane's 8 (4) elements: its 8 slots side by side
+                    const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
+                    u4 vt;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) vt[w] = __builtin_amdgcn_perm(vr[2 * w + 1][hf][i / 2], vr[2 * w][hf][i / 2], sel);
+#pragma unroll
+                    for (int k = NS - 1; k >= 0; --k) o[hf][i] = mfma<BF16>(vt, (u4){p[k][0], p[k][1], p[k][2], p[k][3]}, o[hf][i]);
+                }
+            if (jn < j_end) load_v(jn, nx0, nx1);
+            id0 = nx0; id1 = nx1; nx0 = nn0; nx1 = nn1; j = jn;
+        }
+        // the four waves' results: (m, l) through LDS, then the accumulators on the common maximum
+        l = over_rows(l, [](float p, float r) { return p + r; });
+        __syncthreads();                                                  // (the previous unit's reads of s_o are done)
+        if (g == 0) { s_m[wave][col] = m; s_l[wave][col] = l; }
+        __syncthreads();
+        const float M = fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col])), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+        if (col < heads) {
+            float *so = s_o + (wave * heads + col) * (D + 4);
+#pragma unroll
+            for (int hf = 0; hf < VH; ++hf)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int i = 0; i < VW; i += 4)      // element 128 hf + VW (4 g + r) + i
+                        *reinterpret_cast<f4 *>(so + 128 * hf + VW * (4 * g + r) + i) = (f4){o[hf][i][r] * f, o[hf][i + 1][r] * f, o[hf][i + 2][r] * f, o[hf][i + 3][r] * f};
         }
         __syncthreads();
-        if (lane == 0) { s_m[wave] = m; s_l[wave] = l; }
-        for (int e = 0; e < E; ++e) s_o[wave][lane * E + e] = o[e];
-        __syncthreads();
-        float M = -INFINITY, L = 0.f;
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, s_m[w]);
-        for (int w = 0; w < 4; ++w) L += s_m[w] == -INFINITY ? 0.f : s_l[w] * expf(s_m[w] - M);
-        float *out = reinterpret_cast<float *>(a.dst + (long)s * a.d_seq + (long)h * a.d_head);
-        for (int d = threadIdx.x; d < a.c.D; d += 256) {
-            float v = 0.f;
-            for (int w = 0; w < 4; ++w) v += s_m[w] == -INFINITY ? 0.f : s_o[w][d] * expf(s_m[w] - M);
-            out[d] = L > 0.f || L != L ? v / L : 0.f;
-        }
-        if (a.weight && M != -INFINITY) {
-            float *wr = reinterpret_cast<float *>(a.weight + (long)s * a.w_seq + (long)hk * a.w_head);
-            for (int j = wave; j < n; j += 4) {
-                const int page = paged_page(a.c, s, j); if (page < 0) continue;
-                const float x = score(q, j, page);
-                if (lane == 0) wr[j] += expf(x - M) / L;
+        const bool alone = ntile == tiles;
+        float *part = a.part + ((long)blockIdx.x * 2 + (first ? 0 : 1)) * QH * (D + 2);
+        for (int e = threadIdx.x; e < heads * D / 4; e += 256) {
+            const int h = e / (D / 4), d = (e - h * (D / 4)) * 4;
+            const float Mh = fmaxf(fmaxf(s_m[0][h], s_m[1][h]), fmaxf(s_m[2][h], s_m[3][h]));
+            float L = 0.f; f4 v = (f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                if (s_m[w][h] != -INFINITY) L += s_l[w][h] * __builtin_amdgcn_exp2f(s_m[w][h] - Mh);
+                v += *reinterpret_cast<const f4 *>(s_o + (w * heads + h) * (D + 4) + d);
+            }
+            if (alone) {
+                if (Mh == -INFINITY) v = (f4){0.f, 0.f, 0.f, 0.f}; else v /= L;
+                *reinterpret_cast<f4 *>(a.dst + (long)s * a.d_seq + (long)(h0 + h) * a.d_head + d * 4) = v;
+                if (d == 0 && a.stat) a.stat[(long)s * a.n_head + h0 + h] = make_float2(Mh, L);
+            } else {
+                float *ph = part + h * (D + 2);
+                if (d == 0) { ph[0] = Mh; ph[1] = L; }
+                ph[2 + d] = v[0]; ph[3 + d] = v[1]; ph[4 + d] = v[2]; ph[5 + d] = v[3];
             }
         }
     }
 }
-static int64_t attn_check(const cdna4_tensor *q, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const cdna4_tensor *weight, const cdna4_tensor *dst, AttnArgs *a) {
+// grid (query heads, sequences): the rows that several workgroups share, and the rows of nothing
+template <int D> __global__ void __launch_bounds__(D) paged_attn_join_kernel(AttnArgs a) {
+    const int h = blockIdx.x, s = blockIdx.y, d = threadIdx.x;
+    float *out = reinterpret_cast<float *>(a.dst + (long)s * a.d_seq + (long)h * a.d_head);
+    const int p0 = a.prefix[s], tiles = a.prefix[s + 1] - p0;
+    if (tiles == 0) { out[d] = 0.f; if (d == 0 && a.stat) a.stat[(long)s * a.n_head + h] = make_float2(-INFINITY, 0.f); return; }
+    const long total = (long)a.prefix[a.c.n_seq] * a.n_unit;
+    const int blocks = (a.group + QH - 1) / QH, hk = h / a.group, in = h - hk * a.group, unit = hk * blocks + in / QH, hh = in % QH;
+    const long x0 = (long)p0 * a.n_unit + (long)unit * tiles, x1 = x0 + tiles;
+    auto owner = [&](long x) { int w = (int)min((long)((double)x * a.n_wg / (double)total), (long)a.n_wg - 1); while (share_of(w, total, a.n_wg) > x) --w; while (share_of(w + 1, total, a.n_wg) <= x) ++w; return w; };
+    const int w0 = owner(x0), w1 = owner(x1 - 1);
+    if (w0 == w1) return;
+    // a workgroup's slot 0 is its first unit, slot 1 a later (its last) one
+    auto part = [&](int w) { return a.part + ((long)w * 2 + (share_of(w, total, a.n_wg) >= x0 ? 0 : 1)) * QH * (D + 2) + hh * (D + 2); };
+    float M = -INFINITY;
+    for (int w = w0; w <= w1; ++w) if (share_of(w, total, a.n_wg) < share_of(w + 1, total, a.n_wg)) M = fmaxf(M, part(w)[0]);
+    float L = 0.f, v = 0.f;
+    if (M != -INFINITY) for (int w = w0; w <= w1; ++w) if (share_of(w, total, a.n_wg) < share_of(w + 1, total, a.n_wg)) {
+        const float *p = part(w); const float f = p[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p[0] - M);
+        L += p[1] * f; v += p[2 + d] * f;
+    }
+    out[d] = M == -INFINITY ? 0.f : v / L;
+    if (d == 0 && a.stat) a.stat[(long)s * a.n_head + h] = make_float2(M, L);
+}
+// grid (chunks of 1024 slots, KV heads, sequences): weight[slot] += sum over the group of 2^(z - m) / l
+__global__ void __launch_bounds__(256) paged_attn_weight_kernel(AttnArgs a) {
+    const int hk = blockIdx.y, s = blockIdx.z, n = paged_len(a.c, s), j = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (blockIdx.x * 1024 >= n) return;
+    f4 sum = (f4){0.f, 0.f, 0.f, 0.f};
+    if (j < n) for (int g = 0; g < a.group; ++g) {
+        const long row = (long)s * a.n_head + hk * a.group + g; const float2 st = a.stat[row];
+        if (st.x == -INFINITY) continue;
+        const f4 z = *reinterpret_cast<const f4 *>(a.score + row * a.score_row + j);
+        const float ref = st.x - 8.0f, inv = 1.0f / st.y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(z[i] - ref) * inv;
+    }
+    float *w = reinterpret_cast<float *>(a.weight + (long)s * a.w_seq + (long)hk * a.w_head);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (j + i < n && sum[i] != 0.f) w[j + i] += sum[i];
+}
+static int attn_check(const cdna4_tensor *q, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const cdna4_tensor *weight, const cdna4_tensor *dst, AttnArgs *a) {
     ARG_CHECK(q && dst, "paged_attn: null argument");
     int rc = pg_cache_check("paged_attn", k_cache, v_cache, table, false, &a->c); if (rc) return rc;
     for (const cdna4_tensor *t : {q, dst}) {
@@ -68,16 +346,30 @@ static int64_t attn_check(const cdna4_tensor *q, const cdna4_tensor *k_cache, co
     ARG_CHECK(q->ne[1] % a->c.n_head_kv == 0, "paged_attn: n_head a multiple of n_head_kv");
     OP_CHECK(q->ne[1] <= 16384, "paged_attn: at most 16384 query heads");
     if (weight && (rc = pg_slots_check("paged_attn", "weight", weight, CDNA4_TYPE_F32, a->c, true))) return rc;
-    a->group = (int)(q->ne[1] / a->c.n_head_kv);
-    return 0;
+    a->n_head = (int)q->ne[1]; a->group = a->n_head / a->c.n_head_kv; a->n_unit = a->c.n_head_kv * ((a->group + QH - 1) / QH);
+    const long slots = (long)a->c.W << a->c.page_shift, tiles = (slots + TILE - 1) / TILE;
+    OP_CHECK(tiles * a->c.n_seq < (1l << 31) / std::max(a->n_unit, 1), "paged_attn: too many slots in all");
+    a->score_row = tiles * TILE;
+    return CDNA4_OK;
 }
+// scratch: prefix sums | partial results of the workgroups | row statistics | scores (the last two with weights only)
+struct AttnScratch { size_t part, stat, score, total; };
+static AttnScratch attn_scratch(const AttnArgs &a, bool weight, int n_wg) {
+    auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    AttnScratch s; s.part = up((size_t)(a.c.n_seq + 1) * 4);
+    s.stat = s.part + up((size_t)n_wg * 2 * QH * (a.c.D + 2) * 4);
+    s.score = s.stat + (weight ? up((size_t)a.c.n_seq * a.n_head * 8) : 0);
+    s.total = s.score + (weight ? (size_t)a.c.n_seq * a.n_head * a.score_row * 4 : 0);
+    return s;
+}
+constexpr int ATTN_MAX_WG = 1024;          // what the size function counts with (it knows no device)
 int64_t cdna4_paged_attn_workspace(const cdna4_tensor *q, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const cdna4_tensor *weight, const cdna4_tensor *dst) {
-    AttnArgs a; return attn_check(q, k_cache, v_cache, table, weight, dst, &a);
+    AttnArgs a; const int rc = attn_check(q, k_cache, v_cache, table, weight, dst, &a); return rc ? rc : (int64_t)attn_scratch(a, weight != nullptr, ATTN_MAX_WG).total;
 }
 int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const int32_t *n_kv, const cdna4_tensor *weight,
                         const cdna4_tensor *dst, float scale, float softcap, void *stream) {
     ARG_CHECK(ctx, "paged_attn: null argument");
-    AttnArgs a; const int64_t bytes = attn_check(q, k_cache, v_cache, table, weight, dst, &a); if (bytes < 0) return (int)bytes;
+    AttnArgs a; int rc = attn_check(q, k_cache, v_cache, table, weight, dst, &a); if (rc) return rc;
     if (pg_empty(q)) return CDNA4_OK;
     ARG_CHECK(n_kv && q->data && dst->data && (a.c.W == 0 || (a.c.table && (!weight || weight->data))), "paged_attn: null data");
     ARG_CHECK(!pg_overlap(q, 4, dst, 4) && (!weight || a.c.W == 0 || (!pg_overlap(weight, 4, dst, 4) && !pg_overlap(weight, 4, q, 4))), "paged_attn: q, dst and weight may not overlap");
@@ -85,8 +377,25 @@ int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_t
     a.q = (const char *)q->data; a.q_head = q->nb[1]; a.q_seq = q->nb[2]; a.dst = (char *)dst->data; a.d_head = dst->nb[1]; a.d_seq = dst->nb[2];
     a.weight = weight ? (char *)weight->data : nullptr; a.w_head = weight ? weight->nb[1] : 0; a.w_seq = weight ? weight->nb[2] : 0;
     DEVICE_SCOPE(ctx);
-    const dim3 grid((unsigned)a.c.n_head_kv, (unsigned)a.c.n_seq);
-    if (k_cache->type == CDNA4_TYPE_BF16) hipLaunchKernelGGL(paged_attn_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(paged_attn_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, a);
-    HIP_TRY(hipGetLastError()); return CDNA4_OK;
+    const long tiles = a.score_row / TILE * a.c.n_seq * a.n_unit;
+    a.n_wg = (int)std::max<long>(1, std::min<long>({tiles, (long)ctx->num_cu * (a.c.D == 256 ? 1 : 2), (long)ATTN_MAX_WG}));
+    const AttnScratch sc = attn_scratch(a, weight != nullptr, a.n_wg);
+    hipStream_t st = (hipStream_t)stream;
+    if ((rc = cdna4_ensure_ws(ctx, sc.total, st))) return rc;
+    char *ws = (char *)ctx->ws;
+    a.prefix = (int *)ws; a.part = (float *)(ws + sc.part); a.stat = weight ? (float2 *)(ws + sc.stat) : nullptr; a.score = weight ? (float *)(ws + sc.score) : nullptr;
+    const bool bf = k_cache->type == CDNA4_TYPE_BF16, cap = softcap != 0.0f;
+    const size_t lds = (size_t)((a.c.n_seq + 4) & ~3) * 4 + (size_t)WAVES * std::min(QH, a.group) * (a.c.D + 4) * 4;
+#define ATTN(D_, B_, C_) do { if (lds > 64 * 1024 && (rc = cdna4_opt_in_lds((const void *)paged_attn_kernel<D_, B_, C_>))) return rc; \
+                              hipLaunchKernelGGL((paged_attn_kernel<D_, B_, C_>), dim3((unsigned)a.n_wg), dim3(256), lds, st, a); } while (0)
+#define ATTN_D(D_) do { if (bf) { if (cap) ATTN(D_, true, true); else ATTN(D_, true, false); } else { if (cap) ATTN(D_, false, true); else ATTN(D_, false, false); } \
+                        HIP_TRY(hipGetLastError()); \
+                        hipLaunchKernelGGL(paged_attn_join_kernel<D_>, dim3((unsigned)a.n_head, (unsigned)a.c.n_seq), dim3(D_), 0, st, a); } while (0)
+    if (a.c.D == 64) ATTN_D(64); else if (a.c.D == 128) ATTN_D(128); else ATTN_D(256);
+    HIP_TRY(hipGetLastError());
+    if (weight && a.c.W) {
+        hipLaunchKernelGGL(paged_attn_weight_kernel, dim3((unsigned)((a.score_row + 1023) / 1024), (unsigned)a.c.n_head_kv, (unsigned)a.c.n_seq), dim3(256), 0, st, a);
+        HIP_TRY(hipGetLastError());
+    }
+    return CDNA4_OK;
 }
