@@ -22,6 +22,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int TILE = 128, WAVES = 4, QH = 16;         // slots of a workgroup's tile (32 a wave), waves, query heads of a unit
+constexpr int ATTN_MAX_WG = 1024;                     // most workgroups of a launch; the size function, which knows no device, counts with it
 
 struct AttnArgs {
     PagedCache c; const char *q; long q_head, q_seq; char *dst; long d_head, d_seq; char *weight; long w_head, w_seq;
@@ -84,7 +85,13 @@ static __device__ __forceinline__ void scan_tiles(const AttnArgs &a, int *pre, i
         __syncthreads();
     }
 }
-static __device__ __forceinline__ long share_of(int w, long total, int n_wg) { return (long)((unsigned long)w * (unsigned long)total / (unsigned)n_wg); }
+// the tiles of all units in n_wg contiguous ranges that differ by one at most: the first `more` workgroups take one tile more
+struct Shares {
+    int base, more;
+    __device__ Shares(int total, int n_wg) { base = total / n_wg; more = total - base * n_wg; }
+    __device__ int first(int w) const { return w * base + min(w, more); }
+    __device__ int owner(int x) const { const int cut = more * (base + 1); return x < cut ? x / (base + 1) : more + (x - cut) / base; }
+};
 
 template <int D, bool BF16, bool CAP> __global__ void __launch_bounds__(256) paged_attn_kernel(AttnArgs a) {
     constexpr int KC = D / 32, VW = D == 64 ? 4 : 8, VH = D == 256 ? 2 : 1, NS = Split<BF16>::N;      // K chunks of 32 elements; V elements of a lane and half; halves of 128
@@ -94,19 +101,19 @@ template <int D, bool BF16, bool CAP> __global__ void __launch_bounds__(256) pag
     float *s_o = reinterpret_cast<float *>(s_mem + ((a.c.n_seq + 4) & ~3));       // [WAVES][heads][D + 4]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     scan_tiles(a, pre, s_tot);
-    const long total = (long)pre[a.c.n_seq] * a.n_unit;
+    const Shares shares(pre[a.c.n_seq] * a.n_unit, a.n_wg);              // (the host has checked that tiles * units < 2^31)
     if (blockIdx.x == 0) for (int s = threadIdx.x; s <= a.c.n_seq; s += 256) a.prefix[s] = pre[s];
-    long x = share_of(blockIdx.x, total, a.n_wg); const long x_end = share_of(blockIdx.x + 1, total, a.n_wg);
+    int x = __builtin_amdgcn_readfirstlane(shares.first(blockIdx.x)); const int x_end = __builtin_amdgcn_readfirstlane(shares.first(blockIdx.x + 1));
     if (x >= x_end) return;
     int s = 0;
-    for (int b = 0; b < a.c.n_seq; b += 64) { const int i = b + lane; s += __popcll(__ballot(i < a.c.n_seq && (long)pre[min(i, a.c.n_seq - 1) + 1] * a.n_unit <= x)); }
+    for (int b = 0; b < a.c.n_seq; b += 64) { const int i = b + lane; s += __popcll(__ballot(i < a.c.n_seq && pre[min(i, a.c.n_seq - 1) + 1] * a.n_unit <= x)); }
     s = __builtin_amdgcn_readfirstlane(s);
     for (bool first = true; x < x_end; first = false) {
-        while ((long)pre[s + 1] * a.n_unit <= x) ++s;
+        while (pre[s + 1] * a.n_unit <= x) ++s;
         s = __builtin_amdgcn_readfirstlane(s);
         const int tiles = __builtin_amdgcn_readfirstlane(pre[s + 1] - pre[s]), n = __builtin_amdgcn_readfirstlane(paged_len(a.c, s));
-        const int rem = __builtin_amdgcn_readfirstlane((int)(x - (long)pre[s] * a.n_unit)), unit = rem / tiles, tile0 = rem - unit * tiles;
-        const int ntile = (int)min((long)(tiles - tile0), x_end - x);
+        const int rem = __builtin_amdgcn_readfirstlane(x - pre[s] * a.n_unit), unit = rem / tiles, tile0 = rem - unit * tiles;
+        const int ntile = min(tiles - tile0, x_end - x);
         x += ntile;
         const int blocks = (a.group + QH - 1) / QH, hk = unit / blocks, h0 = hk * a.group + (unit - hk * blocks) * QH, heads = min(QH, (hk + 1) * a.group - h0);
         // the queries: chunk c holds elements 32 c + 8 g ... + 7 of head `col`
@@ -294,29 +301,54 @@ template <int D, bool BF16, bool CAP> __global__ void __launch_bounds__(256) pag
         }
     }
 }
-// grid (query heads, sequences): the rows that several workgroups share, and the rows of nothing
-template <int D> __global__ void __launch_bounds__(D) paged_attn_join_kernel(AttnArgs a) {
-    const int h = blockIdx.x, s = blockIdx.y, d = threadIdx.x;
+// grid (query heads, sequences): the rows that several workgroups share, and the rows of nothing.  256 threads: the partial maxima and sums one to a thread, then D / 4 threads to a
+// partial accumulator and 1024 / D of those at a time.
+template <int D> __global__ void __launch_bounds__(256) paged_attn_join_kernel(AttnArgs a) {
+    __shared__ float s_f[ATTN_MAX_WG], s_red[8]; __shared__ f4 s_v[256];
+    const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     float *out = reinterpret_cast<float *>(a.dst + (long)s * a.d_seq + (long)h * a.d_head);
     const int p0 = a.prefix[s], tiles = a.prefix[s + 1] - p0;
-    if (tiles == 0) { out[d] = 0.f; if (d == 0 && a.stat) a.stat[(long)s * a.n_head + h] = make_float2(-INFINITY, 0.f); return; }
-    const long total = (long)a.prefix[a.c.n_seq] * a.n_unit;
-    const int blocks = (a.group + QH - 1) / QH, hk = h / a.group, in = h - hk * a.group, unit = hk * blocks + in / QH, hh = in % QH;
-    const long x0 = (long)p0 * a.n_unit + (long)unit * tiles, x1 = x0 + tiles;
-    auto owner = [&](long x) { int w = (int)min((long)((double)x * a.n_wg / (double)total), (long)a.n_wg - 1); while (share_of(w, total, a.n_wg) > x) --w; while (share_of(w + 1, total, a.n_wg) <= x) ++w; return w; };
-    const int w0 = owner(x0), w1 = owner(x1 - 1);
-    if (w0 == w1) return;
-    // a workgroup's slot 0 is its first unit, slot 1 a later (its last) one
-    auto part = [&](int w) { return a.part + ((long)w * 2 + (share_of(w, total, a.n_wg) >= x0 ? 0 : 1)) * QH * (D + 2) + hh * (D + 2); };
-    float M = -INFINITY;
-    for (int w = w0; w <= w1; ++w) if (share_of(w, total, a.n_wg) < share_of(w + 1, total, a.n_wg)) M = fmaxf(M, part(w)[0]);
-    float L = 0.f, v = 0.f;
-    if (M != -INFINITY) for (int w = w0; w <= w1; ++w) if (share_of(w, total, a.n_wg) < share_of(w + 1, total, a.n_wg)) {
-        const float *p = part(w); const float f = p[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p[0] - M);
-        L += p[1] * f; v += p[2 + d] * f;
+    if (tiles == 0) {
+        if (tid < D / 4) *reinterpret_cast<f4 *>(out + 4 * tid) = (f4){0.f, 0.f, 0.f, 0.f};
+        if (tid == 0 && a.stat) a.stat[(long)s * a.n_head + h] = make_float2(-INFINITY, 0.f);
+        return;
     }
-    out[d] = M == -INFINITY ? 0.f : v / L;
-    if (d == 0 && a.stat) a.stat[(long)s * a.n_head + h] = make_float2(M, L);
+    const Shares shares(a.prefix[a.c.n_seq] * a.n_unit, a.n_wg);
+    const int blocks = (a.group + QH - 1) / QH, hk = h / a.group, in = h - hk * a.group, unit = hk * blocks + in / QH, hh = in % QH;
+    const int x0 = p0 * a.n_unit + unit * tiles, w0 = shares.owner(x0), count = shares.owner(x0 + tiles - 1) - w0 + 1;
+    if (count == 1) return;
+    // a workgroup's slot 0 is its first unit, slot 1 a later (its last) one: only the first of the row's workgroups can have begun with another unit
+    const float *base = a.part + ((long)w0 * 2 * QH + hh) * (D + 2); constexpr long step = 2l * QH * (D + 2);
+    const long other = shares.first(w0) < x0 ? (long)QH * (D + 2) : 0;
+    float M = -INFINITY;
+    for (int i = tid; i < count; i += 256) { const float m = base[i * step + (i ? 0 : other)]; s_f[i] = m; M = fmaxf(M, m); }
+    M = wave_max(M);
+    if (lane == 0) s_red[wave] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+    float L = 0.f;
+    for (int i = tid; i < count; i += 256) { const float m = s_f[i], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M); s_f[i] = f; L += f * base[i * step + (i ? 0 : other) + 1]; }
+    L = wave_sum_dpp(L);
+    if (lane == 0) s_red[4 + wave] = L;
+    __syncthreads();
+    L = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
+    constexpr int TD = D / 4, ROWS = 256 / TD;
+    const int d = (tid % TD) * 4, row = tid / TD;
+    f4 v = (f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = row; i < count; i += ROWS) {
+        const float *p = base + i * step + (i ? 0 : other) + 2 + d; const float2 lo = *reinterpret_cast<const float2 *>(p), hi = *reinterpret_cast<const float2 *>(p + 2);
+        const float f = s_f[i];
+        v[0] += lo.x * f; v[1] += lo.y * f; v[2] += hi.x * f; v[3] += hi.y * f;
+    }
+    s_v[tid] = v;
+    __syncthreads();
+    if (row) return;
+#pragma unroll
+    for (int r = 1; r < ROWS; ++r) v += s_v[r * TD + tid];
+    if (M == -INFINITY) v = (f4){0.f, 0.f, 0.f, 0.f}; else v /= L;
+    *reinterpret_cast<f4 *>(out + d) = v;
+    if (tid == 0 && a.stat) a.stat[(long)s * a.n_head + h] = make_float2(M, L);
 }
 // grid (chunks of 1024 slots, KV heads, sequences): weight[slot] += sum over the group of 2^(z - m) / l
 __global__ void __launch_bounds__(256) paged_attn_weight_kernel(AttnArgs a) {
@@ -362,7 +394,6 @@ static AttnScratch attn_scratch(const AttnArgs &a, bool weight, int n_wg) {
     s.total = s.score + (weight ? (size_t)a.c.n_seq * a.n_head * a.score_row * 4 : 0);
     return s;
 }
-constexpr int ATTN_MAX_WG = 1024;          // what the size function counts with (it knows no device)
 int64_t cdna4_paged_attn_workspace(const cdna4_tensor *q, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const cdna4_tensor *weight, const cdna4_tensor *dst) {
     AttnArgs a; const int rc = attn_check(q, k_cache, v_cache, table, weight, dst, &a); return rc ? rc : (int64_t)attn_scratch(a, weight != nullptr, ATTN_MAX_WG).total;
 }
@@ -390,7 +421,7 @@ int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_t
                               hipLaunchKernelGGL((paged_attn_kernel<D_, B_, C_>), dim3((unsigned)a.n_wg), dim3(256), lds, st, a); } while (0)
 #define ATTN_D(D_) do { if (bf) { if (cap) ATTN(D_, true, true); else ATTN(D_, true, false); } else { if (cap) ATTN(D_, false, true); else ATTN(D_, false, false); } \
                         HIP_TRY(hipGetLastError()); \
-                        hipLaunchKernelGGL(paged_attn_join_kernel<D_>, dim3((unsigned)a.n_head, (unsigned)a.c.n_seq), dim3(D_), 0, st, a); } while (0)
+                        hipLaunchKernelGGL(paged_attn_join_kernel<D_>, dim3((unsigned)a.n_head, (unsigned)a.c.n_seq), dim3(256), 0, st, a); } while (0)
     if (a.c.D == 64) ATTN_D(64); else if (a.c.D == 128) ATTN_D(128); else ATTN_D(256);
     HIP_TRY(hipGetLastError());
     if (weight && a.c.W) {

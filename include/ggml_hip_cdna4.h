@@ -397,7 +397,8 @@ CDNA4_API int64_t cdna4_paged_evict_workspace(const cdna4_tensor *k_cache, const
 /* One step of a beam search: logits f32 [n_vocab, n_group * n_beam], score f32 [n_group * n_beam].  Candidate (b, t) of a group: score[b] + logits[b][t] - log sum exp logits[b]; a
  * beam with done[b] != 0 (done: i32 or NULL) has the one candidate (b, pad) = score[b], its others are -inf.  The n_out largest of a group in descending order, ties (and candidates
  * of -inf; NaN counts as -inf) to the lower b * n_vocab + t; the order goes by the values in 64 bits, within a beam by the logits.  score_out f32, parent i32 (a ROW: group * n_beam + b) and token i32 are
- * [n_out, n_group], dense.  1 <= n_out <= min(64, n_beam * n_vocab), n_beam <= 256, n_beam * n_vocab < 2^31. */
+ * [n_out, n_group], dense.  1 <= n_out <= min(64, n_beam * n_vocab), n_beam <= 256,
+ * n_beam * n_vocab <= 2^26, at most 65535 rows. */
 CDNA4_API int cdna4_op_beam_select(cdna4_context *ctx, const cdna4_tensor *logits, const float *score, const int32_t *done, int n_beam, int n_out, int pad, float *score_out,
                                    int32_t *parent, int32_t *token, void *stream);
 CDNA4_API int64_t cdna4_beam_select_workspace(const cdna4_tensor *logits, int n_beam, int n_out, int pad);

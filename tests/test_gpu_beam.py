@@ -55,6 +55,15 @@ def test_masked_tokens_finished_beams_and_rows_of_nothing(backend):
             check(backend, x, score, n_beam, n_out, np.ones(12, np.int32), pad=0)
 
 
+def test_a_stretch_of_nan_makes_a_row_of_nothing(backend):
+    r = np.random.default_rng(7)
+    for n_vocab, rows in ((20000, 4), (20000, 300)):
+        x = r.standard_normal((rows, n_vocab)).astype(np.float32)
+        x[1, 8192:16384] = np.nan; x[2, 16384:] = -np.inf; x[3, 16384:] = -np.inf; x[3, 19999] = np.nan
+        check(backend, x, np.zeros(rows, np.float32), 4, 6)
+        check(backend, x, np.zeros(rows, np.float32), 1, 6)
+
+
 def test_strides_and_many_beams(backend):
     r = np.random.default_rng(2)
     x = r.standard_normal((256, 1003)).astype(np.float32); score = -r.random(256).astype(np.float32)
