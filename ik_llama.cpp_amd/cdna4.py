@@ -1,6 +1,7 @@
 """ctypes binding of include/ggml_hip_cdna4.h (the C-ABI drop-in boundary)."""
 import ctypes as C
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 
@@ -157,7 +158,8 @@ def load_library(path=None):
     # torch ships its own libamdhip64 / librccl; whichever HIP runtime is loaded FIRST serves the whole process.  Load torch's before ours
     # so that tensors and kernels share one runtime (loading this library first made a later `import torch` see no device).
     try:
-        import torch  # noqa: F401
+        import torch
+        _DESC_TYPES.update({torch.float32: (T["F32"], 4), torch.float16: (T["F16"], 2), torch.bfloat16: (T["BF16"], 2), torch.int32: (26, 4)})
     except ImportError:
         pass
     lib = C.CDLL(p)
@@ -174,8 +176,8 @@ def load_library(path=None):
     return lib
 
 
-class _Tensor(C.Structure):      # cdna4_tensor {data, type, ne[4], nb[4]} (include/ggml_hip_cdna4.h)
-    _fields_ = [("data", C.c_void_p), ("type", C.c_int), ("ne", C.c_int64 * 4), ("nb", C.c_int64 * 4)]
+_pack_desc = struct.Struct("@Pi8q").pack          # cdna4_tensor {data, type, ne[4], nb[4]} (include/ggml_hip_cdna4.h); native alignment
+_DESC_TYPES = {}          # torch dtype -> (type id, bytes); filled by load_library, which brings torch
 
 
 class _Fusion(C.Structure):      # cdna4_fusion {norm_w, norm_eps, residual, qkv, add_b, add_dst} (include/ggml_hip_cdna4.h)
@@ -248,7 +250,7 @@ class Cdna4Backend:
             raise Cdna4Error(rc, self.lib.cdna4_last_error().decode())
 
     def _stream(self):
-        return C.c_void_p(self.torch.cuda.current_stream(self.device).cuda_stream)
+        return C.c_void_p(self.torch._C._cuda_getCurrentRawStream(self.device.index))          # (torch.cuda.current_stream(device).cuda_stream without its wrapper: 0.1 instead of 1.5 us)
 
     def description(self):
         buf = C.create_string_buffer(256); self._check(self.lib.cdna4_get_device_description(self.device.index, buf, 256))
@@ -434,26 +436,31 @@ class Cdna4Backend:
     # Caches are torch.float16 / torch.bfloat16 [n_pages, n_head_kv, page, D] views of any strides with dense rows (token-major pages: x.transpose(1, 2)), tables int32 [n_seq, W]; n_kv,
     # n_past, start, parent, fresh and done are dense int32 vectors, weight / pos float32 / int32 [n_seq, n_head_kv, >= W * page], all on the backend's device.  What the library refuses
     # raises Cdna4Error before anything is launched.
+    # These calls are short on the device (5 to 20 us), so the host's share counts: descriptors are packed into bytes (ctypes structures cost several times as much).
     def _desc(self, x, name):
-        """the ggml descriptor (sizes and byte strides from the innermost dimension out) of a torch tensor of at most 4 dimensions"""
-        types = {self.torch.float32: T["F32"], self.torch.float16: T["F16"], self.torch.bfloat16: T["BF16"], self.torch.int32: 26}
-        if not self.torch.is_tensor(x) or x.device != self.device or x.dtype not in types or not 1 <= x.dim() <= 4:
-            raise Cdna4Error(-2, "%s: a float32 / float16 / bfloat16 / int32 tensor of 1 to 4 dimensions on %s" % (name, self.device))
-        ne, nb = list(x.shape)[::-1], [s * x.element_size() for s in x.stride()][::-1]
-        for i, n in enumerate(ne):          # (torch gives dimensions of one element arbitrary strides: a dense one says the same)
-            if n == 1:
-                nb[i] = nb[i - 1] * ne[i - 1] if i else x.element_size()
-        while len(ne) < 4:
-            nb.append(nb[-1] * ne[-1]); ne.append(1)
-        return C.byref(_Tensor(x.data_ptr(), types[x.dtype], (C.c_int64 * 4)(*ne), (C.c_int64 * 4)(*nb)))
+        """cdna4_tensor {data, type, ne[4], nb[4]} of a torch tensor of at most 4 dimensions: sizes and byte strides from the innermost dimension out"""
+        t = _DESC_TYPES.get(getattr(x, "dtype", None))
+        if t is None or x.device != self.device:
+            raise Cdna4Error(-2, "%s: a float32 / float16 / bfloat16 / int32 tensor on %s" % (name, self.device))
+        ty, es = t
+        n = x.dim()
+        if n == 3:
+            (c, b, a), (r, q, p) = x.shape, x.stride()
+            return _pack_desc(x.data_ptr(), ty, a, b, c, 1, p * es, q * es, r * es, 0)
+        if n == 4:
+            (d, c, b, a), (s, r, q, p) = x.shape, x.stride()
+            return _pack_desc(x.data_ptr(), ty, a, b, c, d, p * es, q * es, r * es, s * es)
+        if n == 2:
+            (b, a), (q, p) = x.shape, x.stride()
+            return _pack_desc(x.data_ptr(), ty, a, b, 1, 1, p * es, q * es, 0, 0)
+        raise Cdna4Error(-2, "%s: 2 to 4 dimensions" % name)
 
     def _vec(self, x, name, n, dtype=None):
         """address of a dense vector of n elements (int32 unless said), None for None"""
-        dtype = dtype or self.torch.int32
         if x is None:
             return None
-        if not self.torch.is_tensor(x) or x.device != self.device or x.dtype != dtype or x.dim() < 1 or x.numel() != n or not x.is_contiguous():
-            raise Cdna4Error(-2, "%s: a dense %s vector of %d elements on %s" % (name, dtype, n, self.device))
+        if getattr(x, "dtype", None) != (dtype or self.torch.int32) or x.device != self.device or x.numel() != n or not x.is_contiguous():
+            raise Cdna4Error(-2, "%s: a dense %s vector of %d elements on %s" % (name, dtype or self.torch.int32, n, self.device))
         return x.data_ptr()
 
     def _table_rows(self, table, name="table"):
@@ -468,7 +475,7 @@ class Cdna4Backend:
         """cdna4_op_paged_store: k, v f32 [n_tok, n_head_kv, D] into the slots behind n_kv (start int32 [n_seq + 1]: token ranges of the sequences, None: one token each); returns the new n_kv."""
         n = self._table_rows(table)
         if n_kv_out is None:
-            n_kv_out = self._ints(n)
+            n_kv_out = self.torch.empty_like(n_kv)
         self._check(self.lib.cdna4_op_paged_store(self.ctx, self._desc(k, "k"), self._desc(v, "v"), self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), self._desc(table, "table"),
                                                   self._vec(n_kv, "n_kv", n), self._vec(start, "start", n + 1), self._vec(n_past, "n_past", n),
                                                   None if weight is None else self._desc(weight, "weight"), None if pos is None else self._desc(pos, "pos"),
@@ -479,7 +486,7 @@ class Cdna4Backend:
         """cdna4_op_paged_attn: q f32 [n_seq, n_head, D] -> f32 [n_seq, n_head, D]; scale None: 1 / sqrt(D); weight: += the attention weight that every slot gathers, in place."""
         qd = self._desc(q, "q")
         if out is None:
-            out = self.torch.empty(q.shape, dtype=self.torch.float32, device=self.device)
+            out = q.new_empty(q.shape)
         self._check(self.lib.cdna4_op_paged_attn(self.ctx, qd, self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), self._desc(table, "table"),
                                                  self._vec(n_kv, "n_kv", self._table_rows(table)), None if weight is None else self._desc(weight, "weight"), self._desc(out, "out"),
                                                  float(q.shape[-1] ** -0.5 if scale is None else scale), float(softcap), self._stream()))
@@ -489,7 +496,7 @@ class Cdna4Backend:
         """cdna4_op_paged_evict: every (sequence, KV head) keeps `budget` slots, by position and gathered weight; weight_out / pos_out None: in place.  Returns the new n_kv."""
         n = self._table_rows(table)
         if n_kv_out is None:
-            n_kv_out = self._ints(n)
+            n_kv_out = self.torch.empty_like(n_kv)
         self._check(self.lib.cdna4_op_paged_evict(self.ctx, self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), self._desc(table, "table"), self._vec(n_kv, "n_kv", n),
                                                   self._desc(weight, "weight"), self._desc(pos, "pos"), self._vec(n_past, "n_past", n), budget, n_sink, n_recent,
                                                   self._desc(weight if weight_out is None else weight_out, "weight_out"), self._desc(pos if pos_out is None else pos_out, "pos_out"),

@@ -34,54 +34,80 @@ static __device__ __forceinline__ u64 shfl_max(u64 k, int d) {
 struct __attribute__((packed, aligned(4))) F4a4 { float x, y, z, w; };          // rows begin at any multiple of 4 bytes
 
 // EPT logits a thread.  Owners of the bound: quads of lanes (64) for n_out <= 16, single threads above; the list holds n_out shares of either.
+// The bound is first taken on values alone, which costs a maximum and a comparison per logit (with keys of value and index all through, the launch was bound by its vector instructions:
+// 45 us for 256 rows of 128256, 131 MB).  Ties at the bound can make that list too long, and a bound of -inf says nothing: then the keys decide.
 template <int EPT> __global__ void __launch_bounds__(256) beam_scan_kernel(BeamArgs a) {
-    __shared__ u64 s_own[256], s_list[BEAM_MAX_OUT * EPT]; __shared__ float s_red[8]; __shared__ u64 s_bound; __shared__ int s_n;
+    constexpr int CAP = BEAM_MAX_OUT * EPT;
+    __shared__ u64 s_own[256], s_list[CAP]; __shared__ float s_red[8]; __shared__ u64 s_bound; __shared__ int s_n;
     const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, base = blockIdx.x * 256 * EPT;
     const float *x = reinterpret_cast<const float *>(a.logits + (long)r * a.row) + base;
     const int n = min(256 * EPT, a.n_vocab - base);
+    auto index = [&](int e) { return (e / 4 * 256 + tid) * 4 + e % 4; };
     float v[EPT];
     if (n == 256 * EPT) {
 #pragma unroll
         for (int e = 0; e < EPT / 4; ++e) { const F4a4 f = reinterpret_cast<const F4a4 *>(x)[e * 256 + tid]; v[4 * e] = f.x; v[4 * e + 1] = f.y; v[4 * e + 2] = f.z; v[4 * e + 3] = f.w; }
     } else {
 #pragma unroll
-        for (int e = 0; e < EPT; ++e) v[e] = x[min((e / 4 * 256 + tid) * 4 + e % 4, n - 1)];
+        for (int e = 0; e < EPT; ++e) { const float f = x[min(index(e), n - 1)]; v[e] = index(e) < n ? f : -INFINITY; }
     }
-    auto index = [&](int e) { return (e / 4 * 256 + tid) * 4 + e % 4; };
-    // the thread's best (the lowest index of equals: strictly larger ones replace it) and the chunk's maximum
-    float top = -INFINITY; u64 own = 0;
-    int at = -1;
+    float top = v[0];
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) { const bool in = index(e) < n; if (in && (v[e] > top || at < 0)) { at = e; } top = in ? fmaxf(top, v[e]) : top; }
-    // (a NaN first element does not hold its place against numbers: v > top then compares with -inf or with what followed)
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) if (e == at) own = logit_key(v[e], base + index(e));
+    for (int e = 1; e < EPT; ++e) top = fmaxf(top, v[e]);
+    const bool quads = a.n_out <= 16; const int owners = quads ? 64 : 256;
+    float ot = top;
+    if (quads) { ot = fmaxf(ot, fa_dpp<0xb1>(ot)); ot = fmaxf(ot, fa_dpp<0x4e>(ot)); }
+    if (!quads || (lane & 3) == 0) s_own[quads ? tid >> 2 : tid] = logit_key(ot, quads ? tid >> 2 : tid);
     const float wm = wave_max(top);
     if (lane == 0) s_red[wave] = wm;
-    if (tid == 0) { s_bound = 0; s_n = 0; }
-    const bool quads = a.n_out <= 16;
-    if (quads) { own = shfl_max(shfl_max(own, 1), 2); if ((lane & 3) == 0) s_own[tid >> 2] = own; } else s_own[tid] = own;
+    if (tid == 0) s_n = 0;
     __syncthreads();
     const float m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-    if (!quads || tid < 64) {          // the owner with n_out - 1 better ones before it
-        const u64 mine = s_own[tid]; int rank = 0; const int owners = quads ? 64 : 256;
+    if (tid < owners) {          // the owner with n_out - 1 better ones before it (owners differ in their index, so there is one)
+        const u64 mine = s_own[tid]; int rank = 0;
 #pragma unroll 8
         for (int i = 0; i < owners; ++i) rank += s_own[i] > mine;
-        if (rank == a.n_out - 1 && mine) s_bound = mine;          // (fewer owners than n_out: the bound stays 0, everything is listed)
+        if (rank == a.n_out - 1) s_bound = mine;
     }
     float l = 0.f;
+    if (m != -INFINITY) {
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) if (index(e) < n) l += m != -INFINITY ? __builtin_amdgcn_exp2f((v[e] - m) * 1.44269504088896341f) : v[e] != v[e] ? v[e] : 0.f;       // (NaN stays in the sum)
+        for (int e = 0; e < EPT; ++e) l += __builtin_amdgcn_exp2f((v[e] - m) * 1.44269504088896341f);
+    } else {
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) l += v[e] != v[e] ? v[e] : 0.f;       // (nothing but -inf and NaN: NaN stays in the sum)
+    }
     l = wave_sum_dpp(l);
     if (lane == 0) s_red[4 + wave] = l;
     __syncthreads();
-    const u64 bound = s_bound;
+    const float least = key_logit(s_bound);
+    bool by_keys = least == -INFINITY;
+    if (!by_keys) {
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) {
-        const u64 k = logit_key(v[e], base + index(e));
-        if (index(e) < n && k >= bound) s_list[atomicAdd(&s_n, 1)] = k;
+        for (int e = 0; e < EPT; ++e) if (v[e] >= least) { const int p = atomicAdd(&s_n, 1); if (p < CAP) s_list[p] = logit_key(v[e], base + index(e)); }
+        __syncthreads();
+        by_keys = s_n > CAP;
     }
-    __syncthreads();
+    if (by_keys) {          // (uniform)
+        u64 own = 0;
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) { const u64 k = index(e) < n ? logit_key(v[e], base + index(e)) : 0; own = k > own ? k : own; }
+        if (quads) own = shfl_max(shfl_max(own, 1), 2);
+        __syncthreads();
+        if (!quads || (lane & 3) == 0) s_own[quads ? tid >> 2 : tid] = own;
+        if (tid == 0) { s_n = 0; s_bound = 0; }
+        __syncthreads();
+        if (tid < owners) {
+            const u64 mine = s_own[tid]; int rank = 0;
+            for (int i = 0; i < owners; ++i) rank += s_own[i] > mine;
+            if (rank == a.n_out - 1 && mine) s_bound = mine;          // (fewer owners than n_out have logits: the bound stays 0 and everything is listed)
+        }
+        __syncthreads();
+        const u64 bound = s_bound;
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) if (index(e) < n) { const u64 k = logit_key(v[e], base + index(e)); if (k >= bound) s_list[atomicAdd(&s_n, 1)] = k; }
+        __syncthreads();
+    }
     const int count = s_n; const long row = (long)r * a.chunks + blockIdx.x;
     if (tid == 0) a.stat[row] = make_float2(m, (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]));
     for (int i = tid; i < count; i += 256) {
@@ -93,107 +119,128 @@ template <int EPT> __global__ void __launch_bounds__(256) beam_scan_kernel(BeamA
     for (int i = count + tid; i < a.n_out; i += 256) a.best[row * a.n_out + i] = 0;
 }
 
-// a candidate of a group: value descending, then beam, logit descending, token (within a beam the value grows with the logit, in 64 bits not always visibly).  b < 0: none
-struct Cand { double c; u64 key; int b; };
-static __device__ __forceinline__ bool before(const Cand &p, const Cand &q) {
-    if ((p.b < 0) != (q.b < 0)) return q.b < 0;
-    if (p.c != q.c) return p.c > q.c;
-    if (p.b != q.b) return p.b < q.b;
-    return p.key > q.key;
+// A candidate of a group in the order (value descending, beam, logit descending, token): the value's bits, ordered like the value, and the rest packed into one number (n_beam * n_vocab
+// is at most 2^26, so beam and token take 28 bits beside the logit's 32).  rest 0: none.  Within a beam the value grows with the logit, in 64 bits not always visibly.
+struct Cand { u64 value, rest; };
+static __device__ __forceinline__ u64 ordered(double c) { const u64 b = __builtin_bit_cast(u64, c); return b ^ ((b >> 63) ? ~0ull : 1ull << 63); }
+static __device__ __forceinline__ double unordered(u64 k) { return __builtin_bit_cast(double, k ^ ((k >> 63) ? 1ull << 63 : ~0ull)); }
+static __device__ __forceinline__ bool before(const Cand &p, const Cand &q) { return p.value != q.value ? p.value > q.value : p.rest > q.rest; }
+static __device__ __forceinline__ u64 quad_xor(u64 k, int d) {          // the value of lane ^ d, d = 1 or 2
+    const int lo = (int)(uint32_t)k, hi = (int)(k >> 32);
+    return d == 1 ? ((u64)(uint32_t)fa_dpp_i<0xb1>(hi) << 32) | (uint32_t)fa_dpp_i<0xb1>(lo) : ((u64)(uint32_t)fa_dpp_i<0x4e>(hi) << 32) | (uint32_t)fa_dpp_i<0x4e>(lo);
 }
-struct Cands { double c[BEAM_MAX_OUT * ((BEAM_MAX_LISTS + 255) / 256)]; u64 key[BEAM_MAX_OUT * ((BEAM_MAX_LISTS + 255) / 256)]; int b[BEAM_MAX_OUT * ((BEAM_MAX_LISTS + 255) / 256)]; };
-// how many of c[0 .. n) come before `p`: one comparison of doubles each, the rest of the order only where two are equal
-template <typename C> static __device__ __forceinline__ int rank_among(const C &s, int n, const Cand &p) {
+// how many of s[0 .. n) come before `p`, by the four lanes of a quad (all with the same p): values first, the rest of the order only where some are equal
+static __device__ __forceinline__ int rank_among(const Cand *s, int n, const Cand &p) {
     int above = 0, same = 0;
 #pragma unroll 8
-    for (int i = 0; i < n; ++i) { const double c = s.c[i]; above += c > p.c; same += c == p.c; }
+    for (int i = threadIdx.x & 3; i < n; i += 4) { const u64 v = s[i].value; above += v > p.value; same += v == p.value; }
+    same += fa_dpp_i<0xb1>(same); same += fa_dpp_i<0x4e>(same);
     if (same > 1) {
-        above = 0;
-        for (int i = 0; i < n; ++i) { const Cand q = {s.c[i], s.key[i], s.b[i]}; above += before(q, p); }
+#pragma unroll 8
+        for (int i = threadIdx.x & 3; i < n; i += 4) { const Cand q = s[i]; above += q.value == p.value && q.rest > p.rest; }
     }
+    above += fa_dpp_i<0xb1>(above); above += fa_dpp_i<0x4e>(above);
     return above;
 }
-struct Own { double c[256]; u64 key[256]; int b[256]; };
-// the k best of get(0 .. n), sorted, into out (LDS); returns how many there are.  n <= 256 * the share that Cands is made for.
-template <typename F> static __device__ __forceinline__ int choose(int n, int k, F get, Cand *out, Own &own, Cands &list, int *s_n, Cand *s_bound) {
-    const int tid = threadIdx.x;
-    Cand best = {-INFINITY, 0, -1};
-    for (int i = tid; i < n; i += 256) { const Cand q = get(i); if (before(q, best)) best = q; }
+constexpr int BEAM_LIST = BEAM_MAX_OUT * ((BEAM_MAX_LISTS + 255) / 256);
+struct JoinMem { Cand own[256], list[BEAM_LIST], bound; int n; };
+// The k best of get(0 .. n), sorted, into out (LDS); returns how many there are.  1024 threads: a quad of lanes to a candidate (ranking is the longest part: 128 + 136 comparisons of
+// 64 bits for a group of 8 beams and 16 results; with one lane to a candidate the launch took 18 us).  `first` is get(this lane's first index), n at most 256 times the share that JoinMem
+// is made for.
+static __device__ __forceinline__ int first_of_lane() { return (int)(threadIdx.x >> 2) + 256 * (int)(threadIdx.x & 3); }
+template <typename F> static __device__ __forceinline__ int choose(int n, int k, const Cand &first, F get, Cand *out, JoinMem &mem) {
+    const int quad = threadIdx.x >> 2; const bool lead = (threadIdx.x & 3) == 0;
+    Cand best = first;
+    for (int i = first_of_lane() + 1024; i < n; i += 1024) { const Cand q = get(i); if (before(q, best)) best = q; }
+#pragma unroll
+    for (int d = 1; d <= 2; ++d) { const Cand q = {quad_xor(best.value, d), quad_xor(best.rest, d)}; if (before(q, best)) best = q; }
+    if (lead) mem.own[quad] = best;
+    if (threadIdx.x == 0) { mem.n = 0; mem.bound = {0, 0}; }
     __syncthreads();
-    own.c[tid] = best.c; own.key[tid] = best.key; own.b[tid] = best.b;
-    if (tid == 0) { *s_n = 0; *s_bound = {-INFINITY, 0, 0x7fffffff}; }
-    __syncthreads();
-    if (best.b >= 0 && rank_among(own, 256, best) == k - 1) *s_bound = best;
-    __syncthreads();
-    const Cand bound = *s_bound;
-    for (int i = tid; i < n; i += 256) {
-        const Cand q = get(i);
-        if (q.b >= 0 && !before(bound, q)) { const int p = atomicAdd(s_n, 1); list.c[p] = q.c; list.key[p] = q.key; list.b[p] = q.b; }
+    const int rank = best.rest ? rank_among(mem.own, min(n, 256), best) : 256;
+    if (n <= 256) {          // one candidate a quad: its rank is its place
+        if (lead && rank < k) { out[rank] = best; atomicAdd(&mem.n, 1); }
+        __syncthreads();
+        return mem.n;
     }
+    if (lead && rank == k - 1) mem.bound = best;
     __syncthreads();
-    const int count = *s_n;
-    for (int i = tid; i < count; i += 256) { const Cand q = {list.c[i], list.key[i], list.b[i]}; const int rank = rank_among(list, count, q); if (rank < k) out[rank] = q; }
+    const Cand bound = mem.bound;
+    for (int i = threadIdx.x; i < n; i += 1024) { const Cand q = get(i); if (q.rest && !before(bound, q)) mem.list[atomicAdd(&mem.n, 1)] = q; }
+    __syncthreads();
+    const int count = mem.n;
+    for (int i = quad; i < count; i += 256) { const Cand q = mem.list[i]; const int r = rank_among(mem.list, count, q); if (lead && r < k) out[r] = q; }
     __syncthreads();
     return min(count, k);
 }
 // One workgroup per group.  Only the n_out lists with the best heads can hold any of the n_out best, and of the list with rank r among them only its first n_out - r entries.
-__global__ void __launch_bounds__(256) beam_join_kernel(BeamArgs a) {
-    __shared__ double s_top[BEAM_MAX_BEAMS], s_lse[BEAM_MAX_BEAMS]; __shared__ float s_score[BEAM_MAX_BEAMS]; __shared__ int s_kind[BEAM_MAX_BEAMS];       // 0: logits, 1: finished, 2: nothing but -inf
-    __shared__ Own own; __shared__ Cands list; __shared__ Cand s_heads[BEAM_MAX_OUT], s_best[BEAM_MAX_OUT], s_bound; __shared__ int s_n;
-    const int g = blockIdx.x, tid = threadIdx.x, k = a.n_out;
-    // 16 lanes to a beam
-    for (int b0 = 0; b0 < a.n_beam; b0 += 16) {
+// Bound by its chain of memory latencies (statistics, then the lists' entries): the heads are requested before the statistics.
+__global__ void __launch_bounds__(1024) beam_join_kernel(BeamArgs a) {
+    __shared__ float s_top[BEAM_MAX_BEAMS], s_score[BEAM_MAX_BEAMS]; __shared__ double s_lse[BEAM_MAX_BEAMS]; __shared__ int s_kind[BEAM_MAX_BEAMS];       // 0: logits, 1: finished, 2: nothing but -inf
+    __shared__ JoinMem mem; __shared__ Cand s_heads[BEAM_MAX_OUT], s_best[BEAM_MAX_OUT];
+    const int g = blockIdx.x, tid = threadIdx.x, k = a.n_out, lists = a.n_beam * a.chunks;
+    const u64 *best = a.best + (long)g * lists * k;
+    const int l1 = min(first_of_lane(), lists - 1); const u64 head = best[(long)l1 * k];
+    for (int b0 = 0; b0 < a.n_beam; b0 += 64) {          // 16 lanes to a beam
         const int b = b0 + (tid >> 4), r = g * a.n_beam + min(b, a.n_beam - 1);
-        float m = -INFINITY, l = 0.f;
-        for (int c = tid & 15; c < a.chunks; c += 16) m = fmaxf(m, a.stat[(long)r * a.chunks + c].x);
+        const float2 *stat = a.stat + (long)r * a.chunks;
+        const float score = a.score[r]; const bool done = a.done && a.done[r];
+        float m = -INFINITY, l = 0.f;          // the lane's chunks, on their own maximum
+        for (int c = tid & 15; c < a.chunks; c += 16) {
+            const float2 s = stat[c]; const float to = fmaxf(m, s.x);
+            if (to != -INFINITY) l = l * __builtin_amdgcn_exp2f((m - to) * 1.44269504088896341f) + s.y * __builtin_amdgcn_exp2f((s.x - to) * 1.44269504088896341f); else l += s.y;
+            m = to;
+        }
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-        for (int c = tid & 15; c < a.chunks; c += 16) { const float2 s = a.stat[(long)r * a.chunks + c]; l += s.x == m ? s.y : s.y * __builtin_amdgcn_exp2f((s.x - m) * 1.44269504088896341f); }
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) l += __shfl_xor(l, d, 64);
+        for (int d = 1; d < 16; d <<= 1) {
+            const float om = __shfl_xor(m, d, 64), ol = __shfl_xor(l, d, 64), to = fmaxf(m, om);
+            if (to != -INFINITY) l = l * __builtin_amdgcn_exp2f((m - to) * 1.44269504088896341f) + ol * __builtin_amdgcn_exp2f((om - to) * 1.44269504088896341f); else l += ol;
+            m = to;
+        }
         if ((tid & 15) == 0 && b < a.n_beam) {
-            const float score = a.score[r]; const bool done = a.done && a.done[r];
             s_top[b] = m; s_lse[b] = log((double)l); s_score[b] = score;
             const bool none = score != score || score == -INFINITY || (!done && (l != l || m == INFINITY || m == -INFINITY));
             s_kind[b] = none ? 2 : done ? 1 : 0;
         }
     }
     __syncthreads();
-    const int per_row = min(k, a.n_vocab);
-    // entry e of list (beam, chunk); finished beams and those of nothing have one list, made here: pad first if it counts, then tokens of -inf by their index
-    auto entry = [&](int l, int e) {
-        Cand q = {-INFINITY, 0, -1};
-        const int b = l / a.chunks, c = l - b * a.chunks, kind = s_kind[b];
-        if (kind == 0) {
-            q.key = a.best[((long)(g * a.n_beam + b) * a.chunks + c) * k + e];
-            if (q.key) {
-                q.b = b;
-                const float x = key_logit(q.key);
-                q.c = (double)s_score[b] + (((double)x - s_top[b]) - s_lse[b]);
-                if (x == -INFINITY || q.c != q.c) q.c = -INFINITY;
-            }
-        } else if (c == 0 && e < per_row) {
-            const int t = kind == 2 ? e : e == 0 ? a.pad : e - 1 < a.pad ? e - 1 : e;
-            q.b = b; q.key = logit_key(-INFINITY, t); q.c = kind == 1 && e == 0 ? (double)s_score[b] : -INFINITY;
-        }
-        return q;
+    const int per_row = min(k, a.n_vocab), t_bits = 32 - __builtin_clz(a.n_vocab), shift = __builtin_ctz(a.chunk);
+    const u64 t_mask = (1ull << t_bits) - 1;
+    auto made = [&](double c, int b, u64 key) {          // (the beam's field starts at 1, so that no candidate's rest is 0)
+        if (c != c || c == -INFINITY) { c = -INFINITY; key = logit_key(-INFINITY, key_token(key)); }
+        return Cand{ordered(c), ((u64)(a.n_beam - b) << (32 + t_bits)) | ((key >> 32) << t_bits) | (~(u64)key_token(key) & t_mask)};
     };
-    const int lists = a.n_beam * a.chunks;
-    const int heads = choose(lists, k, [&](int i) { return entry(i, 0); }, s_heads, own, list, &s_n, &s_bound);
-    auto list_of = [&](const Cand &q) {          // the chunk of a head is where its token lies
-        return q.b * a.chunks + (s_kind[q.b] ? 0 : key_token(q.key) / a.chunk);
+    auto beam_of = [&](const Cand &q) { return a.n_beam - (int)(q.rest >> (32 + t_bits)); };
+    auto token_of = [&](const Cand &q) { return (int)(~q.rest & t_mask); };
+    // entry e of list c of beam b, which is `key`; finished beams and those of nothing have one list, made here: pad first if it counts, then tokens of -inf by their index
+    auto entry = [&](int b, int c, int e, u64 key) {
+        const int kind = s_kind[b];
+        if (kind == 0) return key ? made((double)s_score[b] + (((double)key_logit(key) - (double)s_top[b]) - s_lse[b]), b, key) : Cand{0, 0};
+        if (c || e >= per_row) return Cand{0, 0};
+        const int t = kind == 2 ? e : e == 0 ? a.pad : e - 1 < a.pad ? e - 1 : e;
+        return made(kind == 1 && e == 0 ? (double)s_score[b] : -INFINITY, b, logit_key(-INFINITY, t));
     };
-    const int total = k * (k + 1) / 2;
-    const int found = choose(total, k, [&](int i) {
-        int r = (int)((sqrtf(8.0f * i + 1.0f) - 1.0f) * 0.5f);          // i = r (r + 1) / 2 + e: entry e of the list with rank k - 1 - r has e <= r
+    const int b1 = l1 / a.chunks;
+    const int heads = choose(lists, k, first_of_lane() < lists ? entry(b1, l1 - b1 * a.chunks, 0, head) : Cand{0, 0},
+                             [&](int i) { const int b = i / a.chunks; return entry(b, i - b * a.chunks, 0, best[(long)i * k]); }, s_heads, mem);
+    auto wanted = [&](int i) {          // i = r (r + 1) / 2 + e: entry e <= r of the list with rank k - 1 - r
+        int r = (int)((sqrtf(8.0f * i + 1.0f) - 1.0f) * 0.5f);
         while (r * (r + 1) / 2 > i) --r;
         while ((r + 1) * (r + 2) / 2 <= i) ++r;
         const int e = i - r * (r + 1) / 2, h = k - 1 - r;
-        return h < heads ? entry(list_of(s_heads[h]), e) : Cand{-INFINITY, 0, -1};
-    }, s_best, own, list, &s_n, &s_bound);
-    for (int i = tid; i < found; i += 256) {
+        if (h < 0 || h >= heads) return Cand{0, 0};
+        const Cand q = s_heads[h];
+        if (e == 0) return q;
+        const int b = beam_of(q), c = s_kind[b] ? 0 : token_of(q) >> shift;          // (the chunk of a head is where its token lies)
+        return entry(b, c, e, best[(long)(b * a.chunks + c) * k + e]);
+    };
+    const int total = k * (k + 1) / 2;
+    const Cand mine = first_of_lane() < total ? wanted(first_of_lane()) : Cand{0, 0};
+    __syncthreads();          // (mem is free)
+    const int found = choose(total, k, mine, wanted, s_best, mem);
+    for (int i = tid; i < found; i += 1024) {
         const Cand q = s_best[i]; const long o = (long)g * k + i;
-        a.score_out[o] = (float)q.c; a.parent[o] = g * a.n_beam + q.b; a.token[o] = key_token(q.key);
+        a.score_out[o] = (float)unordered(q.value); a.parent[o] = g * a.n_beam + beam_of(q); a.token[o] = token_of(q);
     }
 }
 static int64_t beam_check(const cdna4_tensor *x, int n_beam, int n_out, int pad, BeamArgs *a) {
@@ -210,10 +257,11 @@ static int64_t beam_check(const cdna4_tensor *x, int n_beam, int n_out, int pad,
     a->chunks = (a->n_vocab + a->chunk - 1) / a->chunk;
     return x->ne[1] * a->chunks * (8 + 8 * (int64_t)n_out);
 }
-int64_t cdna4_beam_select_workspace(const cdna4_tensor *logits, int n_beam, int n_out, int pad) { BeamArgs a; return beam_check(logits, n_beam, n_out, pad, &a); }
+int64_t cdna4_beam_select_workspace(const cdna4_tensor *logits, int n_beam, int n_out, int pad) { PG_NORM(logits, 4) BeamArgs a; return beam_check(logits, n_beam, n_out, pad, &a); }
 int cdna4_op_beam_select(cdna4_context *ctx, const cdna4_tensor *logits, const float *score, const int32_t *done, int n_beam, int n_out, int pad, float *score_out, int32_t *parent, int32_t *token,
                          void *stream) {
     ARG_CHECK(ctx, "beam_select: null argument");
+    PG_NORM(logits, 4)
     BeamArgs a; const int64_t bytes = beam_check(logits, n_beam, n_out, pad, &a); if (bytes < 0) return (int)bytes;
     const long rows = logits->ne[1], out = rows / n_beam * n_out * 4;
     if (rows == 0) return CDNA4_OK;
@@ -229,6 +277,6 @@ int cdna4_op_beam_select(cdna4_context *ctx, const cdna4_tensor *logits, const f
     if (a.chunk == BEAM_CHUNK) hipLaunchKernelGGL(beam_scan_kernel<32>, grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(beam_scan_kernel<8>, grid, dim3(256), 0, st, a);
     HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)(rows / n_beam)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)(rows / n_beam)), dim3(1024), 0, st, a);
     HIP_TRY(hipGetLastError()); return CDNA4_OK;
 }

@@ -53,12 +53,23 @@ static inline bool pg_same(const cdna4_tensor *a, const cdna4_tensor *b) {
     for (int i = 0; i < 4; ++i) if (a->ne[i] != b->ne[i] || (a->ne[i] > 1 && a->nb[i] != b->nb[i])) return false;
     return true;
 }
-static inline bool pg_sizes_ok(const cdna4_tensor *t) { for (int i = 0; i < 4; ++i) if (t->ne[i] < 0 || t->ne[i] > (1l << 40) || t->nb[i] < 0 || t->nb[i] > (1l << 46)) return false; return true; }
+static inline bool pg_sizes_ok(const cdna4_tensor *t) {                 // (no product of sizes and strides below leaves 64 bits)
+    for (int i = 0; i < 4; ++i) if (t->ne[i] < 0 || t->ne[i] > (1l << 40) || t->nb[i] < 0 || (t->ne[i] > 1 && t->nb[i] > (1l << 48) / (t->ne[i] - 1))) return false;
+    return true;
+}
 
+// a descriptor whose dimensions of one element (or none) have the strides of a dense tensor: the caller's say nothing
+static inline cdna4_tensor pg_norm(const cdna4_tensor *t, int esz) {
+    cdna4_tensor n = *t;
+    for (int i = 0; i < 4; ++i) if (n.ne[i] == 1) n.nb[i] = i ? n.nb[i - 1] * n.ne[i - 1] : esz;
+    return n;
+}
+#define PG_NORM(t, esz) cdna4_tensor t##_n; if (t) { t##_n = pg_norm(t, esz); t = &t##_n; }
 // cache + table of an operator; `written`: the operator stores into the cache.  Fills c (data pointers of an empty call may be NULL: the caller returns before it launches).
 static inline int pg_cache_check(const char *op, const cdna4_tensor *k, const cdna4_tensor *v, const cdna4_tensor *table, bool written, PagedCache *c) {
     ARG_CHECK(k && v && table, "%s: null argument", op);
     ARG_CHECK(pg_sizes_ok(k) && pg_sizes_ok(v) && pg_sizes_ok(table), "%s: sizes and strides", op);
+    PG_NORM(k, 2) PG_NORM(v, 2) PG_NORM(table, 4)
     OP_CHECK((k->type == CDNA4_TYPE_F16 || k->type == CDNA4_TYPE_BF16) && v->type == k->type, "%s: f16 or bf16 K and V caches", op);
     for (int i = 0; i < 4; ++i) ARG_CHECK(k->ne[i] == v->ne[i], "%s: K and V caches of one shape [D, page, n_head_kv, n_pages]", op);
     const long D = k->ne[0], page = k->ne[1];

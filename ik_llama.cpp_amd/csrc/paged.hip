@@ -75,6 +75,7 @@ static int new_rows_check(const char *name, const cdna4_tensor *t, const PagedCa
 int cdna4_op_paged_store(cdna4_context *ctx, const cdna4_tensor *k, const cdna4_tensor *v, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table,
                          const int32_t *n_kv, const int32_t *start, const int32_t *n_past, const cdna4_tensor *weight, const cdna4_tensor *pos, int32_t *n_kv_out, void *stream) {
     ARG_CHECK(ctx && k && v, "paged_store: null argument");
+    PG_NORM(k, 4) PG_NORM(v, 4) PG_NORM(weight, 4) PG_NORM(pos, 4)
     StoreArgs a; int rc = pg_cache_check("paged_store", k_cache, v_cache, table, true, &a.c); if (rc) return rc;
     if ((rc = new_rows_check("k", k, a.c)) || (rc = new_rows_check("v", v, a.c))) return rc;
     ARG_CHECK(k->ne[2] == v->ne[2], "paged_store: as many rows of k as of v");
@@ -126,6 +127,7 @@ __global__ void __launch_bounds__(256) paged_fork_kernel(ForkArgs a) {
 int cdna4_op_paged_fork(cdna4_context *ctx, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const int32_t *n_kv, const int32_t *parent,
                         const int32_t *fresh, const cdna4_tensor *table_out, int32_t *n_kv_out, void *stream) {
     ARG_CHECK(ctx && table_out, "paged_fork: null argument");
+    PG_NORM(table_out, 4)
     ForkArgs a; int rc = pg_cache_check("paged_fork", k_cache, v_cache, table, true, &a.c); if (rc) return rc;
     ARG_CHECK(pg_sizes_ok(table_out) && table_out->type == CDNA4_TYPE_I32 && table_out->nb[0] == 4 && table_out->nb[1] % 4 == 0 && table_out->ne[0] == a.c.W && table_out->ne[2] == 1 &&
               table_out->ne[3] == 1 && pg_disjoint_elems(table_out, 4), "paged_fork: table_out i32 [W, n_out]");
@@ -267,11 +269,13 @@ static int64_t evict_check(const cdna4_tensor *k_cache, const cdna4_tensor *v_ca
 }
 int64_t cdna4_paged_evict_workspace(const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const cdna4_tensor *weight, const cdna4_tensor *pos, int budget, int n_sink,
                                     int n_recent, const cdna4_tensor *weight_out, const cdna4_tensor *pos_out) {
+    PG_NORM(weight, 4) PG_NORM(pos, 4) PG_NORM(weight_out, 4) PG_NORM(pos_out, 4)
     EvictArgs a; return evict_check(k_cache, v_cache, table, weight, pos, budget, n_sink, n_recent, weight_out, pos_out, &a);
 }
 int cdna4_op_paged_evict(cdna4_context *ctx, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const int32_t *n_kv, const cdna4_tensor *weight,
                          const cdna4_tensor *pos, const int32_t *n_past, int budget, int n_sink, int n_recent, const cdna4_tensor *weight_out, const cdna4_tensor *pos_out, int32_t *n_kv_out, void *stream) {
     ARG_CHECK(ctx, "paged_evict: null argument");
+    PG_NORM(weight, 4) PG_NORM(pos, 4) PG_NORM(weight_out, 4) PG_NORM(pos_out, 4)
     EvictArgs a; const int64_t bytes = evict_check(k_cache, v_cache, table, weight, pos, budget, n_sink, n_recent, weight_out, pos_out, &a); if (bytes < 0) return (int)bytes;
     if (a.c.n_seq == 0) return CDNA4_OK;
     const long n = a.c.n_seq;

@@ -395,11 +395,13 @@ static AttnScratch attn_scratch(const AttnArgs &a, bool weight, int n_wg) {
     return s;
 }
 int64_t cdna4_paged_attn_workspace(const cdna4_tensor *q, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const cdna4_tensor *weight, const cdna4_tensor *dst) {
+    PG_NORM(q, 4) PG_NORM(dst, 4) PG_NORM(weight, 4)
     AttnArgs a; const int rc = attn_check(q, k_cache, v_cache, table, weight, dst, &a); return rc ? rc : (int64_t)attn_scratch(a, weight != nullptr, ATTN_MAX_WG).total;
 }
 int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const int32_t *n_kv, const cdna4_tensor *weight,
                         const cdna4_tensor *dst, float scale, float softcap, void *stream) {
     ARG_CHECK(ctx, "paged_attn: null argument");
+    PG_NORM(q, 4) PG_NORM(dst, 4) PG_NORM(weight, 4)
     AttnArgs a; int rc = attn_check(q, k_cache, v_cache, table, weight, dst, &a); if (rc) return rc;
     if (pg_empty(q)) return CDNA4_OK;
     ARG_CHECK(n_kv && q->data && dst->data && (a.c.W == 0 || (a.c.table && (!weight || weight->data))), "paged_attn: null data");

@@ -9,7 +9,11 @@ sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from conftest import load_package  # noqa: E402
 
 pkg = load_package()
-from ik_llama_cpp_amd.cdna4 import _Tensor  # noqa: E402
+
+
+class _Tensor(C.Structure):          # cdna4_tensor
+    _fields_ = [("data", C.c_void_p), ("type", C.c_int), ("ne", C.c_int64 * 4), ("nb", C.c_int64 * 4)]
+
 
 lib = pkg.load_library()
 ctx = lib.cdna4_init(0)
