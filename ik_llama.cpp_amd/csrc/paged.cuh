@@ -1,6 +1,7 @@
 // paged.cuh -- what the paged-cache operators share: the argument checks (pure host code: they run without a device) and the device view of a paged cache.
 #pragma once
 #include "api_internal.h"
+#include <atomic>
 
 #define OP_CHECK(cond, ...) do { if (!(cond)) return cdna4_set_err(CDNA4_E_UNSUPPORTED, __VA_ARGS__); } while (0)
 #define ARG_CHECK(cond, ...) do { if (!(cond)) return cdna4_set_err(CDNA4_E_INVALID, __VA_ARGS__); } while (0)
@@ -17,6 +18,15 @@ struct DeviceScope {
     }
     ~DeviceScope() { if (prev >= 0) (void)hipSetDevice(prev); }
 };
+// opt a kernel in to `bytes` of dynamic LDS beside its static LDS, once per device (function attributes belong to a device).  K: the kernel; a failed attempt is made again by the next call
+template <auto K> static inline hipError_t pg_opt_in_lds(int device, int bytes) {
+    static std::atomic<unsigned long long> done{0};
+    const unsigned long long bit = 1ull << (device & 63);
+    if (device < 64 && (done.load(std::memory_order_acquire) & bit)) return hipSuccess;
+    const hipError_t e = hipFuncSetAttribute((const void *)K, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess && device < 64) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
 #define DEVICE_SCOPE(ctx) DeviceScope device_scope_((ctx)->device); HIP_TRY(device_scope_.err)
 
 // device view of the cache: rows are addressed as 64-bit page base + 32-bit offset inside the page

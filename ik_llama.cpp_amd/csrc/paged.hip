@@ -1,5 +1,6 @@
 // paged.hip -- storing into, evicting from and forking a paged key / value cache (the attention that reads it: paged_attn.hip).
 #include "paged.cuh"
+#include "fa_decode.cuh"
 #include <algorithm>
 
 struct SlotView { char *p; long head, seq; };           // weight / pos: bytes between KV heads and sequences
@@ -159,66 +160,99 @@ static __device__ __forceinline__ uint32_t evict_key(float w, int p, int sink, l
     const uint32_t b = __float_as_uint(w + 0.0f);
     return b ^ ((b & 0x80000000u) ? 0xffffffffu : 0x80000000u);
 }
-// One workgroup per (sequence, KV head).  The budget-th largest key by four passes over 8-bit digits, then the slots in order: which kept ones lie behind the budget, which freed
-// ones before it.  Each wave owns a contiguous range of slots, so that a prefix sum over 16 wave totals is all the order takes.
-constexpr int EVICT_THREADS = 1024, EVICT_WAVES = 16;
-__global__ void __launch_bounds__(EVICT_THREADS) paged_evict_select_kernel(EvictArgs a) {
-    __shared__ unsigned hist[256], tot[3][EVICT_WAVES]; __shared__ unsigned s_digit, s_rest;
+// One workgroup per (sequence, KV head): a chain of dependent steps over n slots, so what counts is that weight and pos are read from memory once and the steps are short.
+// * The first pass turns weight and pos into keys in LDS (up to 32768; a longer row computes them again in every pass) and copies what lies before the budget to weight_out / pos_out: of
+//   those slots the freed ones are written again by the moves.
+// * The budget-th largest key by 8-bit digits: 16 copies of the histogram, by lane, since weights share few leading digits (one copy: up to 64 adds to one address); after the first
+//   digit only the keys of one bin take part.
+// * Slots in order: every wave owns a contiguous range, counts its holes (freed, before the budget) and movers (kept, behind it), and lists them behind those of the waves before it.  Ranks
+//   among equals are taken only if not all keys that equal the last kept one are kept.
+// * Few moves (`here`: at most EVICT_HERE a row, as when a cache is cut back after every few tokens) are made in the same launch from lists in LDS; otherwise the lists go to memory and a
+//   second launch moves the rows with the whole chip.
+constexpr int EVICT_THREADS = 1024, EVICT_WAVES = 16, EVICT_KEYS = 32768, EVICT_HERE = 128, EVICT_COPIES = 16;
+static __device__ __forceinline__ void evict_move(const EvictArgs &a, int s, int h, int from, int to, int sub) {          // 16 lanes to a row: K, V, weight and pos
+    if (sub == 0) {
+        slot_row<float>(a.weight_out, s, h)[to] = slot_row<const float>(a.weight, s, h)[from];
+        slot_row<int>(a.pos_out, s, h)[to] = slot_row<const int>(a.pos, s, h)[from];
+    }
+    const int pf = paged_page(a.c, s, from), pt = paged_page(a.c, s, to);
+    if (pf < 0 || pt < 0) return;
+    const int mask = (1 << a.c.page_shift) - 1;
+    const char *ks = a.c.k + (long)pf * a.c.k_page + (long)h * a.c.k_head + (long)(from & mask) * a.c.k_row, *vs = a.c.v + (long)pf * a.c.v_page + (long)h * a.c.v_head + (long)(from & mask) * a.c.v_row;
+    char *kd = a.c.k + (long)pt * a.c.k_page + (long)h * a.c.k_head + (long)(to & mask) * a.c.k_row, *vd = a.c.v + (long)pt * a.c.v_page + (long)h * a.c.v_head + (long)(to & mask) * a.c.v_row;
+    for (int d = sub * 16; d < a.c.D * 2; d += 256) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(ks + d), y = *reinterpret_cast<const uint4 *>(vs + d);
+        *reinterpret_cast<uint4 *>(kd + d) = x; *reinterpret_cast<uint4 *>(vd + d) = y;
+    }
+}
+template <bool HERE> __global__ void __launch_bounds__(EVICT_THREADS) paged_evict_select_kernel(EvictArgs a) {
+    extern __shared__ uint32_t s_key[];
+    __shared__ unsigned hist[256 * EVICT_COPIES], tot[3][EVICT_WAVES], s_digit, s_rest, s_equal; __shared__ int s_moves[HERE ? 2 * EVICT_HERE : 1];
     const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int raw = a.c.n_kv[s], n = paged_len(a.c, s);
-    int *moves = a.moves + ((long)s * a.c.n_head_kv + h) * a.list; const int most = (a.list - 1) / 2;
+    const int raw = a.c.n_kv[s], n = paged_len(a.c, s), most = (a.list - 1) / 2;
+    int *moves = HERE ? nullptr : a.moves + ((long)s * a.c.n_head_kv + h) * a.list;
     const float *w = slot_row<const float>(a.weight, s, h); const int *p = slot_row<const int>(a.pos, s, h);
     float *wo = slot_row<float>(a.weight_out, s, h); int *po = slot_row<int>(a.pos_out, s, h);
     if (h == 0 && tid == 0) a.n_kv_out[s] = raw < 0 ? raw : min(n, a.budget);
-    if (n <= a.budget) {
-        if (tid == 0) moves[0] = 0;
-        if (!a.in_place) for (int j = tid; j < n; j += EVICT_THREADS) { wo[j] = w[j]; po[j] = p[j]; }
-        return;
-    }
     const long recent_from = (long)a.n_past[s] - a.recent;
-    auto key = [&](int j) { return evict_key(w[j], p[j], a.sink, recent_from); };
+    const bool over = n > a.budget, in_lds = n <= EVICT_KEYS;
+    if (!over && (a.in_place || n == 0)) { if (!HERE && tid == 0) moves[0] = 0; return; }
+#pragma unroll 4
+    for (int j = tid; j < n; j += EVICT_THREADS) {
+        const float x = w[j]; const int y = p[j];
+        if (over && in_lds) s_key[j] = evict_key(x, y, a.sink, recent_from);
+        if (!a.in_place && j < a.budget) { wo[j] = x; po[j] = y; }
+    }
+    if (!over) { if (!HERE && tid == 0) moves[0] = 0; return; }
+    auto key = [&](int j) { return in_lds ? s_key[j] : evict_key(w[j], p[j], a.sink, recent_from); };
     uint32_t prefix = 0, rest = (uint32_t)a.budget;         // the budget-th largest key lies among those whose digits so far equal `prefix`; `rest` of them are kept
     for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
+        for (int i = tid; i < 256 * EVICT_COPIES; i += EVICT_THREADS) hist[i] = 0;
         __syncthreads();
         for (int j = tid; j < n; j += EVICT_THREADS) {
             const uint32_t x = key(j);
-            if (shift == 24 || (x >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(x >> shift) & 255], 1u);
+            if (shift == 24 || (x >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[((x >> shift) & 255) * EVICT_COPIES + (lane & (EVICT_COPIES - 1))], 1u);
         }
         __syncthreads();
-        if (wave == 0) {                                    // the digit at which the count from above reaches `rest`
-            unsigned c[4], sum = 0;
-            for (int i = 0; i < 4; ++i) { c[i] = hist[255 - (4 * lane + i)]; sum += c[i]; }
-            unsigned above = sum;
-            for (int o = 1; o < 64; o <<= 1) { const unsigned y = __shfl_up(above, o, 64); if (lane >= o) above += y; }
-            above -= sum;
-            for (int i = 0; i < 4; ++i) { if (above < rest && above + c[i] >= rest) { s_digit = 255 - (4 * lane + i); s_rest = rest - above; } above += c[i]; }
-        }
+        unsigned c = 0;                                     // four lanes to a bin, from the top bin down
+        for (int i = 0; i < EVICT_COPIES / 4; ++i) c += hist[(255 - (tid >> 2)) * EVICT_COPIES + 4 * i + (lane & 3)];
+        c += fa_dpp_i<0xb1>(c); c += fa_dpp_i<0x4e>(c);
+        unsigned above = (lane & 3) == 0 ? c : 0;           // inclusive over the wave's 16 bins
+#pragma unroll
+        for (int o = 4; o < 64; o <<= 1) { const unsigned y = __shfl_up(above, o, 64); if (lane >= o) above += y; }
+        if (lane == 60) tot[0][wave] = above;
+        __syncthreads();
+        unsigned before = 0;
+        for (int i = 0; i < wave; ++i) before += tot[0][i];
+        above += before - c;
+        if ((lane & 3) == 0 && above < rest && above + c >= rest) { s_digit = 255 - (tid >> 2); s_rest = rest - above; s_equal = c; }
         __syncthreads();
         prefix |= s_digit << shift; rest = s_rest;
-        __syncthreads();
     }
+    const bool all_equal = s_equal == rest;                 // every key that equals the last kept one is kept
     const int span = ((n + EVICT_WAVES - 1) / EVICT_WAVES + 63) & ~63, j0 = min(wave * span, n), j1 = min(j0 + span, n);
     const unsigned long long below = (1ull << lane) - 1;
-    unsigned ties = 0;
-    for (int b = j0; b < j1; b += 64) { const int j = b + lane; ties += __popcll(__ballot(j < j1 && key(min(j, n - 1)) == prefix)); }
-    if (lane == 0) tot[0][wave] = ties;
-    __syncthreads();
-    unsigned tie0 = 0; for (int i = 0; i < wave; ++i) tie0 += tot[0][i];
-    // two rounds over the wave's slots: count holes and movers, then list them
+    unsigned tie0 = 0;
+    if (!all_equal) {                                       // (uniform)
+        unsigned ties = 0;
+        for (int b = j0; b < j1; b += 64) { const int j = b + lane; ties += __popcll(__ballot(j < j1 && key(min(j, n - 1)) == prefix)); }
+        if (lane == 0) tot[1][wave] = ties;
+        __syncthreads();
+        for (int i = 0; i < wave; ++i) tie0 += tot[1][i];
+        __syncthreads();
+    }
     unsigned holes = 0, movers = 0, nh = 0, nm = 0;
-    for (int round = 0; round < 2; ++round) {
+    for (int round = 0; round < 2; ++round) {               // count, then list
         unsigned t = tie0; nh = holes; nm = movers;
         for (int b = j0; b < j1; b += 64) {
             const int j = b + lane; const bool in = j < j1; const uint32_t x = in ? key(j) : 0u;
-            const unsigned long long tie = __ballot(in && x == prefix);
-            const bool keep = in && (x > prefix || (x == prefix && t + __popcll(tie & below) < rest));
-            t += __popcll(tie);
+            bool keep = in && x >= prefix;
+            if (!all_equal) { const unsigned long long tie = __ballot(in && x == prefix); keep = in && (x > prefix || (x == prefix && t + __popcll(tie & below) < rest)); t += __popcll(tie); }
             const unsigned long long hole = __ballot(in && !keep && j < a.budget), mover = __ballot(keep && j >= a.budget);
             if (round) {
-                if ((hole >> lane) & 1) moves[1 + most + nh + __popcll(hole & below)] = j;
-                if ((mover >> lane) & 1) moves[1 + nm + __popcll(mover & below)] = j;
-                if (!a.in_place && keep && j < a.budget) { wo[j] = w[j]; po[j] = p[j]; }
+                int *list = HERE ? s_moves : moves + 1; const int half = HERE ? EVICT_HERE : most;
+                if ((hole >> lane) & 1) list[half + nh + __popcll(hole & below)] = j;
+                if ((mover >> lane) & 1) list[nm + __popcll(mover & below)] = j;
             }
             nh += __popcll(hole); nm += __popcll(mover);
         }
@@ -228,29 +262,18 @@ __global__ void __launch_bounds__(EVICT_THREADS) paged_evict_select_kernel(Evict
             for (int i = 0; i < wave; ++i) { holes += tot[1][i]; movers += tot[2][i]; }
         }
     }
-    if (tid == EVICT_THREADS - 1) moves[0] = (int)nm;       // the last wave's running count is the total
+    if constexpr (HERE) {
+        __syncthreads();
+        int count = 0;
+        for (int i = 0; i < EVICT_WAVES; ++i) count += (int)tot[2][i];
+        for (int m = tid >> 4; m < count; m += EVICT_THREADS / 16) evict_move(a, s, h, s_moves[m], s_moves[EVICT_HERE + m], tid & 15);
+    } else if (tid == EVICT_THREADS - 1) moves[0] = (int)nm;       // the last wave's running count is the total
 }
-// grid (chunks of moves, KV heads, sequences): a 16th of a workgroup per row, K and V; weight and pos of the row ride along
+// grid (chunks of moves, KV heads, sequences)
 __global__ void __launch_bounds__(256) paged_evict_move_kernel(EvictArgs a) {
     const int h = blockIdx.y, s = blockIdx.z;
     const int *moves = a.moves + ((long)s * a.c.n_head_kv + h) * a.list; const int count = moves[0], most = (a.list - 1) / 2;
-    const int sub = threadIdx.x & 15;
-    for (int m = blockIdx.x * 16 + (threadIdx.x >> 4); m < count; m += gridDim.x * 16) {
-        const int from = moves[1 + m], to = moves[1 + most + m];
-        if (sub == 0) {
-            slot_row<float>(a.weight_out, s, h)[to] = slot_row<const float>(a.weight, s, h)[from];
-            slot_row<int>(a.pos_out, s, h)[to] = slot_row<const int>(a.pos, s, h)[from];
-        }
-        const int pf = paged_page(a.c, s, from), pt = paged_page(a.c, s, to);
-        if (pf < 0 || pt < 0) continue;
-        const int mask = (1 << a.c.page_shift) - 1;
-        const char *ks = a.c.k + (long)pf * a.c.k_page + (long)h * a.c.k_head + (long)(from & mask) * a.c.k_row, *vs = a.c.v + (long)pf * a.c.v_page + (long)h * a.c.v_head + (long)(from & mask) * a.c.v_row;
-        char *kd = a.c.k + (long)pt * a.c.k_page + (long)h * a.c.k_head + (long)(to & mask) * a.c.k_row, *vd = a.c.v + (long)pt * a.c.v_page + (long)h * a.c.v_head + (long)(to & mask) * a.c.v_row;
-        for (int d = sub * 16; d < a.c.D * 2; d += 256) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(ks + d), y = *reinterpret_cast<const uint4 *>(vs + d);
-            *reinterpret_cast<uint4 *>(kd + d) = x; *reinterpret_cast<uint4 *>(vd + d) = y;
-        }
-    }
+    for (int m = blockIdx.x * 16 + (threadIdx.x >> 4); m < count; m += gridDim.x * 16) evict_move(a, s, h, moves[1 + m], moves[1 + most + m], threadIdx.x & 15);
 }
 // at most this many rows of a (sequence, head) move: a mover lies behind the budget, a hole before it
 static long evict_most(const PagedCache &c, int budget) { return std::min<long>(budget, std::max<long>(((long)c.W << c.page_shift) - budget, 0)); }
@@ -284,12 +307,19 @@ int cdna4_op_paged_evict(cdna4_context *ctx, const cdna4_tensor *k_cache, const 
     a.c.n_kv = n_kv; a.n_past = n_past; a.n_kv_out = n_kv_out;
     a.weight = slot_view(weight); a.pos = slot_view(pos); a.weight_out = slot_view(weight_out); a.pos_out = slot_view(pos_out);
     DEVICE_SCOPE(ctx);
-    const int rc = cdna4_ensure_ws(ctx, (size_t)bytes, (hipStream_t)stream); if (rc) return rc;
+    int rc = cdna4_ensure_ws(ctx, (size_t)bytes, (hipStream_t)stream); if (rc) return rc;
     a.moves = (int *)ctx->ws;
-    hipLaunchKernelGGL(paged_evict_select_kernel, dim3((unsigned)a.c.n_head_kv, (unsigned)n), dim3(EVICT_THREADS), 0, (hipStream_t)stream, a);
-    HIP_TRY(hipGetLastError());
     const long most = evict_most(a.c, budget);
-    if (most == 0) return CDNA4_OK;
+    const dim3 grid((unsigned)a.c.n_head_kv, (unsigned)n); hipStream_t st = (hipStream_t)stream;
+    const size_t lds = (size_t)std::min<long>((long)a.c.W << a.c.page_shift, EVICT_KEYS) * 4;
+    if (most <= EVICT_HERE) {
+        HIP_TRY(pg_opt_in_lds<paged_evict_select_kernel<true>>(ctx->device, EVICT_KEYS * 4));
+        hipLaunchKernelGGL(paged_evict_select_kernel<true>, grid, dim3(EVICT_THREADS), lds, st, a);
+        HIP_TRY(hipGetLastError()); return CDNA4_OK;
+    }
+    HIP_TRY(pg_opt_in_lds<paged_evict_select_kernel<false>>(ctx->device, EVICT_KEYS * 4));
+    hipLaunchKernelGGL(paged_evict_select_kernel<false>, grid, dim3(EVICT_THREADS), lds, st, a);
+    HIP_TRY(hipGetLastError());
     const unsigned gx = (unsigned)std::min<long>((most + 15) / 16, 64);
     hipLaunchKernelGGL(paged_evict_move_kernel, dim3(gx, (unsigned)a.c.n_head_kv, (unsigned)n), dim3(256), 0, (hipStream_t)stream, a);
     HIP_TRY(hipGetLastError()); return CDNA4_OK;

@@ -418,8 +418,9 @@ int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_t
     char *ws = (char *)ctx->ws;
     a.prefix = (int *)ws; a.part = (float *)(ws + sc.part); a.stat = weight ? (float2 *)(ws + sc.stat) : nullptr; a.score = weight ? (float *)(ws + sc.score) : nullptr;
     const bool bf = k_cache->type == CDNA4_TYPE_BF16, cap = softcap != 0.0f;
+    // (at most (8192 + 4) * 4 + 4 * 16 * 260 * 4 bytes < 100 KB)
     const size_t lds = (size_t)((a.c.n_seq + 4) & ~3) * 4 + (size_t)WAVES * std::min(QH, a.group) * (a.c.D + 4) * 4;
-#define ATTN(D_, B_, C_) do { if (lds > 64 * 1024 && (rc = cdna4_opt_in_lds((const void *)paged_attn_kernel<D_, B_, C_>))) return rc; \
+#define ATTN(D_, B_, C_) do { if (lds > 60 * 1024) HIP_TRY((pg_opt_in_lds<paged_attn_kernel<D_, B_, C_>>(ctx->device, 100 * 1024))); \
                               hipLaunchKernelGGL((paged_attn_kernel<D_, B_, C_>), dim3((unsigned)a.n_wg), dim3(256), lds, st, a); } while (0)
 #define ATTN_D(D_) do { if (bf) { if (cap) ATTN(D_, true, true); else ATTN(D_, true, false); } else { if (cap) ATTN(D_, false, true); else ATTN(D_, false, false); } \
                         HIP_TRY(hipGetLastError()); \

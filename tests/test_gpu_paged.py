@@ -108,6 +108,14 @@ def test_attn_long_and_many(D, dtype, backend):
     check_attn(backend, c, 16, weight=c.slots())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attn_most_lds(dtype, backend):
+    """the largest heads in groups of 16 and more, next to a long vector of lengths"""
+    for n_seq, heads in ((3, 32), (900, 16)):
+        c = Case([int(x) for x in np.random.default_rng(n_seq).integers(0, 40, n_seq)], D=256, heads_kv=1, page=16, dtype=dtype, seed=6)
+        check_attn(backend, c, heads, softcap=30.0 if n_seq == 3 else 0.0, weight=c.slots())
+
+
 def test_attn_many_sequences(backend):
     lens = [int(x) for x in np.random.default_rng(5).integers(0, 5, 700)]
     lens[477] = 700
