@@ -160,16 +160,17 @@ static __device__ __forceinline__ uint32_t evict_key(float w, int p, int sink, l
     const uint32_t b = __float_as_uint(w + 0.0f);
     return b ^ ((b & 0x80000000u) ? 0xffffffffu : 0x80000000u);
 }
-// One workgroup per (sequence, KV head): a chain of dependent steps over n slots, so what counts is that weight and pos are read from memory once and the steps are short.
-// * The first pass turns weight and pos into keys in LDS (up to 32768; a longer row computes them again in every pass) and copies what lies before the budget to weight_out / pos_out: of
-//   those slots the freed ones are written again by the moves.
-// * The budget-th largest key by 8-bit digits: 16 copies of the histogram, by lane, since weights share few leading digits (one copy: up to 64 adds to one address); after the first
-//   digit only the keys of one bin take part.
+// One workgroup per (sequence, KV head): a chain of dependent steps over n slots, so what counts is that weight and pos are read from memory once, that many of their bytes are under way at
+// a time and that the steps are few and short.
+// * The first pass (16 bytes a lane) turns weight and pos into keys in LDS (up to 32768; a longer row computes them again in every pass) and copies what lies before the budget to
+//   weight_out / pos_out: of those slots the freed ones are written again by the moves.
+// * The budget-th largest key by digits of 11, 11 and 10 bits, the first counted while the keys are made.  Two copies of the histogram by lane parity: weights share few leading digits and
+//   adds to one address follow one another.  As soon as all keys of the bin in question are kept the search is over: with weights that differ, after the second digit.
 // * Slots in order: every wave owns a contiguous range, counts its holes (freed, before the budget) and movers (kept, behind it), and lists them behind those of the waves before it.  Ranks
 //   among equals are taken only if not all keys that equal the last kept one are kept.
 // * Few moves (`here`: at most EVICT_HERE a row, as when a cache is cut back after every few tokens) are made in the same launch from lists in LDS; otherwise the lists go to memory and a
 //   second launch moves the rows with the whole chip.
-constexpr int EVICT_THREADS = 1024, EVICT_WAVES = 16, EVICT_KEYS = 32768, EVICT_HERE = 128, EVICT_COPIES = 16;
+constexpr int EVICT_THREADS = 1024, EVICT_WAVES = 16, EVICT_KEYS = 32768, EVICT_HERE = 128, EVICT_BINS = 2048, EVICT_COPIES = 2;
 static __device__ __forceinline__ void evict_move(const EvictArgs &a, int s, int h, int from, int to, int sub) {          // 16 lanes to a row: K, V, weight and pos
     if (sub == 0) {
         slot_row<float>(a.weight_out, s, h)[to] = slot_row<const float>(a.weight, s, h)[from];
@@ -185,52 +186,82 @@ static __device__ __forceinline__ void evict_move(const EvictArgs &a, int s, int
         *reinterpret_cast<uint4 *>(kd + d) = x; *reinterpret_cast<uint4 *>(vd + d) = y;
     }
 }
+struct __attribute__((packed, aligned(4))) F4u { float v[4]; };          // rows of weight / pos begin at any multiple of 4 bytes
+struct __attribute__((packed, aligned(4))) I4u { int v[4]; };
+// inclusive sum over the lanes of a wave (DPP: shifts inside rows of 16, then the rows' last lanes broadcast)
+static __device__ __forceinline__ unsigned wave_scan(unsigned v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true); v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true); v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false); v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+// sum of the totals of the waves before this one
+static __device__ __forceinline__ unsigned waves_before(const unsigned (&tot)[EVICT_WAVES], int wave) {
+    unsigned b = 0;
+#pragma unroll
+    for (int i = 0; i < EVICT_WAVES - 1; ++i) b += i < wave ? tot[i] : 0u;
+    return b;
+}
 template <bool HERE> __global__ void __launch_bounds__(EVICT_THREADS) paged_evict_select_kernel(EvictArgs a) {
     extern __shared__ uint32_t s_key[];
-    __shared__ unsigned hist[256 * EVICT_COPIES], tot[3][EVICT_WAVES], s_digit, s_rest, s_equal; __shared__ int s_moves[HERE ? 2 * EVICT_HERE : 1];
+    __shared__ unsigned hist[EVICT_BINS * EVICT_COPIES], tot[3][EVICT_WAVES], s_digit, s_rest, s_equal; __shared__ int s_moves[HERE ? 2 * EVICT_HERE : 1];
     const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int raw = a.c.n_kv[s], n = paged_len(a.c, s), most = (a.list - 1) / 2;
+    const long recent_from = (long)a.n_past[s] - a.recent;
     int *moves = HERE ? nullptr : a.moves + ((long)s * a.c.n_head_kv + h) * a.list;
     const float *w = slot_row<const float>(a.weight, s, h); const int *p = slot_row<const int>(a.pos, s, h);
     float *wo = slot_row<float>(a.weight_out, s, h); int *po = slot_row<int>(a.pos_out, s, h);
     if (h == 0 && tid == 0) a.n_kv_out[s] = raw < 0 ? raw : min(n, a.budget);
-    const long recent_from = (long)a.n_past[s] - a.recent;
     const bool over = n > a.budget, in_lds = n <= EVICT_KEYS;
     if (!over && (a.in_place || n == 0)) { if (!HERE && tid == 0) moves[0] = 0; return; }
-#pragma unroll 4
-    for (int j = tid; j < n; j += EVICT_THREADS) {
-        const float x = w[j]; const int y = p[j];
-        if (over && in_lds) s_key[j] = evict_key(x, y, a.sink, recent_from);
+    auto zero = [&]() {
+        for (int i = tid * 4; i < EVICT_BINS * EVICT_COPIES; i += EVICT_THREADS * 4) *reinterpret_cast<uint4 *>(hist + i) = make_uint4(0u, 0u, 0u, 0u);
+    };
+    auto count_digit = [&](uint32_t digit) { atomicAdd(&hist[digit * EVICT_COPIES + (lane & (EVICT_COPIES - 1))], 1u); };
+    zero();
+    __syncthreads();
+    auto take = [&](int j, float x, int y) {
+        if (over) { const uint32_t k = evict_key(x, y, a.sink, recent_from); if (in_lds) s_key[j] = k; count_digit(k >> 21); }
         if (!a.in_place && j < a.budget) { wo[j] = x; po[j] = y; }
-    }
-    if (!over) { if (!HERE && tid == 0) moves[0] = 0; return; }
-    auto key = [&](int j) { return in_lds ? s_key[j] : evict_key(w[j], p[j], a.sink, recent_from); };
-    uint32_t prefix = 0, rest = (uint32_t)a.budget;         // the budget-th largest key lies among those whose digits so far equal `prefix`; `rest` of them are kept
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256 * EVICT_COPIES; i += EVICT_THREADS) hist[i] = 0;
-        __syncthreads();
-        for (int j = tid; j < n; j += EVICT_THREADS) {
-            const uint32_t x = key(j);
-            if (shift == 24 || (x >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[((x >> shift) & 255) * EVICT_COPIES + (lane & (EVICT_COPIES - 1))], 1u);
-        }
-        __syncthreads();
-        unsigned c = 0;                                     // four lanes to a bin, from the top bin down
-        for (int i = 0; i < EVICT_COPIES / 4; ++i) c += hist[(255 - (tid >> 2)) * EVICT_COPIES + 4 * i + (lane & 3)];
-        c += fa_dpp_i<0xb1>(c); c += fa_dpp_i<0x4e>(c);
-        unsigned above = (lane & 3) == 0 ? c : 0;           // inclusive over the wave's 16 bins
+    };
+#pragma unroll 4
+    for (int j = 4 * tid; j < n - 3; j += 4 * EVICT_THREADS) {
+        const F4u x = *reinterpret_cast<const F4u *>(w + j); const I4u y = *reinterpret_cast<const I4u *>(p + j);
 #pragma unroll
-        for (int o = 4; o < 64; o <<= 1) { const unsigned y = __shfl_up(above, o, 64); if (lane >= o) above += y; }
-        if (lane == 60) tot[0][wave] = above;
-        __syncthreads();
-        unsigned before = 0;
-        for (int i = 0; i < wave; ++i) before += tot[0][i];
-        above += before - c;
-        if ((lane & 3) == 0 && above < rest && above + c >= rest) { s_digit = 255 - (tid >> 2); s_rest = rest - above; s_equal = c; }
-        __syncthreads();
-        prefix |= s_digit << shift; rest = s_rest;
+        for (int i = 0; i < 4; ++i) take(j + i, x.v[i], y.v[i]);
     }
-    const bool all_equal = s_equal == rest;                 // every key that equals the last kept one is kept
-    const int span = ((n + EVICT_WAVES - 1) / EVICT_WAVES + 63) & ~63, j0 = min(wave * span, n), j1 = min(j0 + span, n);
+    if (tid < (n & 3)) { const int j = (n & ~3) + tid; take(j, w[j], p[j]); }
+    if (!over) { if (!HERE && tid == 0) moves[0] = 0; return; }
+    __syncthreads();
+    auto key = [&](int j) { return in_lds ? s_key[j] : evict_key(w[j], p[j], a.sink, recent_from); };
+    uint32_t prefix = 0, rest = (uint32_t)a.budget; bool all_equal = false;         // the budget-th largest key lies among those that equal `prefix` so far; `rest` of them are kept
+    for (int shift = 21; ; shift = max(shift - 11, 0)) {                            // bits [21, 32), [10, 21), [0, 10)
+        const int width = shift ? 11 : 10;
+        if (shift < 21) {
+            const int high = shift + width;
+            if (in_lds) {
+#pragma unroll 8
+                for (int j = tid; j < n; j += EVICT_THREADS) { const uint32_t x = s_key[j]; if ((x >> high) == (prefix >> high)) count_digit((x >> shift) & ((1u << width) - 1)); }
+            } else
+                for (int j = tid; j < n; j += EVICT_THREADS) { const uint32_t x = key(j); if ((x >> high) == (prefix >> high)) count_digit((x >> shift) & ((1u << width) - 1)); }
+            __syncthreads();
+        }
+        // two bins a thread, from the top bin down
+        const int bin = EVICT_BINS - 2 - 2 * tid; const uint4 c4 = *reinterpret_cast<const uint4 *>(hist + bin * EVICT_COPIES);
+        const unsigned hi = c4.z + c4.w, lo = c4.x + c4.y;
+        unsigned above = wave_scan(hi + lo);
+        if (lane == 63) tot[0][wave] = above;
+        __syncthreads();
+        above += waves_before(tot[0], wave) - (hi + lo);
+        if (above < rest && above + hi >= rest) { s_digit = bin + 1; s_rest = rest - above; s_equal = hi; }
+        else if (above + hi < rest && above + hi + lo >= rest) { s_digit = bin; s_rest = rest - above - hi; s_equal = lo; }
+        zero();
+        __syncthreads();
+        prefix |= s_digit << shift; rest = s_rest; all_equal = s_equal == rest;
+        if (all_equal || shift == 0) break;
+    }
+    // kept: every key >= prefix if all of the last bin are kept, otherwise (the whole key is in prefix) the larger ones and the first `rest` of the equal ones
+    const int span = ((n + EVICT_WAVES - 1) / EVICT_WAVES + 255) & ~255, j0 = min(wave * span, n), j1 = min(j0 + span, n);
     const unsigned long long below = (1ull << lane) - 1;
     unsigned tie0 = 0;
     if (!all_equal) {                                       // (uniform)
@@ -238,33 +269,40 @@ template <bool HERE> __global__ void __launch_bounds__(EVICT_THREADS) paged_evic
         for (int b = j0; b < j1; b += 64) { const int j = b + lane; ties += __popcll(__ballot(j < j1 && key(min(j, n - 1)) == prefix)); }
         if (lane == 0) tot[1][wave] = ties;
         __syncthreads();
-        for (int i = 0; i < wave; ++i) tie0 += tot[1][i];
+        tie0 = waves_before(tot[1], wave);
         __syncthreads();
     }
     unsigned holes = 0, movers = 0, nh = 0, nm = 0;
     for (int round = 0; round < 2; ++round) {               // count, then list
         unsigned t = tie0; nh = holes; nm = movers;
-        for (int b = j0; b < j1; b += 64) {
-            const int j = b + lane; const bool in = j < j1; const uint32_t x = in ? key(j) : 0u;
-            bool keep = in && x >= prefix;
-            if (!all_equal) { const unsigned long long tie = __ballot(in && x == prefix); keep = in && (x > prefix || (x == prefix && t + __popcll(tie & below) < rest)); t += __popcll(tie); }
-            const unsigned long long hole = __ballot(in && !keep && j < a.budget), mover = __ballot(keep && j >= a.budget);
-            if (round) {
-                int *list = HERE ? s_moves : moves + 1; const int half = HERE ? EVICT_HERE : most;
-                if ((hole >> lane) & 1) list[half + nh + __popcll(hole & below)] = j;
-                if ((mover >> lane) & 1) list[nm + __popcll(mover & below)] = j;
+        for (int b = j0; b < j1; b += 256) {
+            uint32_t x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = key(min(b + 64 * u + lane, n - 1));
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int j = b + 64 * u + lane; const bool in = j < j1;
+                bool keep = in && x[u] >= prefix;
+                if (!all_equal) { const unsigned long long tie = __ballot(in && x[u] == prefix); keep = in && (x[u] > prefix || (x[u] == prefix && t + __popcll(tie & below) < rest)); t += __popcll(tie); }
+                const unsigned long long hole = __ballot(in && !keep && j < a.budget), mover = __ballot(keep && j >= a.budget);
+                if (round && (hole | mover)) {
+                    int *list = HERE ? s_moves : moves + 1; const int half = HERE ? EVICT_HERE : most;
+                    if ((hole >> lane) & 1) list[half + nh + __popcll(hole & below)] = j;
+                    if ((mover >> lane) & 1) list[nm + __popcll(mover & below)] = j;
+                }
+                nh += __popcll(hole); nm += __popcll(mover);
             }
-            nh += __popcll(hole); nm += __popcll(mover);
         }
         if (!round) {
             if (lane == 0) { tot[1][wave] = nh; tot[2][wave] = nm; }
             __syncthreads();
-            for (int i = 0; i < wave; ++i) { holes += tot[1][i]; movers += tot[2][i]; }
+            holes = waves_before(tot[1], wave); movers = waves_before(tot[2], wave);
         }
     }
     if constexpr (HERE) {
         __syncthreads();
         int count = 0;
+#pragma unroll
         for (int i = 0; i < EVICT_WAVES; ++i) count += (int)tot[2][i];
         for (int m = tid >> 4; m < count; m += EVICT_THREADS / 16) evict_move(a, s, h, s_moves[m], s_moves[EVICT_HERE + m], tid & 15);
     } else if (tid == EVICT_THREADS - 1) moves[0] = (int)nm;       // the last wave's running count is the total
