@@ -22,11 +22,12 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int TILE = 128, WAVES = 4, QH = 16;         // slots of a workgroup's tile (32 a wave), waves, query heads of a unit
+constexpr int ONE_LDS = 104 * 1024;                   // most dynamic LDS of a workgroup that has a unit to itself (and more than the others take)
 constexpr int ATTN_MAX_WG = 1024;                     // most workgroups of a launch; the size function, which knows no device, counts with it
 
 struct AttnArgs {
     PagedCache c; const char *q; long q_head, q_seq; char *dst; long d_head, d_seq; char *weight; long w_head, w_seq;
-    int group, n_head, n_unit, n_wg; float scale, softcap;          // n_unit: (KV head, 16 query heads) pairs of a sequence; n_wg: workgroups that share the tiles
+    int group, n_head, n_unit, n_wg; float scale, softcap, inv_softcap;          // n_unit: (KV head, 16 query heads) pairs of a sequence; n_wg: workgroups that share the tiles
     int *prefix;                // [n_seq + 1] tiles of a unit before sequence s
     float *part;                // [n_wg][2][QH][D + 2]: what a workgroup leaves of its first / last unit (max, sum, accumulator of every head)
     float2 *stat;               // [n_seq][n_head] max and sum of a row (weight only)
@@ -66,6 +67,15 @@ template <> struct Split<true> {
     }
 };
 
+// tanh in a dozen instructions: 1 - 2 / (e^2x + 1), whose absolute error is that of 1 (10^-7), and below 0.3 in magnitude, where the difference would lose digits, its Taylor series up to
+// x^11 (remainder 2 * 10^-9 of x).  NaN stays NaN; the library's tanhf took 960 of the 1700 cycles of a step of 32 slots of 64 elements.
+static __device__ __forceinline__ float tanh_of(float x) {
+    const float s = x * x;
+    const float small = x * fmaf(s, fmaf(s, fmaf(s, fmaf(s, fmaf(s, -1382.0f / 155925.0f, 62.0f / 2835.0f), -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+    const float large = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * 2.88539008177792681f) + 1.0f);
+    return fabsf(x) < 0.3f ? small : large;
+}
+
 // prefix sums of the sequences' tiles into LDS (pre[0] = 0 ... pre[n_seq]); 256 threads
 static __device__ __forceinline__ void scan_tiles(const AttnArgs &a, int *pre, int *tot) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -93,56 +103,41 @@ struct Shares {
     __device__ int owner(int x) const { const int cut = more * (base + 1); return x < cut ? x / (base + 1) : more + (x - cut) / base; }
 };
 
-template <int D, bool BF16, bool CAP> __global__ void __launch_bounds__(256) paged_attn_kernel(AttnArgs a) {
+// ONE: a workgroup per unit (grid: units, sequences), for tables of few slots: no shares, nothing to join, and the weights are added from scores in LDS by the same launch.
+template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds__(256) paged_attn_kernel(AttnArgs a) {
     constexpr int KC = D / 32, VW = D == 64 ? 4 : 8, VH = D == 256 ? 2 : 1, NS = Split<BF16>::N;      // K chunks of 32 elements; V elements of a lane and half; halves of 128
     extern __shared__ int s_mem[];
-    int *pre = s_mem;
-    __shared__ int s_tot[4]; __shared__ float s_m[WAVES][QH], s_l[WAVES][QH];
-    float *s_o = reinterpret_cast<float *>(s_mem + ((a.c.n_seq + 4) & ~3));       // [WAVES][heads][D + 4]
+    __shared__ int s_tot[4]; __shared__ float s_m[WAVES][QH], s_l[WAVES][QH], s_row[2][QH];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    scan_tiles(a, pre, s_tot);
-    const Shares shares(pre[a.c.n_seq] * a.n_unit, a.n_wg);              // (the host has checked that tiles * units < 2^31)
-    if (blockIdx.x == 0) for (int s = threadIdx.x; s <= a.c.n_seq; s += 256) a.prefix[s] = pre[s];
-    int x = __builtin_amdgcn_readfirstlane(shares.first(blockIdx.x)); const int x_end = __builtin_amdgcn_readfirstlane(shares.first(blockIdx.x + 1));
-    if (x >= x_end) return;
-    int s = 0;
-    for (int b = 0; b < a.c.n_seq; b += 64) { const int i = b + lane; s += __popcll(__ballot(i < a.c.n_seq && pre[min(i, a.c.n_seq - 1) + 1] * a.n_unit <= x)); }
-    s = __builtin_amdgcn_readfirstlane(s);
+    int *pre = s_mem;                                                              // prefix sums (not ONE)
+    float *s_o = reinterpret_cast<float *>(s_mem + (ONE ? 0 : (a.c.n_seq + 4) & ~3));       // [WAVES][heads][D + 4]
+    int x = 0, x_end = 1, s = 0;
+    if constexpr (!ONE) {
+        scan_tiles(a, pre, s_tot);
+        const Shares shares(pre[a.c.n_seq] * a.n_unit, a.n_wg);              // (the host has checked that tiles * units < 2^31)
+        if (blockIdx.x == 0) for (int i = threadIdx.x; i <= a.c.n_seq; i += 256) a.prefix[i] = pre[i];
+        x = __builtin_amdgcn_readfirstlane(shares.first(blockIdx.x)); x_end = __builtin_amdgcn_readfirstlane(shares.first(blockIdx.x + 1));
+        if (x >= x_end) return;
+        for (int b = 0; b < a.c.n_seq; b += 64) { const int i = b + lane; s += __popcll(__ballot(i < a.c.n_seq && pre[min(i, a.c.n_seq - 1) + 1] * a.n_unit <= x)); }
+    }
     for (bool first = true; x < x_end; first = false) {
-        while (pre[s + 1] * a.n_unit <= x) ++s;
-        s = __builtin_amdgcn_readfirstlane(s);
-        const int tiles = __builtin_amdgcn_readfirstlane(pre[s + 1] - pre[s]), n = __builtin_amdgcn_readfirstlane(paged_len(a.c, s));
-        const int rem = __builtin_amdgcn_readfirstlane(x - pre[s] * a.n_unit), unit = rem / tiles, tile0 = rem - unit * tiles;
-        const int ntile = min(tiles - tile0, x_end - x);
-        x += ntile;
-        const int blocks = (a.group + QH - 1) / QH, hk = unit / blocks, h0 = hk * a.group + (unit - hk * blocks) * QH, heads = min(QH, (hk + 1) * a.group - h0);
-        // the queries: chunk c holds elements 32 c + 8 g ... + 7 of head `col`
-        u4 q[NS][KC]; float unscale = 1.0f;
-        {
-            const float *qr = reinterpret_cast<const float *>(a.q + (long)s * a.q_seq + (long)(h0 + min(col, heads - 1)) * a.q_head) + 8 * g;
-            float4 x0[KC], x1[KC]; float top = 0.f;
-            const float pre_scale = CAP ? a.scale : a.scale * 1.44269504088896341f;
-#pragma unroll
-            for (int c = 0; c < KC; ++c) { x0[c] = reinterpret_cast<const float4 *>(qr + 32 * c)[0]; x1[c] = reinterpret_cast<const float4 *>(qr + 32 * c)[1]; }
-            float up = 1.0f;
-            if constexpr (!BF16) {          // a power of two that puts the largest element into [2^10, 2^11): the f16 terms neither overflow nor lose bits to the smallest exponent
-#pragma unroll
-                for (int c = 0; c < KC; ++c) top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(x0[c].x), fabsf(x0[c].y)), fmaxf(fabsf(x0[c].z), fabsf(x0[c].w))),
-                                                                   fmaxf(fmaxf(fabsf(x1[c].x), fabsf(x1[c].y)), fmaxf(fabsf(x1[c].z), fabsf(x1[c].w)))));
-                top = over_rows(top, [](float p, float r) { return fmaxf(p, r); });
-                const int e = top > 0.f ? min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100), 110) : 0;
-                up = __uint_as_float((uint32_t)(127 + 10 - e) << 23); unscale = __uint_as_float((uint32_t)(127 - 10 + e) << 23);
-            }
-            unscale *= pre_scale;
-#pragma unroll
-            for (int c = 0; c < KC; ++c) {
-                const float e[8] = {x0[c].x, x0[c].y, x0[c].z, x0[c].w, x1[c].x, x1[c].y, x1[c].z, x1[c].w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) { uint32_t t[NS]; Split<BF16>::of(e[2 * i] * up, e[2 * i + 1] * up, t);
-#pragma unroll
-                    for (int k = 0; k < NS; ++k) q[k][c][i] = t[k]; }
-            }
+        int n, tiles, unit, tile0 = 0, ntile;
+        if constexpr (ONE) {
+            s = blockIdx.y; unit = blockIdx.x; n = paged_len(a.c, s); tiles = ntile = (n + TILE - 1) / TILE; x = x_end;
+        } else {
+            while (pre[s + 1] * a.n_unit <= x) ++s;
+            s = __builtin_amdgcn_readfirstlane(s);
+            tiles = __builtin_amdgcn_readfirstlane(pre[s + 1] - pre[s]); n = __builtin_amdgcn_readfirstlane(paged_len(a.c, s));
+            const int rem = __builtin_amdgcn_readfirstlane(x - pre[s] * a.n_unit); unit = rem / tiles; tile0 = rem - unit * tiles;
+            ntile = min(tiles - tile0, x_end - x);
+            x += ntile;
         }
+        const int blocks = (a.group + QH - 1) / QH, hk = unit / blocks, h0 = hk * a.group + (unit - hk * blocks) * QH, heads = min(QH, (hk + 1) * a.group - h0);
+        // the queries: chunk c holds elements 32 c + 8 g ... + 7 of head `col`; requested before the cache rows, split under their way
+        const float *qr = reinterpret_cast<const float *>(a.q + (long)s * a.q_seq + (long)(h0 + min(col, heads - 1)) * a.q_head) + 8 * g;
+        float4 x0[KC], x1[KC];
+#pragma unroll
+        for (int c = 0; c < KC; ++c) { x0[c] = reinterpret_cast<const float4 *>(qr + 32 * c)[0]; x1[c] = reinterpret_cast<const float4 *>(qr + 32 * c)[1]; }
         const char *kb = a.c.k + (long)hk * a.c.k_head, *vb = a.c.v + (long)hk * a.c.v_head;
         const int *table = a.c.table + (long)s * a.c.table_row; const int in_page = (1 << a.c.page_shift) - 1;
         // 16 slots from j on lie in one page (pages are powers of two >= 16): its id, -1 past the end or unmapped
@@ -184,8 +179,31 @@ template <int D, bool BF16, bool CAP> __global__ void __launch_bounds__(256) pag
         float m = -INFINITY, l = 0.f;
         int j = (tile0 * WAVES + wave) * 32; const int j_end = min((tile0 + ntile) * TILE, n);
         int id0 = page_of(j), id1 = page_of(j + 16), nx0 = page_of(j + TILE), nx1 = page_of(j + TILE + 16);
-        float *score = a.weight ? a.score + ((long)s * a.n_head + h0 + min(col, heads - 1)) * a.score_row : nullptr;
+        const int hc = min(col, heads - 1);
+        float *score = !a.weight ? nullptr : ONE ? s_o + WAVES * heads * (D + 4) + hc * (int)a.score_row : a.score + ((long)s * a.n_head + h0 + hc) * a.score_row;
         if (j < j_end) { load_k(j, id0, id1); load_v(j, id0, id1); }
+        u4 q[NS][KC]; float unscale = 1.0f;
+        {
+            float top = 0.f; const float pre_scale = CAP ? a.scale : a.scale * 1.44269504088896341f;
+            float up = 1.0f;
+            if constexpr (!BF16) {          // a power of two that puts the largest element into [2^10, 2^11): the f16 terms neither overflow nor lose bits to the smallest exponent
+#pragma unroll
+                for (int c = 0; c < KC; ++c) top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(x0[c].x), fabsf(x0[c].y)), fmaxf(fabsf(x0[c].z), fabsf(x0[c].w))),
+                                                                   fmaxf(fmaxf(fabsf(x1[c].x), fabsf(x1[c].y)), fmaxf(fabsf(x1[c].z), fabsf(x1[c].w)))));
+                top = over_rows(top, [](float p, float r) { return fmaxf(p, r); });
+                const int e = top > 0.f ? min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100), 110) : 0;
+                up = __uint_as_float((uint32_t)(127 + 10 - e) << 23); unscale = __uint_as_float((uint32_t)(127 - 10 + e) << 23);
+            }
+            unscale *= pre_scale;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const float e[8] = {x0[c].x, x0[c].y, x0[c].z, x0[c].w, x1[c].x, x1[c].y, x1[c].z, x1[c].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { uint32_t t[NS]; Split<BF16>::of(e[2 * i] * up, e[2 * i + 1] * up, t);
+#pragma unroll
+                    for (int k = 0; k < NS; ++k) q[k][c][i] = t[k]; }
+            }
+        }
         while (j < j_end) {
             f4 z[2];
 #pragma unroll
@@ -205,7 +223,7 @@ template <int D, bool BF16, bool CAP> __global__ void __launch_bounds__(256) pag
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     float v = z[t][r] * unscale;
-                    if constexpr (CAP) v = a.softcap * 1.44269504088896341f * tanhf(v / a.softcap);
+                    if constexpr (CAP) v = a.softcap * 1.44269504088896341f * tanh_of(v * a.inv_softcap);
                     z[t][r] = v;
                 }
             if (!whole) {
@@ -278,8 +296,8 @@ template <int D, bool BF16, bool CAP> __global__ void __launch_bounds__(256) pag
                         *reinterpret_cast<f4 *>(so + 128 * hf + VW * (4 * g + r) + i) = (f4){o[hf][i][r] * f, o[hf][i + 1][r] * f, o[hf][i + 2][r] * f, o[hf][i + 3][r] * f};
         }
         __syncthreads();
-        const bool alone = ntile == tiles;
-        float *part = a.part + ((long)blockIdx.x * 2 + (first ? 0 : 1)) * QH * (D + 2);
+        const bool alone = ONE || ntile == tiles;
+        float *part = ONE ? nullptr : a.part + ((long)blockIdx.x * 2 + (first ? 0 : 1)) * QH * (D + 2);
         for (int e = threadIdx.x; e < heads * D / 4; e += 256) {
             const int h = e / (D / 4), d = (e - h * (D / 4)) * 4;
             const float Mh = fmaxf(fmaxf(s_m[0][h], s_m[1][h]), fmaxf(s_m[2][h], s_m[3][h]));
@@ -290,44 +308,103 @@ template <int D, bool BF16, bool CAP> __global__ void __launch_bounds__(256) pag
                 v += *reinterpret_cast<const f4 *>(s_o + (w * heads + h) * (D + 4) + d);
             }
             if (alone) {
-                if (Mh == -INFINITY) v = (f4){0.f, 0.f, 0.f, 0.f}; else v /= L;
+                if (Mh == -INFINITY) v = (f4){0.f, 0.f, 0.f, 0.f}; else v /= L;          // (nothing to attend to: a row of zeros)
                 *reinterpret_cast<f4 *>(a.dst + (long)s * a.d_seq + (long)(h0 + h) * a.d_head + d * 4) = v;
-                if (d == 0 && a.stat) a.stat[(long)s * a.n_head + h0 + h] = make_float2(Mh, L);
+                if (ONE) { if (d == 0) { s_row[0][h] = Mh; s_row[1][h] = 1.0f / L; } }
+                else if (d == 0 && a.stat) a.stat[(long)s * a.n_head + h0 + h] = make_float2(Mh, L);
             } else {
                 float *ph = part + h * (D + 2);
                 if (d == 0) { ph[0] = Mh; ph[1] = L; }
                 ph[2 + d] = v[0]; ph[3 + d] = v[1]; ph[4 + d] = v[2]; ph[5 + d] = v[3];
             }
         }
+        if (ONE && a.weight) {          // (one unit to a KV head: the host has seen to it)
+            __syncthreads();
+            const float *z = s_o + WAVES * heads * (D + 4);
+            float *w = reinterpret_cast<float *>(a.weight + (long)s * a.w_seq + (long)hk * a.w_head);
+            for (int i = threadIdx.x; i < n; i += 256) {          // one thread to a slot, the heads in order
+                float sum = 0.f;
+                for (int h = 0; h < heads; ++h) if (s_row[0][h] != -INFINITY) sum += __builtin_amdgcn_exp2f(z[h * (int)a.score_row + i] - (s_row[0][h] - 8.0f)) * s_row[1][h];
+                if (sum != 0.f) w[i] += sum;
+            }
+        }
     }
 }
-// grid (query heads, sequences): the rows that several workgroups share, and the rows of nothing.  256 threads: the partial maxima and sums one to a thread, then D / 4 threads to a
-// partial accumulator and 1024 / D of those at a time.
-template <int D> __global__ void __launch_bounds__(256) paged_attn_join_kernel(AttnArgs a) {
-    __shared__ float s_f[ATTN_MAX_WG], s_red[8]; __shared__ f4 s_v[256];
-    const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    float *out = reinterpret_cast<float *>(a.dst + (long)s * a.d_seq + (long)h * a.d_head);
-    const int p0 = a.prefix[s], tiles = a.prefix[s + 1] - p0;
-    if (tiles == 0) {
-        if (tid < D / 4) *reinterpret_cast<f4 *>(out + 4 * tid) = (f4){0.f, 0.f, 0.f, 0.f};
-        if (tid == 0 && a.stat) a.stat[(long)s * a.n_head + h] = make_float2(-INFINITY, 0.f);
-        return;
+// where the partial results of a query head lie: those of `count` neighbouring workgroups, the first at base + other, the next at base + step ...  A workgroup's slot 0 is its first unit,
+// slot 1 a later (its last) one: only the first of the row's workgroups can have begun with another unit.  count 1: the row is done.
+template <int D> struct RowParts {
+    static constexpr long STEP = 2l * QH * (D + 2);
+    const float *base; long other; int count, tiles;
+    __device__ RowParts(const AttnArgs &a, int h, int s) {
+        const int p0 = a.prefix[s]; tiles = a.prefix[s + 1] - p0; count = 0; base = nullptr; other = 0;
+        if (!tiles) return;
+        const Shares shares(a.prefix[a.c.n_seq] * a.n_unit, a.n_wg);
+        const int blocks = (a.group + QH - 1) / QH, hk = h / a.group, in = h - hk * a.group, unit = hk * blocks + in / QH;
+        const int x0 = p0 * a.n_unit + unit * tiles, w0 = shares.owner(x0);
+        count = shares.owner(x0 + tiles - 1) - w0 + 1;
+        base = a.part + ((long)w0 * 2 * QH + in % QH) * (D + 2);
+        other = shares.first(w0) < x0 ? (long)QH * (D + 2) : 0;
     }
-    const Shares shares(a.prefix[a.c.n_seq] * a.n_unit, a.n_wg);
-    const int blocks = (a.group + QH - 1) / QH, hk = h / a.group, in = h - hk * a.group, unit = hk * blocks + in / QH, hh = in % QH;
-    const int x0 = p0 * a.n_unit + unit * tiles, w0 = shares.owner(x0), count = shares.owner(x0 + tiles - 1) - w0 + 1;
+    __device__ const float *at(int i) const { return base + i * STEP + (i ? 0 : other); }
+};
+// weight[slot] += sum over the group of 2^(z - (m - 8)) / l for 1024 slots of a KV head, four to a thread, the heads in order.  The rows' m and l are joined here once more (16 lanes to a
+// head), which is cheaper than a third launch behind the join.
+template <int D> static __device__ __forceinline__ void add_weights(const AttnArgs &a, int hk, int s, int chunk, float2 *s_row) {
+    const int n = paged_len(a.c, s), j = chunk * 1024 + (int)threadIdx.x * 4;
+    if (chunk * 1024 >= n) return;
+    f4 sum = (f4){0.f, 0.f, 0.f, 0.f};
+    for (int h0 = 0; h0 < a.group; h0 += 16) {
+        const int heads = min(16, a.group - h0), h = hk * a.group + h0 + min((int)threadIdx.x >> 4, heads - 1);
+        const RowParts<D> row(a, h, s);
+        float m = -INFINITY, l = 0.f;
+        if (row.count == 1) { const float2 st = a.stat[(long)s * a.n_head + h]; m = st.x; l = st.y; }
+        else {
+            for (int i = threadIdx.x & 15; i < row.count; i += 16) {
+                const float2 p = *reinterpret_cast<const float2 *>(row.at(i)); const float to = fmaxf(m, p.x);
+                if (to != -INFINITY) l = l * __builtin_amdgcn_exp2f(m - to) + p.y * __builtin_amdgcn_exp2f(p.x - to);
+                m = to;
+            }
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) {
+                const float om = __shfl_xor(m, d, 64), ol = __shfl_xor(l, d, 64), to = fmaxf(m, om);
+                if (to != -INFINITY) l = l * __builtin_amdgcn_exp2f(m - to) + ol * __builtin_amdgcn_exp2f(om - to);
+                m = to;
+            }
+        }
+        __syncthreads();
+        if ((threadIdx.x & 15) == 0) s_row[threadIdx.x >> 4] = make_float2(m, 1.0f / l);
+        __syncthreads();
+        if (j < n) for (int i = 0; i < heads; ++i) {
+            const float2 st = s_row[i];
+            if (st.x == -INFINITY) continue;
+            const f4 z = *reinterpret_cast<const f4 *>(a.score + ((long)s * a.n_head + hk * a.group + h0 + i) * a.score_row + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += __builtin_amdgcn_exp2f(z[e] - (st.x - 8.0f)) * st.y;
+        }
+    }
+    float *w = reinterpret_cast<float *>(a.weight + (long)s * a.w_seq + (long)hk * a.w_head);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) if (j + e < n && sum[e] != 0.f) w[j + e] += sum[e];
+}
+// grid (query heads, then with weights KV heads x chunks of 1024 slots; sequences): the rows that several workgroups share, the rows of nothing, the weights.  256 threads: the partial
+// maxima and sums one to a thread, then D / 4 threads to a partial accumulator and 1024 / D of those at a time.
+template <int D> __global__ void __launch_bounds__(256) paged_attn_join_kernel(AttnArgs a) {
+    __shared__ float s_f[ATTN_MAX_WG], s_red[8]; __shared__ f4 s_v[256]; __shared__ float2 s_row[16];
+    const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (h >= a.n_head) { const int chunks = (int)(a.score_row + 1023) / 1024, i = h - a.n_head; add_weights<D>(a, i / chunks, s, i % chunks, s_row); return; }
+    float *out = reinterpret_cast<float *>(a.dst + (long)s * a.d_seq + (long)h * a.d_head);
+    const RowParts<D> part(a, h, s);
+    if (part.tiles == 0) { if (tid < D / 4) *reinterpret_cast<f4 *>(out + 4 * tid) = (f4){0.f, 0.f, 0.f, 0.f}; return; }
+    const int count = part.count;
     if (count == 1) return;
-    // a workgroup's slot 0 is its first unit, slot 1 a later (its last) one: only the first of the row's workgroups can have begun with another unit
-    const float *base = a.part + ((long)w0 * 2 * QH + hh) * (D + 2); constexpr long step = 2l * QH * (D + 2);
-    const long other = shares.first(w0) < x0 ? (long)QH * (D + 2) : 0;
     float M = -INFINITY;
-    for (int i = tid; i < count; i += 256) { const float m = base[i * step + (i ? 0 : other)]; s_f[i] = m; M = fmaxf(M, m); }
+    for (int i = tid; i < count; i += 256) { const float m = part.at(i)[0]; s_f[i] = m; M = fmaxf(M, m); }
     M = wave_max(M);
     if (lane == 0) s_red[wave] = M;
     __syncthreads();
     M = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
     float L = 0.f;
-    for (int i = tid; i < count; i += 256) { const float m = s_f[i], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M); s_f[i] = f; L += f * base[i * step + (i ? 0 : other) + 1]; }
+    for (int i = tid; i < count; i += 256) { const float m = s_f[i], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M); s_f[i] = f; L += f * part.at(i)[1]; }
     L = wave_sum_dpp(L);
     if (lane == 0) s_red[4 + wave] = L;
     __syncthreads();
@@ -337,7 +414,7 @@ template <int D> __global__ void __launch_bounds__(256) paged_attn_join_kernel(A
     f4 v = (f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int i = row; i < count; i += ROWS) {
-        const float *p = base + i * step + (i ? 0 : other) + 2 + d; const float2 lo = *reinterpret_cast<const float2 *>(p), hi = *reinterpret_cast<const float2 *>(p + 2);
+        const float *p = part.at(i) + 2 + d; const float2 lo = *reinterpret_cast<const float2 *>(p), hi = *reinterpret_cast<const float2 *>(p + 2);
         const float f = s_f[i];
         v[0] += lo.x * f; v[1] += lo.y * f; v[2] += hi.x * f; v[3] += hi.y * f;
     }
@@ -348,24 +425,6 @@ template <int D> __global__ void __launch_bounds__(256) paged_attn_join_kernel(A
     for (int r = 1; r < ROWS; ++r) v += s_v[r * TD + tid];
     if (M == -INFINITY) v = (f4){0.f, 0.f, 0.f, 0.f}; else v /= L;
     *reinterpret_cast<f4 *>(out + d) = v;
-    if (tid == 0 && a.stat) a.stat[(long)s * a.n_head + h] = make_float2(M, L);
-}
-// grid (chunks of 1024 slots, KV heads, sequences): weight[slot] += sum over the group of 2^(z - m) / l
-__global__ void __launch_bounds__(256) paged_attn_weight_kernel(AttnArgs a) {
-    const int hk = blockIdx.y, s = blockIdx.z, n = paged_len(a.c, s), j = (blockIdx.x * 256 + threadIdx.x) * 4;
-    if (blockIdx.x * 1024 >= n) return;
-    f4 sum = (f4){0.f, 0.f, 0.f, 0.f};
-    if (j < n) for (int g = 0; g < a.group; ++g) {
-        const long row = (long)s * a.n_head + hk * a.group + g; const float2 st = a.stat[row];
-        if (st.x == -INFINITY) continue;
-        const f4 z = *reinterpret_cast<const f4 *>(a.score + row * a.score_row + j);
-        const float ref = st.x - 8.0f, inv = 1.0f / st.y;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(z[i] - ref) * inv;
-    }
-    float *w = reinterpret_cast<float *>(a.weight + (long)s * a.w_seq + (long)hk * a.w_head);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) if (j + i < n && sum[i] != 0.f) w[j + i] += sum[i];
 }
 static int attn_check(const cdna4_tensor *q, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const cdna4_tensor *weight, const cdna4_tensor *dst, AttnArgs *a) {
     ARG_CHECK(q && dst, "paged_attn: null argument");
@@ -406,30 +465,40 @@ int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_t
     if (pg_empty(q)) return CDNA4_OK;
     ARG_CHECK(n_kv && q->data && dst->data && (a.c.W == 0 || (a.c.table && (!weight || weight->data))), "paged_attn: null data");
     ARG_CHECK(!pg_overlap(q, 4, dst, 4) && (!weight || a.c.W == 0 || (!pg_overlap(weight, 4, dst, 4) && !pg_overlap(weight, 4, q, 4))), "paged_attn: q, dst and weight may not overlap");
-    a.c.n_kv = n_kv; a.scale = scale; a.softcap = softcap;
+    a.c.n_kv = n_kv; a.scale = scale; a.softcap = softcap; a.inv_softcap = softcap != 0.0f ? 1.0f / softcap : 0.0f;
     a.q = (const char *)q->data; a.q_head = q->nb[1]; a.q_seq = q->nb[2]; a.dst = (char *)dst->data; a.d_head = dst->nb[1]; a.d_seq = dst->nb[2];
     a.weight = weight ? (char *)weight->data : nullptr; a.w_head = weight ? weight->nb[1] : 0; a.w_seq = weight ? weight->nb[2] : 0;
     DEVICE_SCOPE(ctx);
-    const long tiles = a.score_row / TILE * a.c.n_seq * a.n_unit;
+    const long row_tiles = a.score_row / TILE, tiles = row_tiles * a.c.n_seq * a.n_unit;
+    const bool bf = k_cache->type == CDNA4_TYPE_BF16, cap = softcap != 0.0f;
+    hipStream_t st = (hipStream_t)stream;
+    const size_t merge = (size_t)WAVES * std::min(QH, a.group) * (a.c.D + 4) * 4;
+    // A workgroup per unit where a unit is little work, or where there are enough units and none is long (a unit of 16 tiles takes 24 us by itself).  Measured, us with a workgroup per
+    // unit / with equal shares and a join (32 query heads, 8 KV heads of 128; sequences x slots): 1 x 100: 6.6 / 9.6, 1 x 512: 9.9 / 11.8, 1 x 1024: 14.4 / 11.8, 8 x 1024: 15.3 / 14.8,
+    // 64 x 512: 17.8 / 26.4, 64 x 2048: 58 / 61, 256 x 512: 56 / 80, 256 x 2048: 205 / 222.  With weights: if a KV head is one unit and its scores fit LDS.
+    const size_t one_lds = merge + (weight ? (size_t)a.group * a.score_row * 4 : 0);
+    const bool one = (row_tiles <= 4 || (row_tiles <= 16 && (long)a.c.n_seq * a.n_unit >= 2l * ctx->num_cu)) && (!weight || a.group <= QH) && one_lds <= ONE_LDS;
+#define ATTN(D_, B_, C_, O_, grid, lds) do { if ((lds) > 60 * 1024) HIP_TRY((pg_opt_in_lds<paged_attn_kernel<D_, B_, C_, O_>>(ctx->device, ONE_LDS))); \
+                                             hipLaunchKernelGGL((paged_attn_kernel<D_, B_, C_, O_>), grid, dim3(256), lds, st, a); } while (0)
+#define ATTN_D(D_, O_, grid, lds) do { if (bf) { if (cap) ATTN(D_, true, true, O_, grid, lds); else ATTN(D_, true, false, O_, grid, lds); } \
+                                       else { if (cap) ATTN(D_, false, true, O_, grid, lds); else ATTN(D_, false, false, O_, grid, lds); } HIP_TRY(hipGetLastError()); } while (0)
+#define ATTN_ALL(O_, grid, lds) do { if (a.c.D == 64) ATTN_D(64, O_, grid, lds); else if (a.c.D == 128) ATTN_D(128, O_, grid, lds); else ATTN_D(256, O_, grid, lds); } while (0)
+    if (one) {
+        a.n_wg = 0; a.prefix = nullptr; a.part = nullptr; a.stat = nullptr; a.score = nullptr;
+        ATTN_ALL(true, dim3((unsigned)a.n_unit, (unsigned)a.c.n_seq), one_lds);
+        return CDNA4_OK;
+    }
     a.n_wg = (int)std::max<long>(1, std::min<long>({tiles, (long)ctx->num_cu * (a.c.D == 256 ? 1 : 2), (long)ATTN_MAX_WG}));
     const AttnScratch sc = attn_scratch(a, weight != nullptr, a.n_wg);
-    hipStream_t st = (hipStream_t)stream;
     if ((rc = cdna4_ensure_ws(ctx, sc.total, st))) return rc;
     char *ws = (char *)ctx->ws;
     a.prefix = (int *)ws; a.part = (float *)(ws + sc.part); a.stat = weight ? (float2 *)(ws + sc.stat) : nullptr; a.score = weight ? (float *)(ws + sc.score) : nullptr;
-    const bool bf = k_cache->type == CDNA4_TYPE_BF16, cap = softcap != 0.0f;
-    // (at most (8192 + 4) * 4 + 4 * 16 * 260 * 4 bytes < 100 KB)
-    const size_t lds = (size_t)((a.c.n_seq + 4) & ~3) * 4 + (size_t)WAVES * std::min(QH, a.group) * (a.c.D + 4) * 4;
-#define ATTN(D_, B_, C_) do { if (lds > 60 * 1024) HIP_TRY((pg_opt_in_lds<paged_attn_kernel<D_, B_, C_>>(ctx->device, 100 * 1024))); \
-                              hipLaunchKernelGGL((paged_attn_kernel<D_, B_, C_>), dim3((unsigned)a.n_wg), dim3(256), lds, st, a); } while (0)
-#define ATTN_D(D_) do { if (bf) { if (cap) ATTN(D_, true, true); else ATTN(D_, true, false); } else { if (cap) ATTN(D_, false, true); else ATTN(D_, false, false); } \
-                        HIP_TRY(hipGetLastError()); \
-                        hipLaunchKernelGGL(paged_attn_join_kernel<D_>, dim3((unsigned)a.n_head, (unsigned)a.c.n_seq), dim3(256), 0, st, a); } while (0)
-    if (a.c.D == 64) ATTN_D(64); else if (a.c.D == 128) ATTN_D(128); else ATTN_D(256);
+    const size_t lds = (size_t)((a.c.n_seq + 4) & ~3) * 4 + merge;          // (at most (8192 + 4) * 4 + 4 * 16 * 260 * 4 bytes)
+    ATTN_ALL(false, dim3((unsigned)a.n_wg), lds);
+    const dim3 join((unsigned)(a.n_head + (weight ? a.c.n_head_kv * ((a.score_row + 1023) / 1024) : 0)), (unsigned)a.c.n_seq);
+    if (a.c.D == 64) hipLaunchKernelGGL(paged_attn_join_kernel<64>, join, dim3(256), 0, st, a);
+    else if (a.c.D == 128) hipLaunchKernelGGL(paged_attn_join_kernel<128>, join, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(paged_attn_join_kernel<256>, join, dim3(256), 0, st, a);
     HIP_TRY(hipGetLastError());
-    if (weight && a.c.W) {
-        hipLaunchKernelGGL(paged_attn_weight_kernel, dim3((unsigned)((a.score_row + 1023) / 1024), (unsigned)a.c.n_head_kv, (unsigned)a.c.n_seq), dim3(256), 0, st, a);
-        HIP_TRY(hipGetLastError());
-    }
     return CDNA4_OK;
 }
