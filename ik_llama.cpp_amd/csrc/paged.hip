@@ -220,30 +220,43 @@ template <bool HERE> __global__ void __launch_bounds__(EVICT_THREADS) paged_evic
     auto count_digit = [&](uint32_t digit) { atomicAdd(&hist[digit * EVICT_COPIES + (lane & (EVICT_COPIES - 1))], 1u); };
     zero();
     __syncthreads();
-    auto take = [&](int j, float x, int y) {
-        if (over) { const uint32_t k = evict_key(x, y, a.sink, recent_from); if (in_lds) s_key[j] = k; count_digit(k >> 21); }
-        if (!a.in_place && j < a.budget) { wo[j] = x; po[j] = y; }
-    };
+    auto take = [&](float x, int y) { const uint32_t k = evict_key(x, y, a.sink, recent_from); count_digit(k >> 21); return k; };
 #pragma unroll 4
     for (int j = 4 * tid; j < n - 3; j += 4 * EVICT_THREADS) {
         const F4u x = *reinterpret_cast<const F4u *>(w + j); const I4u y = *reinterpret_cast<const I4u *>(p + j);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) take(j + i, x.v[i], y.v[i]);
+        if (over) {
+            uint4 k; k.x = take(x.v[0], y.v[0]); k.y = take(x.v[1], y.v[1]); k.z = take(x.v[2], y.v[2]); k.w = take(x.v[3], y.v[3]);
+            if (in_lds) *reinterpret_cast<uint4 *>(s_key + j) = k;
+        }
+        if (!a.in_place) {
+            if (j + 4 <= a.budget) { *reinterpret_cast<F4u *>(wo + j) = x; *reinterpret_cast<I4u *>(po + j) = y; }
+            else for (int i = 0; i < 4; ++i) if (j + i < a.budget) { wo[j + i] = x.v[i]; po[j + i] = y.v[i]; }
+        }
     }
-    if (tid < (n & 3)) { const int j = (n & ~3) + tid; take(j, w[j], p[j]); }
+    if (tid < (n & 3)) {
+        const int j = (n & ~3) + tid; const float x = w[j]; const int y = p[j];
+        if (over) { const uint32_t k = take(x, y); if (in_lds) s_key[j] = k; }
+        if (!a.in_place && j < a.budget) { wo[j] = x; po[j] = y; }
+    }
     if (!over) { if (!HERE && tid == 0) moves[0] = 0; return; }
     __syncthreads();
-    auto key = [&](int j) { return in_lds ? s_key[j] : evict_key(w[j], p[j], a.sink, recent_from); };
+    // the keys of slots j ... j + 3 (j a multiple of 4; what lies behind the row's end is anything)
+    auto keys4 = [&](int j) {
+        if (in_lds) return *reinterpret_cast<const uint4 *>(s_key + j);
+        auto one = [&](int i) { i = min(i, n - 1); return evict_key(w[i], p[i], a.sink, recent_from); };
+        return make_uint4(one(j), one(j + 1), one(j + 2), one(j + 3));
+    };
     uint32_t prefix = 0, rest = (uint32_t)a.budget; bool all_equal = false;         // the budget-th largest key lies among those that equal `prefix` so far; `rest` of them are kept
     for (int shift = 21; ; shift = max(shift - 11, 0)) {                            // bits [21, 32), [10, 21), [0, 10)
         const int width = shift ? 11 : 10;
         if (shift < 21) {
-            const int high = shift + width;
-            if (in_lds) {
-#pragma unroll 8
-                for (int j = tid; j < n; j += EVICT_THREADS) { const uint32_t x = s_key[j]; if ((x >> high) == (prefix >> high)) count_digit((x >> shift) & ((1u << width) - 1)); }
-            } else
-                for (int j = tid; j < n; j += EVICT_THREADS) { const uint32_t x = key(j); if ((x >> high) == (prefix >> high)) count_digit((x >> shift) & ((1u << width) - 1)); }
+            const int high = shift + width; const uint32_t want = prefix >> high, mask = (1u << width) - 1;
+#pragma unroll 4
+            for (int j = 4 * tid; j < n; j += 4 * EVICT_THREADS) {
+                const uint4 k = keys4(j); const uint32_t x[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) if ((x[i] >> high) == want && j + i < n) count_digit((x[i] >> shift) & mask);
+            }
             __syncthreads();
         }
         // two bins a thread, from the top bin down
@@ -262,39 +275,56 @@ template <bool HERE> __global__ void __launch_bounds__(EVICT_THREADS) paged_evic
     }
     // kept: every key >= prefix if all of the last bin are kept, otherwise (the whole key is in prefix) the larger ones and the first `rest` of the equal ones
     const int span = ((n + EVICT_WAVES - 1) / EVICT_WAVES + 255) & ~255, j0 = min(wave * span, n), j1 = min(j0 + span, n);
-    const unsigned long long below = (1ull << lane) - 1;
     unsigned tie0 = 0;
     if (!all_equal) {                                       // (uniform)
         unsigned ties = 0;
-        for (int b = j0; b < j1; b += 64) { const int j = b + lane; ties += __popcll(__ballot(j < j1 && key(min(j, n - 1)) == prefix)); }
-        if (lane == 0) tot[1][wave] = ties;
+        for (int j = j0 + 4 * lane; j < j1; j += 256) {
+            const uint4 k = keys4(j); const uint32_t x[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ties += x[i] == prefix && j + i < j1;
+        }
+        ties = wave_scan(ties);
+        if (lane == 63) tot[1][wave] = ties;
         __syncthreads();
         tie0 = waves_before(tot[1], wave);
         __syncthreads();
     }
-    unsigned holes = 0, movers = 0, nh = 0, nm = 0;
-    for (int round = 0; round < 2; ++round) {               // count, then list
-        unsigned t = tie0; nh = holes; nm = movers;
+    // four slots to a lane, 256 to a step; holes and movers counted in the halves of one number.  First round: how many has the wave; second: where they go
+    unsigned holes = 0, movers = 0;
+    for (int round = 0; round < 2; ++round) {
+        unsigned t = tie0, found = 0, lane_holes = 0, lane_movers = 0;
         for (int b = j0; b < j1; b += 256) {
-            uint32_t x[4];
+            const int j = b + 4 * lane; const uint4 k = keys4(min(j, (n - 1) & ~3)); const uint32_t x[4] = {k.x, k.y, k.z, k.w};
+            unsigned keep = 0, in = 0;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) x[u] = key(min(b + 64 * u + lane, n - 1));
+            for (int i = 0; i < 4; ++i) { in |= (j + i < j1) << i; keep |= (x[i] >= prefix) << i; }
+            if (!all_equal) {
+                unsigned tie = 0;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int j = b + 64 * u + lane; const bool in = j < j1;
-                bool keep = in && x[u] >= prefix;
-                if (!all_equal) { const unsigned long long tie = __ballot(in && x[u] == prefix); keep = in && (x[u] > prefix || (x[u] == prefix && t + __popcll(tie & below) < rest)); t += __popcll(tie); }
-                const unsigned long long hole = __ballot(in && !keep && j < a.budget), mover = __ballot(keep && j >= a.budget);
-                if (round && (hole | mover)) {
-                    int *list = HERE ? s_moves : moves + 1; const int half = HERE ? EVICT_HERE : most;
-                    if ((hole >> lane) & 1) list[half + nh + __popcll(hole & below)] = j;
-                    if ((mover >> lane) & 1) list[nm + __popcll(mover & below)] = j;
-                }
-                nh += __popcll(hole); nm += __popcll(mover);
+                for (int i = 0; i < 4; ++i) tie |= (x[i] == prefix) << i;
+                tie &= in;
+                const unsigned mine = __popc(tie), upto = wave_scan(mine);
+                unsigned r = t + upto - mine;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) if ((tie >> i) & 1) { if (r >= rest) keep &= ~(1u << i); ++r; }
+                t += (unsigned)__builtin_amdgcn_readlane((int)upto, 63);
             }
+            const unsigned before = a.budget >= j + 4 ? 15u : a.budget <= j ? 0u : (1u << (a.budget - j)) - 1;      // the lane's slots before the budget
+            const unsigned hole = in & ~keep & before, mover = in & keep & ~before, c = __popc(hole) | (__popc(mover) << 16);
+            if (!round) { lane_holes += c & 0xffffu; lane_movers += c >> 16; continue; }
+            const unsigned upto = wave_scan(c), at = found + upto - c;
+            if (c) {
+                int *list = HERE ? s_moves : moves + 1; const int half = HERE ? EVICT_HERE : most;
+                unsigned nh = half + holes + (at & 0xffffu), nm = movers + (at >> 16);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { if ((hole >> i) & 1) list[nh++] = j + i; if ((mover >> i) & 1) list[nm++] = j + i; }
+            }
+            found += (unsigned)__builtin_amdgcn_readlane((int)upto, 63);
+            if (!in_lds) { holes += found & 0xffffu; movers += found >> 16; found = 0; }          // (a long row's wave may have more than 2^16 of either)
         }
         if (!round) {
-            if (lane == 0) { tot[1][wave] = nh; tot[2][wave] = nm; }
+            const unsigned nh = wave_scan(lane_holes), nm = wave_scan(lane_movers);
+            if (lane == 63) { tot[1][wave] = nh; tot[2][wave] = nm; }
             __syncthreads();
             holes = waves_before(tot[1], wave); movers = waves_before(tot[2], wave);
         }
@@ -305,7 +335,7 @@ template <bool HERE> __global__ void __launch_bounds__(EVICT_THREADS) paged_evic
 #pragma unroll
         for (int i = 0; i < EVICT_WAVES; ++i) count += (int)tot[2][i];
         for (int m = tid >> 4; m < count; m += EVICT_THREADS / 16) evict_move(a, s, h, s_moves[m], s_moves[EVICT_HERE + m], tid & 15);
-    } else if (tid == EVICT_THREADS - 1) moves[0] = (int)nm;       // the last wave's running count is the total
+    } else if (tid == EVICT_THREADS - 1) moves[0] = (int)(waves_before(tot[2], EVICT_WAVES - 1) + tot[2][EVICT_WAVES - 1]);
 }
 // grid (chunks of moves, KV heads, sequences)
 __global__ void __launch_bounds__(256) paged_evict_move_kernel(EvictArgs a) {
