@@ -230,6 +230,7 @@ class Cdna4Backend:
             raise Cdna4Error(-3, self.lib.cdna4_last_error().decode())
         self.comm = None
         self.window = None
+        self._i32 = torch.int32; self._i0 = torch.empty(0, dtype=torch.int32, device=self.device)          # (new_empty of it: an int32 tensor at half the price of torch.empty)
 
     def close(self):
         self.window_free()
@@ -439,10 +440,13 @@ class Cdna4Backend:
     # These calls are short on the device (5 to 20 us), so the host's share counts: descriptors are packed into bytes (ctypes structures cost several times as much).
     def _desc(self, x, name):
         """cdna4_tensor {data, type, ne[4], nb[4]} of a torch tensor of at most 4 dimensions: sizes and byte strides from the innermost dimension out"""
-        t = _DESC_TYPES.get(getattr(x, "dtype", None))
-        if t is None or x.device != self.device:
+        try:
+            ty, es = _DESC_TYPES[x.dtype]
+            here = x.device == self.device
+        except (AttributeError, KeyError):
+            here = False
+        if not here:
             raise Cdna4Error(-2, "%s: a float32 / float16 / bfloat16 / int32 tensor on %s" % (name, self.device))
-        ty, es = t
         n = x.dim()
         if n == 3:
             (c, b, a), (r, q, p) = x.shape, x.stride()
@@ -459,24 +463,20 @@ class Cdna4Backend:
         """address of a dense vector of n elements (int32 unless said), None for None"""
         if x is None:
             return None
-        if getattr(x, "dtype", None) != (dtype or self.torch.int32) or x.device != self.device or x.numel() != n or not x.is_contiguous():
-            raise Cdna4Error(-2, "%s: a dense %s vector of %d elements on %s" % (name, dtype or self.torch.int32, n, self.device))
+        try:
+            fits = x.dtype == (dtype or self._i32) and x.device == self.device and x.numel() == n and x.is_contiguous()
+        except AttributeError:
+            fits = False
+        if not fits:
+            raise Cdna4Error(-2, "%s: a dense %s vector of %d elements on %s" % (name, dtype or self._i32, n, self.device))
         return x.data_ptr()
-
-    def _table_rows(self, table, name="table"):
-        if not self.torch.is_tensor(table) or table.dim() != 2:
-            raise Cdna4Error(-2, "%s: int32 [n_seq, W]" % name)
-        return table.shape[0]
-
-    def _ints(self, *shape):
-        return self.torch.empty(shape, dtype=self.torch.int32, device=self.device)
 
     def paged_store(self, k, v, k_cache, v_cache, table, n_kv, start=None, n_past=None, weight=None, pos=None, n_kv_out=None):
         """cdna4_op_paged_store: k, v f32 [n_tok, n_head_kv, D] into the slots behind n_kv (start int32 [n_seq + 1]: token ranges of the sequences, None: one token each); returns the new n_kv."""
-        n = self._table_rows(table)
+        td = self._desc(table, "table"); n = table.shape[-2]
         if n_kv_out is None:
-            n_kv_out = self.torch.empty_like(n_kv)
-        self._check(self.lib.cdna4_op_paged_store(self.ctx, self._desc(k, "k"), self._desc(v, "v"), self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), self._desc(table, "table"),
+            n_kv_out = table.new_empty(n)
+        self._check(self.lib.cdna4_op_paged_store(self.ctx, self._desc(k, "k"), self._desc(v, "v"), self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), td,
                                                   self._vec(n_kv, "n_kv", n), self._vec(start, "start", n + 1), self._vec(n_past, "n_past", n),
                                                   None if weight is None else self._desc(weight, "weight"), None if pos is None else self._desc(pos, "pos"),
                                                   self._vec(n_kv_out, "n_kv_out", n), self._stream()))
@@ -484,20 +484,20 @@ class Cdna4Backend:
 
     def paged_attn(self, q, k_cache, v_cache, table, n_kv, scale=None, softcap=0.0, weight=None, out=None):
         """cdna4_op_paged_attn: q f32 [n_seq, n_head, D] -> f32 [n_seq, n_head, D]; scale None: 1 / sqrt(D); weight: += the attention weight that every slot gathers, in place."""
-        qd = self._desc(q, "q")
+        qd, td = self._desc(q, "q"), self._desc(table, "table")
         if out is None:
             out = q.new_empty(q.shape)
-        self._check(self.lib.cdna4_op_paged_attn(self.ctx, qd, self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), self._desc(table, "table"),
-                                                 self._vec(n_kv, "n_kv", self._table_rows(table)), None if weight is None else self._desc(weight, "weight"), self._desc(out, "out"),
+        self._check(self.lib.cdna4_op_paged_attn(self.ctx, qd, self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), td,
+                                                 self._vec(n_kv, "n_kv", table.shape[-2]), None if weight is None else self._desc(weight, "weight"), self._desc(out, "out"),
                                                  float(q.shape[-1] ** -0.5 if scale is None else scale), float(softcap), self._stream()))
         return out
 
     def paged_evict(self, k_cache, v_cache, table, n_kv, weight, pos, n_past, budget, n_sink=0, n_recent=0, weight_out=None, pos_out=None, n_kv_out=None):
         """cdna4_op_paged_evict: every (sequence, KV head) keeps `budget` slots, by position and gathered weight; weight_out / pos_out None: in place.  Returns the new n_kv."""
-        n = self._table_rows(table)
+        td = self._desc(table, "table"); n = table.shape[-2]
         if n_kv_out is None:
-            n_kv_out = self.torch.empty_like(n_kv)
-        self._check(self.lib.cdna4_op_paged_evict(self.ctx, self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), self._desc(table, "table"), self._vec(n_kv, "n_kv", n),
+            n_kv_out = table.new_empty(n)
+        self._check(self.lib.cdna4_op_paged_evict(self.ctx, self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), td, self._vec(n_kv, "n_kv", n),
                                                   self._desc(weight, "weight"), self._desc(pos, "pos"), self._vec(n_past, "n_past", n), budget, n_sink, n_recent,
                                                   self._desc(weight if weight_out is None else weight_out, "weight_out"), self._desc(pos if pos_out is None else pos_out, "pos_out"),
                                                   self._vec(n_kv_out, "n_kv_out", n), self._stream()))
@@ -509,20 +509,21 @@ class Cdna4Backend:
         rows = logits.shape[0]; n_group = rows // n_beam if n_beam > 0 else 0
         if outs is None:
             shape = (n_group, max(n_out, 0))
-            outs = (self.torch.empty(shape, dtype=self.torch.float32, device=self.device), self._ints(*shape), self._ints(*shape))
-        ptr = [self._vec(x, name, n_group * n_out, want) for x, name, want in
-               zip(outs, ("score_out", "parent", "token"), (self.torch.float32, self.torch.int32, self.torch.int32))]
-        self._check(self.lib.cdna4_op_beam_select(self.ctx, d, self._vec(score, "score", rows, self.torch.float32), self._vec(done, "done", rows), n_beam, n_out, pad, *ptr, self._stream()))
+            parent = self._i0.new_empty(shape)
+            outs = (logits.new_empty(shape), parent, self.torch.empty_like(parent))
+        f32, m = self.torch.float32, n_group * n_out
+        self._check(self.lib.cdna4_op_beam_select(self.ctx, d, self._vec(score, "score", rows, f32), self._vec(done, "done", rows), n_beam, n_out, pad,
+                                                  self._vec(outs[0], "score_out", m, f32), self._vec(outs[1], "parent", m), self._vec(outs[2], "token", m), self._stream()))
         return outs
 
     def paged_fork(self, k_cache, v_cache, table, n_kv, parent, fresh, table_out=None, n_kv_out=None):
         """cdna4_op_paged_fork: rows that go on from row parent[i] (full pages shared, a cut last page copied into page fresh[i]); returns (table int32 [n_out, W], n_kv int32 [n_out])."""
-        n = self._table_rows(table); n_out = parent.numel() if self.torch.is_tensor(parent) else 0
+        td = self._desc(table, "table"); n = table.shape[-2]; n_out = parent.numel() if self.torch.is_tensor(parent) else 0
         if table_out is None:
-            table_out = self._ints(n_out, table.shape[1])
+            table_out = table.new_empty((n_out, table.shape[-1]))
         if n_kv_out is None:
-            n_kv_out = self._ints(n_out)
-        self._check(self.lib.cdna4_op_paged_fork(self.ctx, self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), self._desc(table, "table"), self._vec(n_kv, "n_kv", n),
+            n_kv_out = table.new_empty(n_out)
+        self._check(self.lib.cdna4_op_paged_fork(self.ctx, self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), td, self._vec(n_kv, "n_kv", n),
                                                  self._vec(parent, "parent", n_out), self._vec(fresh, "fresh", n_out), self._desc(table_out, "table_out"),
                                                  self._vec(n_kv_out, "n_kv_out", n_out), self._stream()))
         return table_out, n_kv_out

@@ -119,8 +119,10 @@ __global__ void __launch_bounds__(256) paged_fork_kernel(ForkArgs a) {
     const int per_row = a.c.D / 8, units = used * per_row;
     const char *ks = a.c.k + (long)from * a.c.k_page + (long)h * a.c.k_head, *vs = a.c.v + (long)from * a.c.v_page + (long)h * a.c.v_head;
     char *kd = a.c.k + (long)to * a.c.k_page + (long)h * a.c.k_head, *vd = a.c.v + (long)to * a.c.v_page + (long)h * a.c.v_head;
+    const int lg = a.c.D == 64 ? 3 : a.c.D == 128 ? 4 : 5;
+#pragma unroll 4
     for (int u = threadIdx.x; u < units; u += 256) {
-        const int r = u / per_row, d = (u - r * per_row) * 16;
+        const int r = u >> lg, d = (u & (per_row - 1)) * 16;
         const uint4 x = *reinterpret_cast<const uint4 *>(ks + r * a.c.k_row + d), y = *reinterpret_cast<const uint4 *>(vs + r * a.c.v_row + d);
         *reinterpret_cast<uint4 *>(kd + r * a.c.k_row + d) = x; *reinterpret_cast<uint4 *>(vd + r * a.c.v_row + d) = y;
     }

@@ -31,6 +31,7 @@ def be():
     pkg = load_package()
     b = object.__new__(pkg.Cdna4Backend)
     b.torch, b.lib, b.ctx, b.comm, b.window, b.device = torch, pkg.load_library(), None, None, None, torch.device("cpu")
+    b._i32, b._i0 = torch.int32, torch.empty(0, dtype=torch.int32)
     b._stream = lambda: None
     return b
 
