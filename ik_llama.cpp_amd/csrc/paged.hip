@@ -81,14 +81,16 @@ int cdna4_op_paged_store(cdna4_context *ctx, const cdna4_tensor *k, const cdna4_
     if ((rc = new_rows_check("k", k, a.c)) || (rc = new_rows_check("v", v, a.c))) return rc;
     ARG_CHECK(k->ne[2] == v->ne[2], "paged_store: as many rows of k as of v");
     const long n_tok = k->ne[2], n_seq = a.c.n_seq;
-    OP_CHECK(n_tok <= 0x7fffffff - PAGED_MAX_SEQ, "paged_store: too many tokens");
+    OP_CHECK(n_tok <= (1l << 23), "paged_store: at most 2^23 tokens");
     ARG_CHECK(start || n_tok == n_seq, "paged_store: without start, one token per sequence");
     if (weight && (rc = pg_slots_check("paged_store", "weight", weight, CDNA4_TYPE_F32, a.c, true))) return rc;
     if (pos && (rc = pg_slots_check("paged_store", "pos", pos, CDNA4_TYPE_I32, a.c, true))) return rc;
     if (n_seq == 0) return CDNA4_OK;
     ARG_CHECK(n_kv && (a.c.table || a.c.W == 0) && (n_tok == 0 || (k->data && v->data)) && (!pos || n_past), "paged_store: null data");
     ARG_CHECK((!weight || weight->data || a.c.W == 0) && (!pos || pos->data || a.c.W == 0), "paged_store: null data");
-    ARG_CHECK(!n_kv_out || !pg_overlap(n_kv_out, n_seq * 4, n_kv, n_seq * 4), "paged_store: n_kv_out overlaps n_kv");
+    ARG_CHECK(!n_kv_out || (!pg_overlap(n_kv_out, n_seq * 4, n_kv, n_seq * 4) && !pg_overlap(n_kv_out, n_seq * 4, start, (n_seq + 1) * 4) && !pg_overlap(n_kv_out, n_seq * 4, n_past, n_seq * 4)),
+              "paged_store: n_kv_out overlaps an input");
+    ARG_CHECK(!weight || !pos || a.c.W == 0 || !pg_overlap(weight, 4, pos, 4), "paged_store: weight overlaps pos");
     a.k = (const char *)k->data; a.v = (const char *)v->data; a.k_head = k->nb[1]; a.v_head = v->nb[1]; a.k_tok = k->nb[2]; a.v_tok = v->nb[2];
     a.c.n_kv = n_kv; a.start = start; a.n_past = n_past; a.weight = slot_view(weight); a.pos = slot_view(pos); a.n_kv_out = n_kv_out; a.n_tok = (int)n_tok;
     const long blocks = n_tok + (n_kv_out ? (n_seq + 255) / 256 : 0);

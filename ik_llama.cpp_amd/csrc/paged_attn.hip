@@ -281,6 +281,7 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
         }
         // the four waves' results: (m, l) through LDS, then the accumulators on the common maximum
         l = over_rows(l, [](float p, float r) { return p + r; });
+        if (m == -INFINITY && l != l) m = 0.f;                            // (scores that are all NaN: the maximum has passed them over, the result is NaN and not a row of nothing)
         __syncthreads();                                                  // (the previous unit's reads of s_o are done)
         if (g == 0) { s_m[wave][col] = m; s_l[wave][col] = l; }
         __syncthreads();
@@ -439,7 +440,7 @@ static int attn_check(const cdna4_tensor *q, const cdna4_tensor *k_cache, const 
     if (weight && (rc = pg_slots_check("paged_attn", "weight", weight, CDNA4_TYPE_F32, a->c, true))) return rc;
     a->n_head = (int)q->ne[1]; a->group = a->n_head / a->c.n_head_kv; a->n_unit = a->c.n_head_kv * ((a->group + QH - 1) / QH);
     const long slots = (long)a->c.W << a->c.page_shift, tiles = (slots + TILE - 1) / TILE;
-    OP_CHECK(tiles * a->c.n_seq < (1l << 31) / std::max(a->n_unit, 1), "paged_attn: too many slots in all");
+    OP_CHECK(tiles * a->c.n_seq < (1l << 31) / std::max(a->n_unit, 1) && tiles * a->c.n_head_kv < (1l << 26), "paged_attn: too many slots in all");
     a->score_row = tiles * TILE;
     return CDNA4_OK;
 }

@@ -367,7 +367,7 @@ CDNA4_API int cdna4_op_moe_router_norm(cdna4_context *ctx, const cdna4_tensor *w
  *   weight, pos      : f32 / i32 [>= W * page, n_head_kv, n_seq]: per slot and KV head, the attention weight that the slot has gathered and the position of its token (the heads keep
  *                      different tokens after an eviction).
  * Attention does not depend on the order of the slots (K is rotated before it is stored), so evictions leave the slots of a sequence in disorder and pos says which token is where.
- * Strides of dimensions with one element do not count.  n_seq, W * page: at most 8192 and 2^30.  n_kv_out may not overlap n_kv.  Errors: CDNA4_E_INVALID null / inconsistent arguments, CDNA4_E_UNSUPPORTED shapes and types outside the
+ * Strides of dimensions with one element do not count.  n_seq, W * page: at most 8192 and 2^30.  n_kv_out may not overlap an input.  Errors: CDNA4_E_INVALID null / inconsistent arguments, CDNA4_E_UNSUPPORTED shapes and types outside the
  * above, CDNA4_E_NOMEM a workspace that would have to grow during stream capture: reserve the largest cdna4_paged_*_workspace / cdna4_beam_select_workspace beforehand.  Those
  * functions run the same checks and return the bytes, or the error; they need no device. */
 

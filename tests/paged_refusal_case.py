@@ -120,6 +120,9 @@ expect("store", INVALID, k=lambda a: tensor(F32, 64, 1, 3))
 expect("store", UNSUPPORTED, k=lambda a: tensor(F32, 64, 2, 3, nb=(4, 264, 528)))
 expect("store", INVALID, n_past=None)
 expect("store", INVALID, n_out=lambda a: a["n_kv"] + 8)
+expect("store", INVALID, n_out=lambda a: a["n_past"] + 8)
+expect("store", INVALID, start=lambda a: a["n_out"])
+expect("store", INVALID, pos=lambda a: tensor(I32, 64, 2, 3, data=a["weight"].data + 256))
 expect("store", INVALID, weight=lambda a: tensor(F32, 63, 2, 3))
 expect("store", INVALID, weight=lambda a: tensor(F32, 64, 2, 3, nb=(4, 0, 256)))
 expect("store", INVALID, pos=lambda a: tensor(F32, 64, 2, 3))
@@ -136,6 +139,9 @@ expect("attn", OK, q=lambda a: tensor(F32, 64, 8, 3, nb=(4, 256, 0)))
 expect("attn", UNSUPPORTED, q=lambda a: tensor(F32, 64, 8, 3, nb=(4, 260, 2080)))
 expect("attn", INVALID, weight=lambda a: tensor(F32, 64, 8, 3))
 expect("attn", INVALID, weight=lambda a: tensor(F32, 64, 2, 3, data=a["dst"].data + 1024))
+one = dict(kc=lambda a: tensor(F16, 64, 16, 1, 10, nb=(2, 128, 7, 2048)), vc=lambda a: tensor(F16, 64, 16, 1, 10, nb=(2, 128, 7, 2048)), q=lambda a: tensor(F32, 64, 8, 3),
+           weight=lambda a: tensor(F32, 64, 1, 3, nb=(4, 1, 256)))
+expect("attn", OK, **one)                                                                      # (strides of one-element dimensions do not count)
 # evict
 for name in ("weight", "pos", "weight_out", "pos_out", "n_past", "n_out"):
     expect("evict", INVALID, **{name: None})

@@ -145,6 +145,18 @@ def test_attn_extreme_queries_and_masses(backend):
     check_attn(backend, c, 8, q=g(q), scale=0.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attn_a_query_that_is_no_number_stays_in_its_row(dtype, backend):
+    for lens in ([300, 40], [3000, 2000]):
+        c = Case(lens, dtype=dtype, seed=11)
+        q = c.rng.standard_normal((2, 8, 128)).astype(np.float32)
+        want, tol, _ = ref.attn(q.astype(np.float64), *c.host(), scale=0.1)
+        q[0, 1] = np.nan; q[1, 6, 5] = np.nan; q[1, 0, 0] = np.inf
+        got = host(backend.paged_attn(g(q), *c.dev(), scale=0.1))
+        bad = np.zeros((2, 8), bool); bad[0, 1] = bad[1, 6] = bad[1, 0] = True
+        assert np.isnan(got[bad]).all() and (np.abs(got - want) <= tol)[~bad].all()
+
+
 def test_attn_strided_arguments(backend):
     c = Case([70, 5, 129], heads_kv=2, page=32, seed=9)
     wide = g(c.rng.standard_normal((3, 24, 128)).astype(np.float32))
@@ -324,6 +336,70 @@ def test_fork_of_an_unmapped_or_overfull_tail(backend):
     np.testing.assert_array_equal(host(got_t), want_t); np.testing.assert_array_equal(host(got_n), want_n)
     assert (wide[:, [0, 4]] == 99).all()
     np.testing.assert_array_equal(host(k), kh); np.testing.assert_array_equal(host(v), vh)
+
+
+def test_store_evict_and_fork_past_32_bit_offsets(backend):
+    """the first and the last pages of a pool of more than 4 GiB"""
+    page, heads_kv, D, n_pages = 4096, 8, 128, 300
+    pool = torch.zeros(n_pages, 2, heads_kv, page, D, dtype=torch.float16, device=DEV)             # 5 GB
+    k, v = pool[:, 0], pool[:, 1]
+    table = torch.tensor([[299, 0]], dtype=torch.int32, device=DEV); n_kv = torch.tensor([4090], dtype=torch.int32, device=DEV)
+    kn, vn = (torch.randn(20, heads_kv, D, device=DEV) for _ in "kv")
+    n_kv = backend.paged_store(kn, vn, k, v, table, n_kv, start=torch.tensor([0, 20], dtype=torch.int32, device=DEV))
+    assert n_kv.tolist() == [4110]
+    for x, new in ((k, kn), (v, vn)):
+        assert torch.equal(x[299, :, 4090:], new[:6].half().transpose(0, 1)) and torch.equal(x[0, :, :14], new[6:].half().transpose(0, 1))
+        assert not x[299, :, :4090].any() and not x[0, :, 14:].any()
+    table2, n2 = backend.paged_fork(k, v, table, n_kv, torch.tensor([0], dtype=torch.int32, device=DEV), torch.tensor([298], dtype=torch.int32, device=DEV))
+    assert table2.tolist() == [[299, 298]] and n2.tolist() == [4110] and torch.equal(k[298, :, :14], k[0, :, :14]) and torch.equal(v[298, :, :14], v[0, :, :14]) and not v[298, :, 14:].any()
+    weight = torch.zeros(1, heads_kv, 8192, device=DEV); weight[:, :, 4100:4110] = 1
+    pos = torch.arange(8192, dtype=torch.int32, device=DEV).expand(1, heads_kv, 8192).contiguous()
+    n3 = backend.paged_evict(k, v, table2, n2, weight, pos, n2, 4096)
+    moved = torch.arange(4100, 4110, dtype=torch.int32, device=DEV).expand(heads_kv, 10)
+    assert n3.tolist() == [4096] and torch.equal(pos[0, :, 4086:4096], moved)
+    assert torch.equal(k[299, :, 4086:4096], kn[10:].half().transpose(0, 1)) and torch.equal(v[299, :, 4086:4096], vn[10:].half().transpose(0, 1))
+
+
+def test_recorded_calls_replay(backend):
+    """CallPlan: a store, an attention and a selection recorded once run again on what their tensors then hold"""
+    c = Case([33, 5], page=16, W=6, seed=12, junk=0.0)
+    k, v, table, n_kv = c.dev()
+    kn, vn, q = torch.randn(2, 2, 128, device=DEV), torch.randn(2, 2, 128, device=DEV), torch.randn(2, 8, 128, device=DEV)
+    x, score = torch.randn(2, 500, device=DEV), torch.zeros(2, device=DEV)
+    out, after = torch.zeros_like(q), torch.zeros_like(n_kv); outs = (torch.zeros(1, 3, device=DEV), torch.zeros(1, 3, dtype=torch.int32, device=DEV), torch.zeros(1, 3, dtype=torch.int32, device=DEV))
+
+    def step():
+        backend.paged_store(kn, vn, k, v, table, n_kv, n_kv_out=after)
+        backend.paged_attn(q, k, v, table, after, out=out)
+        backend.beam_select(x, score, 2, 3, outs=outs)
+    with backend.record() as plan:
+        step()
+    for i in range(3):
+        n_kv.copy_(after)
+        for y in (kn, vn, q, x):
+            y.normal_()
+        plan.replay(backend._check)
+        got = out.clone(), after.clone(), [o.clone() for o in outs]
+        step()
+        assert torch.equal(got[0], out) and torch.equal(got[1], after) and all(torch.equal(a, b) for a, b in zip(got[2], outs)) and after.tolist() == [35 + i, 7 + i]
+
+
+def test_fork_in_a_graph(backend):
+    c = Case([40, 17, 64], page=16, W=6, junk=0.5, spare=12, seed=13)
+    k, v, table, n_kv = c.dev()
+    parent, fresh = g(np.array([0, 0, 1, 2], np.int32)), g(c.spare[:4].copy())
+    table_out, n_out = torch.zeros(4, 6, dtype=torch.int32, device=DEV), torch.zeros(4, dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        backend.paged_fork(k, v, table, n_kv, parent, fresh, table_out=table_out, n_kv_out=n_out)
+    for i, (p, f) in enumerate((([0, 0, 1, 2], 0), ([2, 1, 1, -1], 4), ([1, 1, 1, 1], 8))):
+        parent.copy_(g(np.array(p, np.int32))); fresh.copy_(g(c.spare[f:f + 4].copy()))
+        kh, vh = host(k), host(v)
+        graph.replay(); torch.cuda.synchronize()
+        want_t, want_n = ref.fork(kh, vh, c.table, c.n_kv, p, c.spare[f:f + 4])
+        np.testing.assert_array_equal(host(table_out), want_t); np.testing.assert_array_equal(host(n_out), want_n)
+        np.testing.assert_array_equal(host(k), kh); np.testing.assert_array_equal(host(v), vh)
 
 
 # ---- together, as they are used
