@@ -15,6 +15,7 @@
 #include "fa_decode.cuh"
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
@@ -140,8 +141,10 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
         for (int c = 0; c < KC; ++c) { x0[c] = reinterpret_cast<const float4 *>(qr + 32 * c)[0]; x1[c] = reinterpret_cast<const float4 *>(qr + 32 * c)[1]; }
         const char *kb = a.c.k + (long)hk * a.c.k_head, *vb = a.c.v + (long)hk * a.c.v_head;
         const int *table = a.c.table + (long)s * a.c.table_row; const int in_page = (1 << a.c.page_shift) - 1;
-        // 16 slots from j on lie in one page (pages are powers of two >= 16): its id, -1 past the end or unmapped
-        auto page_of = [&](int j) { int id = -1; if (j < n) { id = table[j >> a.c.page_shift]; if ((unsigned)id >= (unsigned)a.c.n_pages) id = -1; } return id; };
+        // 16 slots from j on lie in one page (pages are powers of two >= 16).  Its entry in the table (requested without a branch: the last one stands for those past the end), and the id that
+        // this entry is: -1 past the end or unmapped
+        auto entry = [&](int j) { return table[min(j, max(n - 1, 0)) >> a.c.page_shift]; };
+        auto id_of = [&](int e, int j) { return j < n && (unsigned)e < (unsigned)a.c.n_pages ? e : -1; };
         const uint32_t k_lane = (uint32_t)col * (uint32_t)a.c.k_row + 16u * g, v_lane = 4u * g * (uint32_t)a.c.v_row + 2u * VW * col;
         u4 kr[2][KC]; uint32_t vr[8][VH][VW / 2];
         // (a half that is past the end or unmapped loads page 0: in bounds, and masked below)
@@ -178,33 +181,13 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
             for (int i = 0; i < VW; ++i) o[hf][i] = (f4){0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.f;
         int j = (tile0 * WAVES + wave) * 32; const int j_end = min((tile0 + ntile) * TILE, n);
-        int id0 = page_of(j), id1 = page_of(j + 16), nx0 = page_of(j + TILE), nx1 = page_of(j + TILE + 16);
         const int hc = min(col, heads - 1);
         float *score = !a.weight ? nullptr : ONE ? s_o + WAVES * heads * (D + 4) + hc * (int)a.score_row : a.score + ((long)s * a.n_head + h0 + hc) * a.score_row;
-        if (j < j_end) { load_k(j, id0, id1); load_v(j, id0, id1); }
-        u4 q[NS][KC]; float unscale = 1.0f;
-        {
-            float top = 0.f; const float pre_scale = CAP ? a.scale : a.scale * 1.44269504088896341f;
-            float up = 1.0f;
-            if constexpr (!BF16) {          // a power of two that puts the largest element into [2^10, 2^11): the f16 terms neither overflow nor lose bits to the smallest exponent
-#pragma unroll
-                for (int c = 0; c < KC; ++c) top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(x0[c].x), fabsf(x0[c].y)), fmaxf(fabsf(x0[c].z), fabsf(x0[c].w))),
-                                                                   fmaxf(fmaxf(fabsf(x1[c].x), fabsf(x1[c].y)), fmaxf(fabsf(x1[c].z), fabsf(x1[c].w)))));
-                top = over_rows(top, [](float p, float r) { return fmaxf(p, r); });
-                const int e = top > 0.f ? min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100), 110) : 0;
-                up = __uint_as_float((uint32_t)(127 + 10 - e) << 23); unscale = __uint_as_float((uint32_t)(127 - 10 + e) << 23);
-            }
-            unscale *= pre_scale;
-#pragma unroll
-            for (int c = 0; c < KC; ++c) {
-                const float e[8] = {x0[c].x, x0[c].y, x0[c].z, x0[c].w, x1[c].x, x1[c].y, x1[c].z, x1[c].w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) { uint32_t t[NS]; Split<BF16>::of(e[2 * i] * up, e[2 * i + 1] * up, t);
-#pragma unroll
-                    for (int k = 0; k < NS; ++k) q[k][c][i] = t[k]; }
-            }
-        }
-        while (j < j_end) {
+        u4 q[NS][KC]; float unscale = 1.0f; int id0 = -1, id1 = -1, nx0 = -1, nx1 = -1;
+        // One step: the tile in kr / vr.  MORE: the next tile is requested on the way, K as soon as its registers are read, V at the end.  (The last tile is a step of its own and not a
+        // condition around the loads: behind a condition the compiler waits for V of the next tile before the first product of K.)
+        auto step = [&](auto more) {
+            constexpr bool MORE = decltype(more)::value;
             f4 z[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -214,9 +197,8 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
 #pragma unroll
                     for (int k = NS - 1; k >= 0; --k) z[t] = mfma<BF16>(kr[t][c], q[k][c], z[t]);
             }
-            const int jn = j + TILE;
-            if (jn < j_end) load_k(jn, nx0, nx1);
-            const int nn0 = page_of(jn + TILE), nn1 = page_of(jn + TILE + 16);
+            const int jn = j + TILE; int e0 = 0, e1 = 0;
+            if constexpr (MORE) { load_k(jn, nx0, nx1); e0 = entry(jn + TILE); e1 = entry(jn + TILE + 16); }
             const bool whole = id0 >= 0 && id1 >= 0 && j + 32 <= n;          // (wave-uniform)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -276,8 +258,36 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
 #pragma unroll
                     for (int k = NS - 1; k >= 0; --k) o[hf][i] = mfma<BF16>(vt, (u4){p[k][0], p[k][1], p[k][2], p[k][3]}, o[hf][i]);
                 }
-            if (jn < j_end) load_v(jn, nx0, nx1);
-            id0 = nx0; id1 = nx1; nx0 = nn0; nx1 = nn1; j = jn;
+            if constexpr (MORE) { load_v(jn, nx0, nx1); id0 = nx0; id1 = nx1; nx0 = id_of(e0, jn + TILE); nx1 = id_of(e1, jn + TILE + 16); j = jn; }
+        };
+        if (j < j_end) {
+            const int e0 = entry(j), e1 = entry(j + 16), e2 = entry(j + TILE), e3 = entry(j + TILE + 16);
+            id0 = id_of(e0, j); id1 = id_of(e1, j + 16); nx0 = id_of(e2, j + TILE); nx1 = id_of(e3, j + TILE + 16);
+            load_k(j, id0, id1); load_v(j, id0, id1);
+            __builtin_amdgcn_sched_barrier(0);          // (V too is requested before the split of the queries)
+        {
+            float top = 0.f; const float pre_scale = CAP ? a.scale : a.scale * 1.44269504088896341f;
+            float up = 1.0f;
+            if constexpr (!BF16) {          // a power of two that puts the largest element into [2^10, 2^11): the f16 terms neither overflow nor lose bits to the smallest exponent
+#pragma unroll
+                for (int c = 0; c < KC; ++c) top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(x0[c].x), fabsf(x0[c].y)), fmaxf(fabsf(x0[c].z), fabsf(x0[c].w))),
+                                                                   fmaxf(fmaxf(fabsf(x1[c].x), fabsf(x1[c].y)), fmaxf(fabsf(x1[c].z), fabsf(x1[c].w)))));
+                top = over_rows(top, [](float p, float r) { return fmaxf(p, r); });
+                const int e = top > 0.f ? min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100), 110) : 0;
+                up = __uint_as_float((uint32_t)(127 + 10 - e) << 23); unscale = __uint_as_float((uint32_t)(127 - 10 + e) << 23);
+            }
+            unscale *= pre_scale;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const float e[8] = {x0[c].x, x0[c].y, x0[c].z, x0[c].w, x1[c].x, x1[c].y, x1[c].z, x1[c].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { uint32_t t[NS]; Split<BF16>::of(e[2 * i] * up, e[2 * i + 1] * up, t);
+#pragma unroll
+                    for (int k = 0; k < NS; ++k) q[k][c][i] = t[k]; }
+            }
+        }
+            while (j + TILE < j_end) step(std::true_type());
+            step(std::false_type());
         }
         // the four waves' results: (m, l) through LDS, then the accumulators on the common maximum
         l = over_rows(l, [](float p, float r) { return p + r; });
@@ -285,7 +295,13 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
         __syncthreads();                                                  // (the previous unit's reads of s_o are done)
         if (g == 0) { s_m[wave][col] = m; s_l[wave][col] = l; }
         __syncthreads();
-        const float M = fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col])), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+        const float m0 = s_m[0][col], m1 = s_m[1][col], m2 = s_m[2][col], m3 = s_m[3][col], M = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)), to = M == -INFINITY ? 0.f : M;
+        const float f = __builtin_amdgcn_exp2f(m - to);                   // (0 for a wave that had nothing)
+        if (wave == 0 && g == 0) {
+            s_row[0][col] = M;
+            s_row[1][col] = (s_l[0][col] * __builtin_amdgcn_exp2f(m0 - to) + s_l[1][col] * __builtin_amdgcn_exp2f(m1 - to)) +
+                            (s_l[2][col] * __builtin_amdgcn_exp2f(m2 - to) + s_l[3][col] * __builtin_amdgcn_exp2f(m3 - to));
+        }
         if (col < heads) {
             float *so = s_o + (wave * heads + col) * (D + 4);
 #pragma unroll
@@ -301,18 +317,13 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
         float *part = ONE ? nullptr : a.part + ((long)blockIdx.x * 2 + (first ? 0 : 1)) * QH * (D + 2);
         for (int e = threadIdx.x; e < heads * D / 4; e += 256) {
             const int h = e / (D / 4), d = (e - h * (D / 4)) * 4;
-            const float Mh = fmaxf(fmaxf(s_m[0][h], s_m[1][h]), fmaxf(s_m[2][h], s_m[3][h]));
-            float L = 0.f; f4 v = (f4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
-                if (s_m[w][h] != -INFINITY) L += s_l[w][h] * __builtin_amdgcn_exp2f(s_m[w][h] - Mh);
-                v += *reinterpret_cast<const f4 *>(s_o + (w * heads + h) * (D + 4) + d);
-            }
+            const float Mh = s_row[0][h], L = s_row[1][h];
+            const float *so = s_o + h * (D + 4) + d; const int next = heads * (D + 4);
+            f4 v = (*reinterpret_cast<const f4 *>(so) + *reinterpret_cast<const f4 *>(so + next)) + (*reinterpret_cast<const f4 *>(so + 2 * next) + *reinterpret_cast<const f4 *>(so + 3 * next));
             if (alone) {
                 if (Mh == -INFINITY) v = (f4){0.f, 0.f, 0.f, 0.f}; else v /= L;          // (nothing to attend to: a row of zeros)
                 *reinterpret_cast<f4 *>(a.dst + (long)s * a.d_seq + (long)(h0 + h) * a.d_head + d * 4) = v;
-                if (ONE) { if (d == 0) { s_row[0][h] = Mh; s_row[1][h] = 1.0f / L; } }
-                else if (d == 0 && a.stat) a.stat[(long)s * a.n_head + h0 + h] = make_float2(Mh, L);
+                if (!ONE && d == 0 && a.stat) a.stat[(long)s * a.n_head + h0 + h] = make_float2(Mh, L);
             } else {
                 float *ph = part + h * (D + 2);
                 if (d == 0) { ph[0] = Mh; ph[1] = L; }
@@ -320,12 +331,11 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
             }
         }
         if (ONE && a.weight) {          // (one unit to a KV head: the host has seen to it)
-            __syncthreads();
             const float *z = s_o + WAVES * heads * (D + 4);
             float *w = reinterpret_cast<float *>(a.weight + (long)s * a.w_seq + (long)hk * a.w_head);
             for (int i = threadIdx.x; i < n; i += 256) {          // one thread to a slot, the heads in order
                 float sum = 0.f;
-                for (int h = 0; h < heads; ++h) if (s_row[0][h] != -INFINITY) sum += __builtin_amdgcn_exp2f(z[h * (int)a.score_row + i] - (s_row[0][h] - 8.0f)) * s_row[1][h];
+                for (int h = 0; h < heads; ++h) if (s_row[0][h] != -INFINITY) sum += __builtin_amdgcn_exp2f(z[h * (int)a.score_row + i] - (s_row[0][h] - 8.0f)) / s_row[1][h];
                 if (sum != 0.f) w[i] += sum;
             }
         }
@@ -466,6 +476,7 @@ int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_t
     if (pg_empty(q)) return CDNA4_OK;
     ARG_CHECK(n_kv && q->data && dst->data && (a.c.W == 0 || (a.c.table && (!weight || weight->data))), "paged_attn: null data");
     ARG_CHECK(!pg_overlap(q, 4, dst, 4) && (!weight || a.c.W == 0 || (!pg_overlap(weight, 4, dst, 4) && !pg_overlap(weight, 4, q, 4))), "paged_attn: q, dst and weight may not overlap");
+    if (a.c.W == 0) { a.c.table = n_kv; a.c.table_row = 0; }          // (no slots: the entry that is read for a missing one is anything)
     a.c.n_kv = n_kv; a.scale = scale; a.softcap = softcap; a.inv_softcap = softcap != 0.0f ? 1.0f / softcap : 0.0f;
     a.q = (const char *)q->data; a.q_head = q->nb[1]; a.q_seq = q->nb[2]; a.dst = (char *)dst->data; a.d_head = dst->nb[1]; a.d_seq = dst->nb[2];
     a.weight = weight ? (char *)weight->data : nullptr; a.w_head = weight ? weight->nb[1] : 0; a.w_seq = weight ? weight->nb[2] : 0;

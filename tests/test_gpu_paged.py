@@ -73,6 +73,14 @@ def check_attn(be, c, heads, scale=None, softcap=0.0, weight=None, q=None, out=N
     return got
 
 
+@pytest.mark.parametrize("heads_kv,heads", [(1, 1), (2, 6), (1, 8), (2, 14), (1, 16), (1, 17), (2, 40), (1, 71)])
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("D,dtype", [(64, torch.bfloat16), (128, torch.float16), (256, torch.float16)])
+def test_attn_groups_of_short_tables(D, dtype, heads_kv, heads, weights, backend):
+    c = Case([37, 0, 200, 511], D=D, dtype=dtype, heads_kv=heads_kv, page=16, W=32, seed=heads)
+    check_attn(backend, c, heads, weight=c.slots() if weights else None, softcap=15.0 if heads % 2 else 0.0)
+
+
 LENS = [0, 1, 15, 16, 17, 31, 32, 33, 63, 127, 128, 129, 300]
 
 
@@ -133,6 +141,16 @@ def test_attn_unmapped_pages_inactive_rows_and_oversized_lengths(junk, backend):
         x[g(c.table[3].astype(np.int64))] = 0.25
     out = check_attn(backend, c, 4, weight=c.slots())
     assert (host(out)[[1, 2]] == 0).all()
+
+
+@pytest.mark.parametrize("size", [2e-6, 2e4])
+def test_attn_smallest_and_largest_cache_values(size, backend):
+    """f16 subnormals (K and V of 10^-6) and rows near the largest f16 keep their value: the bound of every element is relative to |k| and |v|"""
+    for lens in ([300, 64], [2100, 2000]):
+        c = Case(lens, seed=15, junk=0.0)
+        for x in c.caches:
+            x.copy_((x.float() * size).clamp(-65504, 65504).half())
+        check_attn(backend, c, 8, scale=0.5 / size, weight=c.slots())
 
 
 def test_attn_extreme_queries_and_masses(backend):
@@ -400,6 +418,30 @@ def test_fork_in_a_graph(backend):
         want_t, want_n = ref.fork(kh, vh, c.table, c.n_kv, p, c.spare[f:f + 4])
         np.testing.assert_array_equal(host(table_out), want_t); np.testing.assert_array_equal(host(n_out), want_n)
         np.testing.assert_array_equal(host(k), kh); np.testing.assert_array_equal(host(v), vh)
+
+
+def test_tables_of_no_pages_and_batches_of_nothing(backend):
+    """W = 0: nothing can be held; n_seq = 0, no tokens, no rows: nothing happens"""
+    c = Case([16, 16], page=16, W=1, junk=0.5, seed=14)
+    k, v, _, _ = c.dev(); k0, v0 = k.clone(), v.clone()
+    table, n_kv = torch.empty(2, 0, dtype=torch.int32, device=DEV), torch.tensor([5, -1], dtype=torch.int32, device=DEV)
+    q, rows = torch.randn(2, 4, 128, device=DEV), torch.randn(2, 2, 128, device=DEV)
+    weight, pos = torch.empty(2, 2, 0, device=DEV), torch.empty(2, 2, 0, dtype=torch.int32, device=DEV)
+    assert not backend.paged_attn(q, k, v, table, n_kv).any() and not backend.paged_attn(q, k, v, table, n_kv, weight=weight).any()
+    assert backend.paged_store(rows, rows, k, v, table, n_kv, n_past=n_kv, weight=weight, pos=pos).tolist() == [0, -1]
+    assert backend.paged_evict(k, v, table, n_kv, weight, pos, n_kv, 3).tolist() == [0, -1]
+    t2, n2 = backend.paged_fork(k, v, table, n_kv, torch.tensor([0, 1, 5], dtype=torch.int32, device=DEV), torch.tensor([0, 1, 1], dtype=torch.int32, device=DEV))
+    assert t2.shape == (3, 0) and n2.tolist() == [0, -1, -1]
+    none, empty = torch.empty(0, 1, dtype=torch.int32, device=DEV), torch.empty(0, dtype=torch.int32, device=DEV)
+    assert backend.paged_attn(q[:0], k, v, none, empty).shape == (0, 4, 128)
+    assert backend.paged_store(rows[:0], rows[:0], k, v, none, empty).numel() == 0
+    full = g(c.table)
+    assert backend.paged_store(rows[:0], rows[:0], k, v, full, n_kv, start=torch.zeros(3, dtype=torch.int32, device=DEV)).tolist() == [5, -1]
+    t3, n3 = backend.paged_fork(k, v, full, n_kv, empty, empty)
+    assert t3.shape == (0, 1) and n3.numel() == 0
+    assert all(x.shape == (0, 2) for x in backend.beam_select(torch.empty(0, 10, device=DEV), torch.empty(0, device=DEV), 3, 2))
+    torch.cuda.synchronize()
+    assert torch.equal(k, k0) and torch.equal(v, v0)
 
 
 # ---- together, as they are used
