@@ -2,6 +2,7 @@
 //
 // The logits are read once (4 bytes a candidate against a handful of operations: bound by that read).  A workgroup takes 8192 (2048) neighbouring logits of a row into registers and leaves
 // their maximum, the sum of their exponentials and their n_out best, sorted; a second launch joins a group's chunks: log sum exp of every beam, then the best of the sorted lists.
+// Measured: 256 rows of 128256 (131 MB), 32 groups of 8, 16 results: 29 us for the chunks (4.5 TB/s) and 9 us for the join; 4 rows of 32000: 4.1 and 4.9 us.
 //
 // Choosing the k best of many without sorting them: in a total order without ties, the k-th best of the threads' (or lanes' quads') own best elements is a bound that at least k elements
 // reach, and every element that reaches it belongs to one of the k owners whose best does -- so the collected list is never longer than k shares, whatever the values, and in random order

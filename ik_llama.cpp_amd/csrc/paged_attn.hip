@@ -11,6 +11,9 @@
 // * Equal shares: all tiles of 128 slots of all (sequence, KV head, 16 query heads) units are numbered through, and every workgroup takes an equal contiguous range of the numbers, from
 //   the lengths as they are on the device.  A long sequence in a batch of short ones spreads over the chip by itself; a workgroup that covers a unit alone writes its result, the others
 //   leave (max, sum, accumulator) for the join.
+//
+// Measured (8 KV heads of 128): 64 sequences of up to 8192 slots, f16, 32 query heads: 1.12 GB in 197 us + 6 us for the join, 5.5 TB/s; one of 131071, bf16, 64 query heads: 537 MB in 92 -
+// 105 us + 5 us; one of 301 slots: 6.8 us.  The first form, a wave per slot and a workgroup per KV head, took 10.7 ms, 336 ms and 192 us.
 #include "paged.cuh"
 #include "fa_decode.cuh"
 #include <algorithm>
@@ -485,11 +488,12 @@ int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_t
     const bool bf = k_cache->type == CDNA4_TYPE_BF16, cap = softcap != 0.0f;
     hipStream_t st = (hipStream_t)stream;
     const size_t merge = (size_t)WAVES * std::min(QH, a.group) * (a.c.D + 4) * 4;
-    // A workgroup per unit where a unit is little work, or where there are enough units and none is long (a unit of 16 tiles takes 24 us by itself).  Measured, us with a workgroup per
-    // unit / with equal shares and a join (32 query heads, 8 KV heads of 128; sequences x slots): 1 x 100: 6.6 / 9.6, 1 x 512: 9.9 / 11.8, 1 x 1024: 14.4 / 11.8, 8 x 1024: 15.3 / 14.8,
-    // 64 x 512: 17.8 / 26.4, 64 x 2048: 58 / 61, 256 x 512: 56 / 80, 256 x 2048: 205 / 222.  With weights: if a KV head is one unit and its scores fit LDS.
+    // A workgroup per unit where a unit is little work, or where the units fill the chip and none is long.  Measured, us with a workgroup per unit / with equal shares and a join (f16, 32
+    // query heads and 8 KV heads of 128; sequences x slots): 1 x 100: 5.9 / 8.8, 1 x 640: 9.8 / 10.5, 1 x 1024: 13.0 / 10.6, 8 x 1024: 13.4 / 13.2, 32 x 1024: 16.9 / 23.2, 64 x 512: 16.7 /
+    // 24.4, 64 x 2048: 56 / 62, 256 x 2048: 204 / 223; bf16, 4 heads of 64, 1 x 768: 7.8 / 9.6; of 256, 1 x 512: 14.3 / 13.0, 128 x 2048: 111 / 110.
+    // With weights: if a KV head is one unit and its scores fit LDS.
     const size_t one_lds = merge + (weight ? (size_t)a.group * a.score_row * 4 : 0);
-    const bool one = (row_tiles <= 4 || (row_tiles <= 16 && (long)a.c.n_seq * a.n_unit >= 2l * ctx->num_cu)) && (!weight || a.group <= QH) && one_lds <= ONE_LDS;
+    const bool one = (row_tiles * a.c.D <= 640 || (row_tiles <= 16 && (long)a.c.n_seq * a.n_unit >= ctx->num_cu)) && (!weight || a.group <= QH) && one_lds <= ONE_LDS;
 #define ATTN(D_, B_, C_, O_, grid, lds) do { if ((lds) > 60 * 1024) HIP_TRY((pg_opt_in_lds<paged_attn_kernel<D_, B_, C_, O_>>(ctx->device, ONE_LDS))); \
                                              hipLaunchKernelGGL((paged_attn_kernel<D_, B_, C_, O_>), grid, dim3(256), lds, st, a); } while (0)
 #define ATTN_D(D_, O_, grid, lds) do { if (bf) { if (cap) ATTN(D_, true, true, O_, grid, lds); else ATTN(D_, true, false, O_, grid, lds); } \
