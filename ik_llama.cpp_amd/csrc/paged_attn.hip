@@ -268,7 +268,6 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
             id0 = id_of(e0, j); id1 = id_of(e1, j + 16); nx0 = id_of(e2, j + TILE); nx1 = id_of(e3, j + TILE + 16);
             load_k(j, id0, id1); load_v(j, id0, id1);
             __builtin_amdgcn_sched_barrier(0);          // (V too is requested before the split of the queries)
-        {
             float top = 0.f; const float pre_scale = CAP ? a.scale : a.scale * 1.44269504088896341f;
             float up = 1.0f;
             if constexpr (!BF16) {          // a power of two that puts the largest element into [2^10, 2^11): the f16 terms neither overflow nor lose bits to the smallest exponent
@@ -276,7 +275,7 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
                 for (int c = 0; c < KC; ++c) top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(x0[c].x), fabsf(x0[c].y)), fmaxf(fabsf(x0[c].z), fabsf(x0[c].w))),
                                                                    fmaxf(fmaxf(fabsf(x1[c].x), fabsf(x1[c].y)), fmaxf(fabsf(x1[c].z), fabsf(x1[c].w)))));
                 top = over_rows(top, [](float p, float r) { return fmaxf(p, r); });
-                const int e = top > 0.f ? min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100), 110) : 0;
+                const int e = top > 0.f ? min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100), 127) : 0;
                 up = __uint_as_float((uint32_t)(127 + 10 - e) << 23); unscale = __uint_as_float((uint32_t)(127 - 10 + e) << 23);
             }
             unscale *= pre_scale;
@@ -288,7 +287,6 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
 #pragma unroll
                     for (int k = 0; k < NS; ++k) q[k][c][i] = t[k]; }
             }
-        }
             while (j + TILE < j_end) step(std::true_type());
             step(std::false_type());
         }
@@ -338,7 +336,10 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
             float *w = reinterpret_cast<float *>(a.weight + (long)s * a.w_seq + (long)hk * a.w_head);
             for (int i = threadIdx.x; i < n; i += 256) {          // one thread to a slot, the heads in order
                 float sum = 0.f;
-                for (int h = 0; h < heads; ++h) if (s_row[0][h] != -INFINITY) sum += __builtin_amdgcn_exp2f(z[h * (int)a.score_row + i] - (s_row[0][h] - 8.0f)) / s_row[1][h];
+                for (int h = 0; h < heads; ++h) {
+                    const float zi = z[h * (int)a.score_row + i];          // -inf: not attended to, whatever the row is
+                    if (zi != -INFINITY) sum += __builtin_amdgcn_exp2f(zi - (s_row[0][h] - 8.0f)) / s_row[1][h];
+                }
                 if (sum != 0.f) w[i] += sum;
             }
         }
@@ -393,7 +394,7 @@ template <int D> static __device__ __forceinline__ void add_weights(const AttnAr
             if (st.x == -INFINITY) continue;
             const f4 z = *reinterpret_cast<const f4 *>(a.score + ((long)s * a.n_head + hk * a.group + h0 + i) * a.score_row + j);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] += __builtin_amdgcn_exp2f(z[e] - (st.x - 8.0f)) * st.y;
+            for (int e = 0; e < 4; ++e) if (z[e] != -INFINITY) sum[e] += __builtin_amdgcn_exp2f(z[e] - (st.x - 8.0f)) * st.y;          // (-inf: not attended to, whatever the row is)
         }
     }
     float *w = reinterpret_cast<float *>(a.weight + (long)s * a.w_seq + (long)hk * a.w_head);

@@ -175,6 +175,28 @@ def test_attn_a_query_that_is_no_number_stays_in_its_row(dtype, backend):
         assert np.isnan(got[bad]).all() and (np.abs(got - want) <= tol)[~bad].all()
 
 
+def test_attn_queries_near_the_largest_float(backend):
+    """f16 terms of a query are taken of q scaled by a power of two, whatever its size"""
+    c = Case([300, 40], seed=16)
+    for size in (3e38, 1e36, 1e30, 1e-30):
+        q = c.rng.uniform(-1, 1, (2, 8, 128)).astype(np.float32) * np.float32(size)
+        check_attn(backend, c, 8, q=g(q), scale=float(np.float32(0.1) / np.float32(size)) if size < 1e37 else 1e-37)
+
+
+def test_attn_weights_of_a_row_that_is_no_number(backend):
+    """NaN reaches the slots that were attended to and no others"""
+    for lens, W in (([100], 7), ([3000], 190)):
+        c = Case(lens, page=16, W=W, seed=17)
+        c.table[0, 2] = -1
+        q = c.rng.standard_normal((1, 4, 128)).astype(np.float32); q[0, 1] = np.nan          # heads 0, 1 share the first KV head
+        k, v, table, n_kv = c.dev(); w = c.slots(); before = w.clone()
+        backend.paged_attn(g(q), k, v, table, n_kv, weight=w)
+        n = lens[0]; hole = slice(32, 48)
+        assert torch.equal(w[0, :, hole], before[0, :, hole]) and torch.equal(w[0, :, n:], before[0, :, n:])
+        seen = torch.ones(n, dtype=torch.bool, device=DEV); seen[hole] = False
+        assert w[0, 0, :n][seen].isnan().all() and not w[0, 1].isnan().any()
+
+
 def test_attn_strided_arguments(backend):
     c = Case([70, 5, 129], heads_kv=2, page=32, seed=9)
     wide = g(c.rng.standard_normal((3, 24, 128)).astype(np.float32))
