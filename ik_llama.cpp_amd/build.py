@@ -107,6 +107,31 @@ def build_library(force=False, verbose=False, extra_flags=(), out=None, tag=None
     return LIB
 
 
+BINDING = os.path.join(HERE, "cdna4_args.so")
+
+
+def build_binding(force=False, verbose=False):
+    """Compile the binding's C++ part (csrc/binding_args.cpp: torch tensors into descriptors; host code only) against the torch and Python of this interpreter.  Returns its path."""
+    import sysconfig
+    import torch
+    src = os.path.join(CSRC, "binding_args.cpp"); inc = os.path.join(os.path.dirname(torch.__file__), "include"); lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
+           "-I" + inc, "-I" + os.path.join(inc, "torch", "csrc", "api", "include"), "-I" + sysconfig.get_paths()["include"], src, "-o", BINDING + ".tmp",
+           "-L" + lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+    h = hashlib.sha256((" ".join(cmd) + torch.__version__).encode()); h.update(open(src, "rb").read())
+    os.makedirs(OBJDIR, exist_ok=True)
+    stamp = os.path.join(OBJDIR, "binding_args.sha")
+    if not force and os.path.exists(BINDING) and os.path.exists(stamp) and open(stamp).read() == h.hexdigest():
+        return BINDING
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    os.replace(BINDING + ".tmp", BINDING)
+    open(stamp, "w").write(h.hexdigest())
+    return BINDING
+
+
 if __name__ == "__main__":
     import sys
     print(build_library(force="--force" in sys.argv, verbose=True))
+    print(build_binding(force="--force" in sys.argv, verbose=True))

@@ -1,7 +1,6 @@
 """ctypes binding of include/ggml_hip_cdna4.h (the C-ABI drop-in boundary)."""
 import ctypes as C
 import os
-import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 
@@ -158,8 +157,7 @@ def load_library(path=None):
     # torch ships its own libamdhip64 / librccl; whichever HIP runtime is loaded FIRST serves the whole process.  Load torch's before ours
     # so that tensors and kernels share one runtime (loading this library first made a later `import torch` see no device).
     try:
-        import torch
-        _DESC_TYPES.update({torch.float32: (T["F32"], 4), torch.float16: (T["F16"], 2), torch.bfloat16: (T["BF16"], 2), torch.int32: (26, 4)})
+        import torch  # noqa: F401
     except ImportError:
         pass
     lib = C.CDLL(p)
@@ -176,8 +174,23 @@ def load_library(path=None):
     return lib
 
 
-_pack_desc = struct.Struct("@Pi8q").pack          # cdna4_tensor {data, type, ne[4], nb[4]} (include/ggml_hip_cdna4.h); native alignment
-_DESC_TYPES = {}          # torch dtype -> (type id, bytes); filled by load_library, which brings torch
+_args = None
+
+
+def load_args():
+    """The binding's C++ part (csrc/binding_args.cpp): descriptors of torch tensors for the paged calls.  Raises if it is not built; there is no other form of it."""
+    global _args
+    if _args is None:
+        import importlib.util
+        import torch  # noqa: F401  (its libraries are what the module is linked against)
+        p = os.path.join(HERE, "cdna4_args.so")
+        if not os.path.exists(p):
+            raise FileNotFoundError("%s not found: build it with `python -m ik_llama.cpp_amd.build` / __graft_entry__.build()" % p)
+        spec = importlib.util.spec_from_file_location("cdna4_args", p)
+        m = importlib.util.module_from_spec(spec); spec.loader.exec_module(m)
+        m.set_error(Cdna4Error)
+        _args = m
+    return _args
 
 
 class _Fusion(C.Structure):      # cdna4_fusion {norm_w, norm_eps, residual, qkv, add_b, add_dst} (include/ggml_hip_cdna4.h)
@@ -230,7 +243,7 @@ class Cdna4Backend:
             raise Cdna4Error(-3, self.lib.cdna4_last_error().decode())
         self.comm = None
         self.window = None
-        self._i32 = torch.int32; self._i0 = torch.empty(0, dtype=torch.int32, device=self.device)          # (new_empty of it: an int32 tensor at half the price of torch.empty)
+        args = load_args(); self._desc, self._vec, self._empty, self._dev = args.desc, args.vec, args.empty, device
 
     def close(self):
         self.window_free()
@@ -437,110 +450,81 @@ class Cdna4Backend:
     # Caches are torch.float16 / torch.bfloat16 [n_pages, n_head_kv, page, D] views of any strides with dense rows (token-major pages: x.transpose(1, 2)), tables int32 [n_seq, W]; n_kv,
     # n_past, start, parent, fresh and done are dense int32 vectors, weight / pos float32 / int32 [n_seq, n_head_kv, >= W * page], all on the backend's device.  What the library refuses
     # raises Cdna4Error before anything is launched.
-    # These calls are short on the device (5 to 20 us), so the host's share counts: descriptors are packed into bytes (ctypes structures cost several times as much).
-    def _desc(self, x, name):
-        """cdna4_tensor {data, type, ne[4], nb[4]} of a torch tensor of at most 4 dimensions: sizes and byte strides from the innermost dimension out"""
-        try:
-            ty, es = _DESC_TYPES[x.dtype]
-            here = x.device == self.device
-        except (AttributeError, KeyError):
-            here = False
-        if not here:
-            raise Cdna4Error(-2, "%s: a float32 / float16 / bfloat16 / int32 tensor on %s" % (name, self.device))
-        n = x.dim()
-        if n == 3:
-            (c, b, a), (r, q, p) = x.shape, x.stride()
-            return _pack_desc(x.data_ptr(), ty, a, b, c, 1, p * es, q * es, r * es, 0)
-        if n == 4:
-            (d, c, b, a), (s, r, q, p) = x.shape, x.stride()
-            return _pack_desc(x.data_ptr(), ty, a, b, c, d, p * es, q * es, r * es, s * es)
-        if n == 2:
-            (b, a), (q, p) = x.shape, x.stride()
-            return _pack_desc(x.data_ptr(), ty, a, b, 1, 1, p * es, q * es, 0, 0)
-        raise Cdna4Error(-2, "%s: 2 to 4 dimensions" % name)
-
-    def _vec(self, x, name, n, dtype=None):
-        """address of a dense vector of n elements (int32 unless said), None for None"""
-        if x is None:
-            return None
-        try:
-            fits = x.dtype == (dtype or self._i32) and x.device == self.device and x.numel() == n and x.is_contiguous()
-        except AttributeError:
-            fits = False
-        if not fits:
-            raise Cdna4Error(-2, "%s: a dense %s vector of %d elements on %s" % (name, dtype or self._i32, n, self.device))
-        return x.data_ptr()
-
+    # These calls are short on the device (5 to 20 us), so the host's share counts: descriptors are made in C++ (csrc/binding_args.cpp).
     def paged_store(self, k, v, k_cache, v_cache, table, n_kv, start=None, n_past=None, weight=None, pos=None, n_kv_out=None):
         """cdna4_op_paged_store: k, v f32 [n_tok, n_head_kv, D] into the slots behind n_kv (start int32 [n_seq + 1]: token ranges of the sequences, None: one token each); returns the new n_kv."""
-        td = self._desc(table, "table"); n = table.shape[-2]
+        d, vec, dev = self._desc, self._vec, self._dev
+        td = d(table, "table", dev); n = table.shape[-2]
         if n_kv_out is None:
-            n_kv_out = table.new_empty(n)
-        self._check(self.lib.cdna4_op_paged_store(self.ctx, self._desc(k, "k"), self._desc(v, "v"), self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), td,
-                                                  self._vec(n_kv, "n_kv", n), self._vec(start, "start", n + 1), self._vec(n_past, "n_past", n),
-                                                  None if weight is None else self._desc(weight, "weight"), None if pos is None else self._desc(pos, "pos"),
-                                                  self._vec(n_kv_out, "n_kv_out", n), self._stream()))
+            n_kv_out = self._empty(table, 26, n)
+        self._check(self.lib.cdna4_op_paged_store(self.ctx, d(k, "k", dev), d(v, "v", dev), d(k_cache, "k_cache", dev), d(v_cache, "v_cache", dev), td, vec(n_kv, "n_kv", n, 26, dev),
+                                                  vec(start, "start", n + 1, 26, dev), vec(n_past, "n_past", n, 26, dev), None if weight is None else d(weight, "weight", dev),
+                                                  None if pos is None else d(pos, "pos", dev), vec(n_kv_out, "n_kv_out", n, 26, dev), self._stream()))
         return n_kv_out
 
     def paged_attn(self, q, k_cache, v_cache, table, n_kv, scale=None, softcap=0.0, weight=None, out=None):
         """cdna4_op_paged_attn: q f32 [n_seq, n_head, D] -> f32 [n_seq, n_head, D]; scale None: 1 / sqrt(D); weight: += the attention weight that every slot gathers, in place."""
-        qd, td = self._desc(q, "q"), self._desc(table, "table")
+        d, dev = self._desc, self._dev
+        qd, td = d(q, "q", dev), d(table, "table", dev)
         if out is None:
-            out = q.new_empty(q.shape)
-        self._check(self.lib.cdna4_op_paged_attn(self.ctx, qd, self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), td,
-                                                 self._vec(n_kv, "n_kv", table.shape[-2]), None if weight is None else self._desc(weight, "weight"), self._desc(out, "out"),
-                                                 float(q.shape[-1] ** -0.5 if scale is None else scale), float(softcap), self._stream()))
+            out = self._empty(q, 0, *q.shape)
+        self._check(self.lib.cdna4_op_paged_attn(self.ctx, qd, d(k_cache, "k_cache", dev), d(v_cache, "v_cache", dev), td, self._vec(n_kv, "n_kv", table.shape[-2], 26, dev),
+                                                 None if weight is None else d(weight, "weight", dev), d(out, "out", dev), q.shape[-1] ** -0.5 if scale is None else scale, softcap,
+                                                 self._stream()))
         return out
 
     def paged_evict(self, k_cache, v_cache, table, n_kv, weight, pos, n_past, budget, n_sink=0, n_recent=0, weight_out=None, pos_out=None, n_kv_out=None):
         """cdna4_op_paged_evict: every (sequence, KV head) keeps `budget` slots, by position and gathered weight; weight_out / pos_out None: in place.  Returns the new n_kv."""
-        td = self._desc(table, "table"); n = table.shape[-2]
+        d, vec, dev = self._desc, self._vec, self._dev
+        td = d(table, "table", dev); n = table.shape[-2]
         if n_kv_out is None:
-            n_kv_out = table.new_empty(n)
-        self._check(self.lib.cdna4_op_paged_evict(self.ctx, self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), td, self._vec(n_kv, "n_kv", n),
-                                                  self._desc(weight, "weight"), self._desc(pos, "pos"), self._vec(n_past, "n_past", n), budget, n_sink, n_recent,
-                                                  self._desc(weight if weight_out is None else weight_out, "weight_out"), self._desc(pos if pos_out is None else pos_out, "pos_out"),
-                                                  self._vec(n_kv_out, "n_kv_out", n), self._stream()))
+            n_kv_out = self._empty(table, 26, n)
+        wd, pd = d(weight, "weight", dev), d(pos, "pos", dev)
+        self._check(self.lib.cdna4_op_paged_evict(self.ctx, d(k_cache, "k_cache", dev), d(v_cache, "v_cache", dev), td, vec(n_kv, "n_kv", n, 26, dev), wd, pd, vec(n_past, "n_past", n, 26, dev),
+                                                  budget, n_sink, n_recent, wd if weight_out is None else d(weight_out, "weight_out", dev),
+                                                  pd if pos_out is None else d(pos_out, "pos_out", dev), vec(n_kv_out, "n_kv_out", n, 26, dev), self._stream()))
         return n_kv_out
 
     def beam_select(self, logits, score, n_beam, n_out, done=None, pad=0, outs=None):
         """cdna4_op_beam_select: logits f32 [n_group * n_beam, n_vocab], score f32 [n_group * n_beam] -> (score f32, parent row int32, token int32), each [n_group, n_out]."""
-        d = self._desc(logits, "logits")
-        rows = logits.shape[0]; n_group = rows // n_beam if n_beam > 0 else 0
+        vec, dev = self._vec, self._dev
+        ld = self._desc(logits, "logits", dev)
+        rows = logits.shape[-2]; n_group = rows // n_beam if n_beam > 0 else 0
         if outs is None:
-            shape = (n_group, max(n_out, 0))
-            parent = self._i0.new_empty(shape)
-            outs = (logits.new_empty(shape), parent, self.torch.empty_like(parent))
-        f32, m = self.torch.float32, n_group * n_out
-        self._check(self.lib.cdna4_op_beam_select(self.ctx, d, self._vec(score, "score", rows, f32), self._vec(done, "done", rows), n_beam, n_out, pad,
-                                                  self._vec(outs[0], "score_out", m, f32), self._vec(outs[1], "parent", m), self._vec(outs[2], "token", m), self._stream()))
+            k = max(n_out, 0)
+            outs = (self._empty(logits, 0, n_group, k), self._empty(logits, 26, n_group, k), self._empty(logits, 26, n_group, k))
+        m = n_group * n_out
+        self._check(self.lib.cdna4_op_beam_select(self.ctx, ld, vec(score, "score", rows, 0, dev), vec(done, "done", rows, 26, dev), n_beam, n_out, pad, vec(outs[0], "score_out", m, 0, dev),
+                                                  vec(outs[1], "parent", m, 26, dev), vec(outs[2], "token", m, 26, dev), self._stream()))
         return outs
 
     def paged_fork(self, k_cache, v_cache, table, n_kv, parent, fresh, table_out=None, n_kv_out=None):
         """cdna4_op_paged_fork: rows that go on from row parent[i] (full pages shared, a cut last page copied into page fresh[i]); returns (table int32 [n_out, W], n_kv int32 [n_out])."""
-        td = self._desc(table, "table"); n = table.shape[-2]; n_out = parent.numel() if self.torch.is_tensor(parent) else 0
+        d, vec, dev = self._desc, self._vec, self._dev
+        td = d(table, "table", dev); n = table.shape[-2]; n_out = parent.numel() if self.torch.is_tensor(parent) else 0
         if table_out is None:
-            table_out = table.new_empty((n_out, table.shape[-1]))
+            table_out = self._empty(table, 26, n_out, table.shape[-1])
         if n_kv_out is None:
-            n_kv_out = table.new_empty(n_out)
-        self._check(self.lib.cdna4_op_paged_fork(self.ctx, self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), td, self._vec(n_kv, "n_kv", n),
-                                                 self._vec(parent, "parent", n_out), self._vec(fresh, "fresh", n_out), self._desc(table_out, "table_out"),
-                                                 self._vec(n_kv_out, "n_kv_out", n_out), self._stream()))
+            n_kv_out = self._empty(table, 26, n_out)
+        self._check(self.lib.cdna4_op_paged_fork(self.ctx, d(k_cache, "k_cache", dev), d(v_cache, "v_cache", dev), td, vec(n_kv, "n_kv", n, 26, dev), vec(parent, "parent", n_out, 26, dev),
+                                                 vec(fresh, "fresh", n_out, 26, dev), d(table_out, "table_out", dev), vec(n_kv_out, "n_kv_out", n_out, 26, dev), self._stream()))
         return table_out, n_kv_out
 
     def paged_workspace(self, q, k_cache, v_cache, table, weight=None, out=None):
         """bytes of scratch that paged_attn takes for these tensors (reserve_workspace them before a capture)"""
-        return self._bytes(self.lib.cdna4_paged_attn_workspace(self._desc(q, "q"), self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), self._desc(table, "table"),
-                                                               None if weight is None else self._desc(weight, "weight"), self._desc(q if out is None else out, "out")))
+        d, dev = self._desc, self._dev
+        return self._bytes(self.lib.cdna4_paged_attn_workspace(d(q, "q", dev), d(k_cache, "k_cache", dev), d(v_cache, "v_cache", dev), d(table, "table", dev),
+                                                               None if weight is None else d(weight, "weight", dev), d(q if out is None else out, "out", dev)))
 
     def evict_workspace(self, k_cache, v_cache, table, weight, pos, budget, n_sink=0, n_recent=0):
         """bytes of scratch that paged_evict takes"""
-        w, p = self._desc(weight, "weight"), self._desc(pos, "pos")
-        return self._bytes(self.lib.cdna4_paged_evict_workspace(self._desc(k_cache, "k_cache"), self._desc(v_cache, "v_cache"), self._desc(table, "table"), w, p, budget, n_sink, n_recent, w, p))
+        d, dev = self._desc, self._dev
+        w, p = d(weight, "weight", dev), d(pos, "pos", dev)
+        return self._bytes(self.lib.cdna4_paged_evict_workspace(d(k_cache, "k_cache", dev), d(v_cache, "v_cache", dev), d(table, "table", dev), w, p, budget, n_sink, n_recent, w, p))
 
     def beam_workspace(self, logits, n_beam, n_out, pad=0):
         """bytes of scratch that beam_select takes"""
-        return self._bytes(self.lib.cdna4_beam_select_workspace(self._desc(logits, "logits"), n_beam, n_out, pad))
+        return self._bytes(self.lib.cdna4_beam_select_workspace(self._desc(logits, "logits", self._dev), n_beam, n_out, pad))
 
     def _bytes(self, n):
         if n < 0:

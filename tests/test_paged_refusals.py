@@ -31,7 +31,8 @@ def be():
     pkg = load_package()
     b = object.__new__(pkg.Cdna4Backend)
     b.torch, b.lib, b.ctx, b.comm, b.window, b.device = torch, pkg.load_library(), None, None, None, torch.device("cpu")
-    b._i32, b._i0 = torch.int32, torch.empty(0, dtype=torch.int32)
+    args = pkg.cdna4.load_args()
+    b._desc, b._vec, b._empty, b._dev = args.desc, args.vec, args.empty, -1
     b._stream = lambda: None
     return b
 
@@ -61,9 +62,30 @@ def test_the_binding_refuses_other_devices_types_and_shapes(be):
     k, table, q, n = cache(9, 2, 16, 64), torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, 8, 64), torch.zeros(3, dtype=torch.int32)
     elsewhere = torch.zeros(3, 8, 64, device="meta")
     for bad in (lambda: be.paged_attn(elsewhere, k, k, table, n), lambda: be.paged_attn(q, k, k, table, n.long()), lambda: be.paged_attn(q, k, k, table, n[:2]), lambda: be.paged_attn(q, k, k, table[0], n),
-                lambda: be.paged_attn(q.double(), k, k, table, n), lambda: be.paged_attn(None, k, k, table, n), lambda: be.paged_attn(q, k, k, table, torch.zeros(6, dtype=torch.int32)[::2]),
+                lambda: be.paged_attn(q.double(), k, k, table, n), lambda: be.paged_attn(None, k, k, table, n), lambda: be.paged_attn(q.to_sparse(), k, k, table, n), lambda: be.paged_attn(q, k, k, table[0, 0], n), lambda: be.paged_attn(q, k, k, table, torch.zeros(6, dtype=torch.int32)[::2]),
                 lambda: be.paged_store(q[:, :2], q[:, :2], k, k, table, n, start=n), lambda: be.paged_fork(k, k, table, n, n[:2], n), lambda: be.paged_fork(k, k, table, n, None, n),
                 lambda: be.beam_select(torch.zeros(6, 100), torch.zeros(5), 3, 2), lambda: be.beam_select(torch.zeros(6, 100), torch.zeros(6), 0, 2),
                 lambda: be.beam_select(torch.zeros(6, 100), torch.zeros(6), 3, -1), lambda: be.paged_evict(k, k, table, n, torch.zeros(3, 2, 64), torch.zeros(3, 2, 64), n, 8)):
         with pytest.raises(Error):
             bad()
+
+
+def test_descriptors_say_what_the_tensors_are(be):
+    import struct
+    for dtype, code, size in ((torch.float32, 0, 4), (torch.float16, 1, 2), (torch.bfloat16, 30, 2), (torch.int32, 26, 4)):
+        x = torch.zeros(7, 6, 5, 4, dtype=dtype)
+        for y in (x, x[2], x[2, 1], x.transpose(1, 2), x[:, ::2, 1:, :3], x[3:4, :1], x[:0], x.permute(3, 0, 2, 1)):
+            ptr, ty, *rest = struct.unpack("@Pi8q", be._desc(y, "x", -1))
+            ne, nb = list(y.shape)[::-1], [s * size for s in y.stride()][::-1]
+            assert (ptr, ty) == (y.data_ptr(), code) and rest[:4] == ne + [1] * (4 - len(ne)) and rest[4:] == nb + [0] * (4 - len(nb))
+    v = torch.arange(9, dtype=torch.int32)
+    assert be._vec(v[2:7], "v", 5, 26, -1) == v.data_ptr() + 8 and be._vec(None, "v", 5, 26, -1) is None
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        fake = torch.zeros(2, 3)
+    for bad in (lambda: be._desc(fake, "x", -1), lambda: be._desc(torch.zeros(2, 3, dtype=torch.float64), "x", -1), lambda: be._desc(torch.zeros(2, 3), "x", 0), lambda: be._desc("x", "x", -1),
+                lambda: be._vec(v[::2], "v", 5, 26, -1), lambda: be._vec(v, "v", 9, 0, -1), lambda: be._vec(v, "v", 9, 26, 0), lambda: be._desc(torch.zeros(1, 1, 1, 2, 3), "x", -1)):
+        with pytest.raises(load_package().Cdna4Error):
+            bad()
+    with pytest.raises(TypeError):
+        be._desc(v, "x")
