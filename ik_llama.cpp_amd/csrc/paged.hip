@@ -104,7 +104,7 @@ int cdna4_op_paged_store(cdna4_context *ctx, const cdna4_tensor *k, const cdna4_
 
 // ------------------------------------------------------------------------------------------------ fork
 struct ForkArgs { PagedCache c; const int *parent, *fresh; int *table_out, *n_kv_out; long out_row; };
-// grid (KV heads, rows): a workgroup copies the cut page's used slots of one head, K and V; the first head's workgroup also writes the row of the table.  Bound by memory: 256 rows with
+// grid (KV heads, rows): a workgroup copies one share in n_head_kv of the cut page's used slots, K and V; the first one also writes the row of the table.  Bound by memory: 256 rows with
 // tables of 8192 slots and on average half a page of 256 slots each (8 heads of 128): 278 MB in 54 us, 5.2 TB/s; 4 rows: 3 us, the chain parent -> length -> page -> copy.
 __global__ void __launch_bounds__(256) paged_fork_kernel(ForkArgs a) {
     const int h = blockIdx.x, i = blockIdx.y, p = a.parent[i];
@@ -120,15 +120,19 @@ __global__ void __launch_bounds__(256) paged_fork_kernel(ForkArgs a) {
     if (!used || to < 0) return;
     const int from = paged_page(a.c, p, full << a.c.page_shift);
     if (from < 0) return;
-    const int per_row = a.c.D / 8, units = used * per_row;
-    const char *ks = a.c.k + (long)from * a.c.k_page + (long)h * a.c.k_head, *vs = a.c.v + (long)from * a.c.v_page + (long)h * a.c.v_head;
-    char *kd = a.c.k + (long)to * a.c.k_page + (long)h * a.c.k_head, *vd = a.c.v + (long)to * a.c.v_page + (long)h * a.c.v_head;
+    // the workgroup's share of the page in the order of memory: K and V of a head's slots where those are neighbours, of a slot's heads where these are (token-major pages)
+    const unsigned per_row = a.c.D / 8, share = used * per_row, first = h * share, heads = a.c.n_head_kv;
+    const bool by_slot = a.c.k_head < a.c.k_row;
+    const char *ks = a.c.k + (long)from * a.c.k_page, *vs = a.c.v + (long)from * a.c.v_page;
+    char *kd = a.c.k + (long)to * a.c.k_page, *vd = a.c.v + (long)to * a.c.v_page;
     const int lg = a.c.D == 64 ? 3 : a.c.D == 128 ? 4 : 5;
 #pragma unroll 4
-    for (int u = threadIdx.x; u < units; u += 256) {
-        const int r = u >> lg, d = (u & (per_row - 1)) * 16;
-        const uint4 x = *reinterpret_cast<const uint4 *>(ks + r * a.c.k_row + d), y = *reinterpret_cast<const uint4 *>(vs + r * a.c.v_row + d);
-        *reinterpret_cast<uint4 *>(kd + r * a.c.k_row + d) = x; *reinterpret_cast<uint4 *>(vd + r * a.c.v_row + d) = y;
+    for (unsigned u = threadIdx.x; u < share; u += 256) {
+        const unsigned at = (by_slot ? first + u : u) >> lg, d = (u & (per_row - 1)) * 16;          // (share is whole rows)
+        const unsigned r = by_slot ? at / heads : at, hh = by_slot ? at - r * heads : (unsigned)h;
+        const long ko = (long)hh * a.c.k_head + (long)r * a.c.k_row + d, vo = (long)hh * a.c.v_head + (long)r * a.c.v_row + d;
+        const uint4 x = *reinterpret_cast<const uint4 *>(ks + ko), y = *reinterpret_cast<const uint4 *>(vs + vo);
+        *reinterpret_cast<uint4 *>(kd + ko) = x; *reinterpret_cast<uint4 *>(vd + vo) = y;
     }
 }
 int cdna4_op_paged_fork(cdna4_context *ctx, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const int32_t *n_kv, const int32_t *parent,
