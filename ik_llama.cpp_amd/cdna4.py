@@ -243,7 +243,14 @@ class Cdna4Backend:
             raise Cdna4Error(-3, self.lib.cdna4_last_error().decode())
         self.comm = None
         self.window = None
-        args = load_args(); self._desc, self._vec, self._empty, self._dev = args.desc, args.vec, args.empty, device
+        self._dev = device
+
+    def __getattr__(self, name):          # (asked for what is not there yet)
+        """The binding's C++ part is loaded by the first paged call: everything else runs without it."""
+        if name not in ("_desc", "_vec", "_empty"):
+            raise AttributeError("%s has no attribute %s" % (type(self).__name__, name))
+        args = load_args(); self._desc, self._vec, self._empty = args.desc, args.vec, args.empty
+        return getattr(args, name[1:])
 
     def close(self):
         self.window_free()

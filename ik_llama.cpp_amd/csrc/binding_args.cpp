@@ -40,7 +40,7 @@ PyObject *desc(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!THPVariable_Check(a[0])) return refuse(name, "a tensor");
     GUARDED(
     const at::Tensor &x = THPVariable_Unpack(a[0]);
-    if (x.layout() != at::kStrided || !is_on(x, index)) return refuse(name, "a strided tensor on the backend's device");
+    if (x.layout() != at::kStrided || x.is_neg() || !is_on(x, index)) return refuse(name, "a strided tensor on the backend's device");          // (is_neg: memory holds the negated values)
     const int type = type_of(x.scalar_type()); const int64_t dims = x.dim(), es = type == 0 || type == 26 ? 4 : 2;
     if (type < 0) return refuse(name, "float32, float16, bfloat16 or int32");
     if (dims < 2 || dims > 4) return refuse(name, "2 to 4 dimensions");
@@ -62,7 +62,7 @@ PyObject *vec(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!THPVariable_Check(a[0])) return refuse(name, what);
     GUARDED(
     const at::Tensor &x = THPVariable_Unpack(a[0]);
-    if (x.layout() != at::kStrided || !is_on(x, index) || type_of(x.scalar_type()) != type || x.numel() != count || !x.is_contiguous()) return refuse(name, what);
+    if (x.layout() != at::kStrided || x.is_neg() || !is_on(x, index) || type_of(x.scalar_type()) != type || x.numel() != count || !x.is_contiguous()) return refuse(name, what);
     return PyLong_FromVoidPtr(x.data_ptr());
     )
 }

@@ -89,3 +89,22 @@ def test_descriptors_say_what_the_tensors_are(be):
             bad()
     with pytest.raises(TypeError):
         be._desc(v, "x")
+
+
+def test_a_negated_view_is_refused(be):
+    z = torch.zeros(3, 4, dtype=torch.complex64).conj().imag          # float32 values whose memory holds their negatives
+    assert z.is_neg()
+    for bad in (lambda: be._desc(z, "x", -1), lambda: be._vec(z[0], "v", 4, 0, -1)):
+        with pytest.raises(load_package().Cdna4Error):
+            bad()
+    be._desc(z.resolve_neg(), "x", -1)
+
+
+def test_the_binding_part_is_loaded_by_the_first_paged_call():
+    pkg = load_package()
+    b = object.__new__(pkg.Cdna4Backend)
+    b.torch, b.lib, b.ctx, b.comm, b.window, b._dev = torch, pkg.load_library(), None, None, None, -1
+    assert "_desc" not in b.__dict__
+    with pytest.raises(AttributeError):
+        b.no_such_method
+    assert b.beam_workspace(torch.zeros(6, 100), 3, 5) > 0 and "_desc" in b.__dict__
