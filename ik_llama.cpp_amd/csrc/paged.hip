@@ -105,7 +105,7 @@ int cdna4_op_paged_store(cdna4_context *ctx, const cdna4_tensor *k, const cdna4_
 // ------------------------------------------------------------------------------------------------ fork
 struct ForkArgs { PagedCache c; const int *parent, *fresh; int *table_out, *n_kv_out; long out_row; };
 // grid (KV heads, rows): a workgroup copies one share in n_head_kv of the cut page's used slots, K and V; the first one also writes the row of the table.  Bound by memory: 256 rows with
-// tables of 8192 slots and on average half a page of 256 slots each (8 heads of 128): 278 MB in 54 us, 5.2 TB/s; 4 rows: 3 us, the chain parent -> length -> page -> copy.
+// tables of 8192 slots and on average half a page of 256 slots each (8 heads of 128): 278 MB in 53 us, 5.2 TB/s; 4 rows: 3 us, the chain parent -> length -> page -> copy.
 __global__ void __launch_bounds__(256) paged_fork_kernel(ForkArgs a) {
     const int h = blockIdx.x, i = blockIdx.y, p = a.parent[i];
     const bool live = (unsigned)p < (unsigned)a.c.n_seq && a.c.n_kv[(unsigned)p < (unsigned)a.c.n_seq ? p : 0] >= 0;
