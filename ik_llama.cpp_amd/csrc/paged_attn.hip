@@ -8,8 +8,8 @@
 //   (16 bytes a lane, a row per 16 lanes) and becomes the other operand by v_perm, so the loop touches no LDS at all.
 // * f32 results from 16-bit operands: q and p are split into two f16 (2^-22; q scaled by a power of two, p by 2^8) or three bf16 (exactly 24 bits) terms, K and V are what the cache
 //   holds; products and sums are f32.  The extra matrix instructions stay far below the load time (32 or 48 of 16 clk per 16 KB and SIMD).
-// * Equal shares: all tiles of 128 slots of all (sequence, KV head, 16 query heads) units are numbered through, and every workgroup takes an equal contiguous range of the numbers, from
-//   the lengths as they are on the device.  A long sequence in a batch of short ones spreads over the chip by itself; a workgroup that covers a unit alone writes its result, the others
+// * Equal shares: all tiles of 128 slots of all (sequence, KV head) pairs are numbered through, and every workgroup takes an equal contiguous range of the numbers, from the lengths as
+//   they are on the device.  Groups of more than 16 query heads: the blocks of 16 have workgroups of their own, with the same ranges.  A long sequence in a batch of short ones spreads over the chip by itself; a workgroup that covers a unit alone writes its result, the others
 //   leave (max, sum, accumulator) for the join.
 //
 // Measured (8 KV heads of 128): 64 sequences of up to 8192 slots, f16, 32 query heads: 1.12 GB in 197 us + 6 us for the join, 5.5 TB/s; one of 131071, bf16, 64 query heads: 537 MB in 92 -
@@ -31,9 +31,9 @@ constexpr int ATTN_MAX_WG = 1024;                     // most workgroups of a la
 
 struct AttnArgs {
     PagedCache c; const char *q; long q_head, q_seq; char *dst; long d_head, d_seq; char *weight; long w_head, w_seq;
-    int group, n_head, n_unit, n_wg; float scale, softcap, inv_softcap;          // n_unit: (KV head, 16 query heads) pairs of a sequence; n_wg: workgroups that share the tiles
+    int group, n_head, blocks, n_wg; float scale, softcap, inv_softcap;          // blocks: of 16 query heads in a group; n_wg: workgroups that share the tiles of one block of every group
     int *prefix;                // [n_seq + 1] tiles of a unit before sequence s
-    float *part;                // [n_wg][2][QH][D + 2]: what a workgroup leaves of its first / last unit (max, sum, accumulator of every head)
+    float *part;                // [blocks][n_wg][2][QH][D + 2]: what a workgroup leaves of its first / last unit (max, sum, accumulator of every head)
     float2 *stat;               // [n_seq][n_head] max and sum of a row (weight only)
     float *score; long score_row;   // [n_seq][n_head][score_row] scores in units of log 2 (weight only)
 };
@@ -115,28 +115,29 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     int *pre = s_mem;                                                              // prefix sums (not ONE)
     float *s_o = reinterpret_cast<float *>(s_mem + (ONE ? 0 : (a.c.n_seq + 4) & ~3));       // [WAVES][heads][D + 4]
-    int x = 0, x_end = 1, s = 0;
+    int x = 0, x_end = 1, s = 0, blk = 0;
     if constexpr (!ONE) {
         scan_tiles(a, pre, s_tot);
-        const Shares shares(pre[a.c.n_seq] * a.n_unit, a.n_wg);              // (the host has checked that tiles * units < 2^31)
+        blk = blockIdx.x / a.n_wg;
+        const Shares shares(pre[a.c.n_seq] * a.c.n_head_kv, a.n_wg);         // (the host has checked that tiles * KV heads < 2^31)
         if (blockIdx.x == 0) for (int i = threadIdx.x; i <= a.c.n_seq; i += 256) a.prefix[i] = pre[i];
-        x = __builtin_amdgcn_readfirstlane(shares.first(blockIdx.x)); x_end = __builtin_amdgcn_readfirstlane(shares.first(blockIdx.x + 1));
+        const int wg = blockIdx.x - blk * a.n_wg; x = __builtin_amdgcn_readfirstlane(shares.first(wg)); x_end = __builtin_amdgcn_readfirstlane(shares.first(wg + 1));
         if (x >= x_end) return;
-        for (int b = 0; b < a.c.n_seq; b += 64) { const int i = b + lane; s += __popcll(__ballot(i < a.c.n_seq && pre[min(i, a.c.n_seq - 1) + 1] * a.n_unit <= x)); }
+        for (int b = 0; b < a.c.n_seq; b += 64) { const int i = b + lane; s += __popcll(__ballot(i < a.c.n_seq && pre[min(i, a.c.n_seq - 1) + 1] * a.c.n_head_kv <= x)); }
     }
     for (bool first = true; x < x_end; first = false) {
-        int n, tiles, unit, tile0 = 0, ntile;
+        int n, tiles, hk, tile0 = 0, ntile;
         if constexpr (ONE) {
-            s = blockIdx.y; unit = blockIdx.x; n = paged_len(a.c, s); tiles = ntile = (n + TILE - 1) / TILE; x = x_end;
+            s = blockIdx.y; hk = blockIdx.x / a.blocks; blk = blockIdx.x - hk * a.blocks; n = paged_len(a.c, s); tiles = ntile = (n + TILE - 1) / TILE; x = x_end;
         } else {
-            while (pre[s + 1] * a.n_unit <= x) ++s;
+            while (pre[s + 1] * a.c.n_head_kv <= x) ++s;
             s = __builtin_amdgcn_readfirstlane(s);
             tiles = __builtin_amdgcn_readfirstlane(pre[s + 1] - pre[s]); n = __builtin_amdgcn_readfirstlane(paged_len(a.c, s));
-            const int rem = __builtin_amdgcn_readfirstlane(x - pre[s] * a.n_unit); unit = rem / tiles; tile0 = rem - unit * tiles;
+            const int rem = __builtin_amdgcn_readfirstlane(x - pre[s] * a.c.n_head_kv); hk = rem / tiles; tile0 = rem - hk * tiles;
             ntile = min(tiles - tile0, x_end - x);
             x += ntile;
         }
-        const int blocks = (a.group + QH - 1) / QH, hk = unit / blocks, h0 = hk * a.group + (unit - hk * blocks) * QH, heads = min(QH, (hk + 1) * a.group - h0);
+        const int h0 = hk * a.group + blk * QH, heads = min(QH, (hk + 1) * a.group - h0);
         // the queries: chunk c holds elements 32 c + 8 g ... + 7 of head `col`; requested before the cache rows, split under their way
         const float *qr = reinterpret_cast<const float *>(a.q + (long)s * a.q_seq + (long)(h0 + min(col, heads - 1)) * a.q_head) + 8 * g;
         float4 x0[KC], x1[KC];
@@ -353,11 +354,10 @@ template <int D> struct RowParts {
     __device__ RowParts(const AttnArgs &a, int h, int s) {
         const int p0 = a.prefix[s]; tiles = a.prefix[s + 1] - p0; count = 0; base = nullptr; other = 0;
         if (!tiles) return;
-        const Shares shares(a.prefix[a.c.n_seq] * a.n_unit, a.n_wg);
-        const int blocks = (a.group + QH - 1) / QH, hk = h / a.group, in = h - hk * a.group, unit = hk * blocks + in / QH;
-        const int x0 = p0 * a.n_unit + unit * tiles, w0 = shares.owner(x0);
+        const Shares shares(a.prefix[a.c.n_seq] * a.c.n_head_kv, a.n_wg);
+        const int hk = h / a.group, in = h - hk * a.group, x0 = p0 * a.c.n_head_kv + hk * tiles, w0 = shares.owner(x0);
         count = shares.owner(x0 + tiles - 1) - w0 + 1;
-        base = a.part + ((long)w0 * 2 * QH + in % QH) * (D + 2);
+        base = a.part + (((long)(in / QH) * a.n_wg + w0) * 2 * QH + in % QH) * (D + 2);
         other = shares.first(w0) < x0 ? (long)QH * (D + 2) : 0;
     }
     __device__ const float *at(int i) const { return base + i * STEP + (i ? 0 : other); }
@@ -452,9 +452,9 @@ static int attn_check(const cdna4_tensor *q, const cdna4_tensor *k_cache, const 
     ARG_CHECK(q->ne[1] % a->c.n_head_kv == 0, "paged_attn: n_head a multiple of n_head_kv");
     OP_CHECK(q->ne[1] <= 16384, "paged_attn: at most 16384 query heads");
     if (weight && (rc = pg_slots_check("paged_attn", "weight", weight, CDNA4_TYPE_F32, a->c, true))) return rc;
-    a->n_head = (int)q->ne[1]; a->group = a->n_head / a->c.n_head_kv; a->n_unit = a->c.n_head_kv * ((a->group + QH - 1) / QH);
+    a->n_head = (int)q->ne[1]; a->group = a->n_head / a->c.n_head_kv; a->blocks = (a->group + QH - 1) / QH;
     const long slots = (long)a->c.W << a->c.page_shift, tiles = (slots + TILE - 1) / TILE;
-    OP_CHECK(tiles * a->c.n_seq < (1l << 31) / std::max(a->n_unit, 1) && tiles * a->c.n_head_kv < (1l << 26), "paged_attn: too many slots in all");
+    OP_CHECK(tiles * a->c.n_seq < (1l << 31) / std::max(a->c.n_head_kv * a->blocks, 1) && tiles * a->c.n_head_kv < (1l << 26), "paged_attn: too many slots in all");
     a->score_row = tiles * TILE;
     return CDNA4_OK;
 }
@@ -485,7 +485,7 @@ int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_t
     a.q = (const char *)q->data; a.q_head = q->nb[1]; a.q_seq = q->nb[2]; a.dst = (char *)dst->data; a.d_head = dst->nb[1]; a.d_seq = dst->nb[2];
     a.weight = weight ? (char *)weight->data : nullptr; a.w_head = weight ? weight->nb[1] : 0; a.w_seq = weight ? weight->nb[2] : 0;
     DEVICE_SCOPE(ctx);
-    const long row_tiles = a.score_row / TILE, tiles = row_tiles * a.c.n_seq * a.n_unit;
+    const long row_tiles = a.score_row / TILE, tiles = row_tiles * a.c.n_seq * a.c.n_head_kv; const int n_unit = a.c.n_head_kv * a.blocks;
     const bool bf = k_cache->type == CDNA4_TYPE_BF16, cap = softcap != 0.0f;
     hipStream_t st = (hipStream_t)stream;
     const size_t merge = (size_t)WAVES * std::min(QH, a.group) * (a.c.D + 4) * 4;
@@ -494,7 +494,7 @@ int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_t
     // 24.4, 64 x 2048: 56 / 62, 256 x 2048: 204 / 223; bf16, 4 heads of 64, 1 x 768: 7.8 / 9.6; of 256, 1 x 512: 14.3 / 13.0, 128 x 2048: 111 / 110.
     // With weights: if a KV head is one unit and its scores fit LDS.
     const size_t one_lds = merge + (weight ? (size_t)a.group * a.score_row * 4 : 0);
-    const bool one = (row_tiles * a.c.D <= 640 || (row_tiles <= 16 && (long)a.c.n_seq * a.n_unit >= ctx->num_cu)) && (!weight || a.group <= QH) && one_lds <= ONE_LDS;
+    const bool one = (row_tiles * a.c.D <= 640 || (row_tiles <= 16 && (long)a.c.n_seq * n_unit >= ctx->num_cu)) && (!weight || a.group <= QH) && one_lds <= ONE_LDS;
 #define ATTN(D_, B_, C_, O_, grid, lds) do { if ((lds) > 60 * 1024) HIP_TRY((pg_opt_in_lds<paged_attn_kernel<D_, B_, C_, O_>>(ctx->device, ONE_LDS))); \
                                              hipLaunchKernelGGL((paged_attn_kernel<D_, B_, C_, O_>), grid, dim3(256), lds, st, a); } while (0)
 #define ATTN_D(D_, O_, grid, lds) do { if (bf) { if (cap) ATTN(D_, true, true, O_, grid, lds); else ATTN(D_, true, false, O_, grid, lds); } \
@@ -502,16 +502,22 @@ int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_t
 #define ATTN_ALL(O_, grid, lds) do { if (a.c.D == 64) ATTN_D(64, O_, grid, lds); else if (a.c.D == 128) ATTN_D(128, O_, grid, lds); else ATTN_D(256, O_, grid, lds); } while (0)
     if (one) {
         a.n_wg = 0; a.prefix = nullptr; a.part = nullptr; a.stat = nullptr; a.score = nullptr;
-        ATTN_ALL(true, dim3((unsigned)a.n_unit, (unsigned)a.c.n_seq), one_lds);
+        ATTN_ALL(true, dim3((unsigned)n_unit, (unsigned)a.c.n_seq), one_lds);
         return CDNA4_OK;
     }
-    a.n_wg = (int)std::max<long>(1, std::min<long>({tiles, (long)ctx->num_cu * (a.c.D == 256 ? 1 : 2), (long)ATTN_MAX_WG}));
-    const AttnScratch sc = attn_scratch(a, weight != nullptr, a.n_wg);
+    // Blocks of 16 heads that share a KV head read the same tiles at the same time: workgroups that are a multiple of 8 apart share an XCD and its L2, so much of the cache comes from memory
+    // once.  us with a numbering of all blocks one after the other / with this one (f16; sequences x slots, heads on KV heads): 64 x 8192, 32 on 1 of 128: 54.5 / 51.4, 160 on 8: 382 / 374;
+    // 1 x 130000, 20 on 1 of 256: 50.4 / 43.5, 80 on 4 of 64: 46.6 / 37.8; bf16, 128 on 1 of 128: 80.8 / 51.8.  (Registers leave two waves to a SIMD, so with every block the loads under way
+    // are of fewer different rows: 3 TB/s of them.)
+    long most_wg = std::min<long>((long)ctx->num_cu * (a.c.D == 256 ? 1 : 2), ATTN_MAX_WG) / a.blocks;          // (blocks: at most 1024, so blocks * n_wg is at most ATTN_MAX_WG)
+    if (a.blocks > 1 && most_wg > 8) most_wg &= ~7l;
+    a.n_wg = (int)std::max<long>(1, std::min(tiles, most_wg));
+    const AttnScratch sc = attn_scratch(a, weight != nullptr, a.n_wg * a.blocks);
     if ((rc = cdna4_ensure_ws(ctx, sc.total, st))) return rc;
     char *ws = (char *)ctx->ws;
     a.prefix = (int *)ws; a.part = (float *)(ws + sc.part); a.stat = weight ? (float2 *)(ws + sc.stat) : nullptr; a.score = weight ? (float *)(ws + sc.score) : nullptr;
     const size_t lds = (size_t)((a.c.n_seq + 4) & ~3) * 4 + merge;          // (at most (8192 + 4) * 4 + 4 * 16 * 260 * 4 bytes)
-    ATTN_ALL(false, dim3((unsigned)a.n_wg), lds);
+    ATTN_ALL(false, dim3((unsigned)(a.n_wg * a.blocks)), lds);
     const dim3 join((unsigned)(a.n_head + (weight ? a.c.n_head_kv * ((a.score_row + 1023) / 1024) : 0)), (unsigned)a.c.n_seq);
     if (a.c.D == 64) hipLaunchKernelGGL(paged_attn_join_kernel<64>, join, dim3(256), 0, st, a);
     else if (a.c.D == 128) hipLaunchKernelGGL(paged_attn_join_kernel<128>, join, dim3(256), 0, st, a);

@@ -91,6 +91,14 @@ def test_attn_lengths(D, page, dtype, backend):
     check_attn(backend, Case(LENS, D=D, page=page, dtype=dtype, seed=D + page), heads=8, weight=None)
 
 
+@pytest.mark.parametrize("D,heads_kv,heads,dtype", [(64, 1, 17, torch.float16), (128, 2, 40, torch.bfloat16), (256, 1, 33, torch.float16), (64, 1, 300, torch.bfloat16), (128, 3, 60, torch.float16)])
+@pytest.mark.parametrize("weights", [False, True])
+def test_attn_large_groups_over_long_tables(D, heads_kv, heads, dtype, weights, backend):
+    """the blocks of 16 heads of a group have workgroups of their own: rows of many and of no tiles, more blocks than workgroups to a block"""
+    c = Case([2700, 0, 129, 1], D=D, heads_kv=heads_kv, page=64, dtype=dtype, seed=heads)
+    check_attn(backend, c, heads, weight=c.slots() if weights else None, softcap=20.0 if D == 256 else 0.0)
+
+
 @pytest.mark.parametrize("heads_kv,heads", [(1, 1), (2, 2), (8, 8), (2, 6), (1, 8), (2, 14), (1, 16), (1, 17), (2, 40), (1, 71), (3, 12)])
 @pytest.mark.parametrize("weights", [False, True])
 def test_attn_groups(heads_kv, heads, weights, backend):
