@@ -10,30 +10,31 @@ template <typename X> static __device__ __forceinline__ X *slot_row(const SlotVi
 // ------------------------------------------------------------------------------------------------ store
 struct StoreArgs {
     PagedCache c; const char *k, *v; long k_head, v_head, k_tok, v_tok;
-    const int *start, *n_past; SlotView weight, pos; int *n_kv_out; int n_tok; int bf16;
+    const int *start, *n_past; SlotView weight, pos; int *n_kv_out; int n_tok, pack, blocks;          // pack: tokens of a workgroup; blocks: workgroups of tokens
 };
 // two f32 -> two 16-bit values of the cache type, rounded to nearest even (the one rounding of K and V)
 template <bool BF16> static __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if constexpr (BF16) return float_to_bf16_bits(a) | (float_to_bf16_bits(b) << 16);
     else { typedef _Float16 h2 __attribute__((ext_vector_type(2))); const h2 h = {(_Float16)a, (_Float16)b}; return __builtin_bit_cast(uint32_t, h); }
 }
-// the sequence of token i: the last s with start[s] <= i (a wave reads the whole vector at once: one memory latency instead of a binary search's chain of them)
+// the sequence of token i (the same for all lanes): the last s with start[s] <= i, -1 if there is none (a wave reads the whole vector at once: one memory latency instead of a binary
+// search's chain of them)
 static __device__ __forceinline__ int token_seq(const int *start, int n_seq, int i) {
-    if (!start) return i;
     int n = 0;
     for (int b = 0; b < n_seq; b += 64) {
         const int s = b + (int)(threadIdx.x & 63);
         n += __popcll(__ballot(s < n_seq && start[min(s, n_seq - 1)] <= i));
     }
-    return i < start[n_seq] ? n - 1 : -1;
+    return n - 1;
 }
-// One workgroup per token; a thread moves 8 values of K or V at a time (32 bytes in, 16 out).  Bound by memory for prompts (16866 tokens of 8 x 128 in six ragged sequences, bf16: 208 MB in
-// 42 us, 5.0 TB/s, what a large copy reaches), by the chain of lookups for single tokens (64 sequences: 3 us).  The f32 rows do not depend on where they go: the first load of every thread runs under the lookups of sequence,
-// length and page (unconditional, on a clamped unit: loaded under a branch and carried into the loop, this compiler reuses three of the four registers before they are read).
+// One workgroup per token, or per 256 / units tokens where a token's rows are half a workgroup's or less (one to a workgroup / packed: 16000 tokens of one head of 64: 18.5 / 5.5 us, of four:
+// 13.4 / 8.5).  A thread moves 8 values of K or V at a time (32 bytes in, 16 out).  Bound by memory for prompts (16866 tokens of 8 x 128 in six ragged sequences, bf16: 208 MB in 42 us,
+// 5.0 TB/s, what a large copy reaches), by the chain of lookups for single tokens (64 sequences: 3 us).  The f32 rows do not depend on where they go: the first load of every thread runs
+// under the lookups of sequence, length and page (unconditional, on a clamped unit: loaded under a branch and carried into the loop, this compiler reuses three of the four registers before
+// they are read).
 template <bool BF16> __global__ void __launch_bounds__(256) paged_store_kernel(StoreArgs a) {
-    const int tok = blockIdx.x;
-    if (tok >= a.n_tok) {          // the workgroups behind the tokens: the new lengths
-        const int s = (tok - a.n_tok) * 256 + (int)threadIdx.x;
+    if ((int)blockIdx.x >= a.blocks) {          // the workgroups behind the tokens: the new lengths
+        const int s = ((int)blockIdx.x - a.blocks) * 256 + (int)threadIdx.x;
         if (s < a.c.n_seq) {
             const int n = a.c.n_kv[s], add = a.start ? max(a.start[s + 1] - a.start[s], 0) : 1;
             a.n_kv_out[s] = n < 0 ? n : (int)min((long)n + add, (long)a.c.W << a.c.page_shift);
@@ -41,15 +42,21 @@ template <bool BF16> __global__ void __launch_bounds__(256) paged_store_kernel(S
         return;
     }
     const int lg = a.c.D == 64 ? 3 : a.c.D == 128 ? 4 : 5, half = a.c.n_head_kv << lg, units = 2 * half;        // units of 8 values: all of K, then all of V
+    int tok = blockIdx.x, u = threadIdx.x, step = 256;
+    if (a.pack > 1) { const int nth = (int)threadIdx.x / units; tok = tok * a.pack + nth; u -= nth * units; step = units; if (nth >= a.pack) tok = a.n_tok; }
+    const int row = min(tok, a.n_tok - 1);
     auto source = [&](int u) {
         const int w = u >= half ? u - half : u, h = w >> lg, d = (w - (h << lg)) * 8;
-        return reinterpret_cast<const float4 *>((u >= half ? a.v + (long)tok * a.v_tok + (long)h * a.v_head : a.k + (long)tok * a.k_tok + (long)h * a.k_head) + d * 4);
+        return reinterpret_cast<const float4 *>((u >= half ? a.v + (long)row * a.v_tok + (long)h * a.v_head : a.k + (long)row * a.k_tok + (long)h * a.k_head) + d * 4);
     };
-    int u = threadIdx.x;
     const float4 *src = source(min(u, units - 1));
     const float4 f0 = src[0], f1 = src[1];
-    const int s = token_seq(a.start, a.c.n_seq, tok);
-    if (s < 0 || s >= a.c.n_seq) return;
+    int s = tok;
+    if (a.start) {
+        s = token_seq(a.start, a.c.n_seq, __builtin_amdgcn_readfirstlane(tok));                                     // of the wave's first token;
+        if (a.pack > 1) while (s + 1 < a.c.n_seq && a.start[s + 1] <= tok) ++s;                                     // its others lie in the same or a later one
+    }
+    if (tok >= a.n_tok || s < 0 || s >= a.c.n_seq || (a.start && tok >= a.start[a.c.n_seq])) return;
     const int n = a.c.n_kv[s], nth = a.start ? tok - a.start[s] : 0;
     const long slot = (long)n + nth;
     if (n < 0 || nth < 0 || slot >= ((long)a.c.W << a.c.page_shift)) return;
@@ -62,9 +69,10 @@ template <bool BF16> __global__ void __launch_bounds__(256) paged_store_kernel(S
         char *p = unit >= half ? vp + (long)h * a.c.v_head : kp + (long)h * a.c.k_head;
         *reinterpret_cast<uint4 *>(p + d * 2) = make_uint4(pack2<BF16>(x.x, x.y), pack2<BF16>(x.z, x.w), pack2<BF16>(y.x, y.y), pack2<BF16>(y.z, y.w));
     };
+    const int first = u;
     if (u < units) store(u, f0, f1);
-    for (u += 256; u < units; u += 256) { const float4 *p = source(u); const float4 x = p[0], y = p[1]; store(u, x, y); }
-    for (int h = threadIdx.x; h < a.c.n_head_kv; h += 256) {
+    for (u += step; u < units; u += step) { const float4 *p = source(u); const float4 x = p[0], y = p[1]; store(u, x, y); }
+    for (int h = first; h < a.c.n_head_kv; h += step) {
         if (a.weight.p) slot_row<float>(a.weight, s, h)[slot] = 0.0f;
         if (a.pos.p) slot_row<int>(a.pos, s, h)[slot] = a.n_past[s] + nth;
     }
@@ -94,7 +102,9 @@ int cdna4_op_paged_store(cdna4_context *ctx, const cdna4_tensor *k, const cdna4_
     ARG_CHECK(!weight || !pos || a.c.W == 0 || !pg_overlap(weight, 4, pos, 4), "paged_store: weight overlaps pos");
     a.k = (const char *)k->data; a.v = (const char *)v->data; a.k_head = k->nb[1]; a.v_head = v->nb[1]; a.k_tok = k->nb[2]; a.v_tok = v->nb[2];
     a.c.n_kv = n_kv; a.start = start; a.n_past = n_past; a.weight = slot_view(weight); a.pos = slot_view(pos); a.n_kv_out = n_kv_out; a.n_tok = (int)n_tok;
-    const long blocks = n_tok + (n_kv_out ? (n_seq + 255) / 256 : 0);
+    const int units = 2 * a.c.n_head_kv * (a.c.D / 8);
+    a.pack = std::max(1, 256 / units); a.blocks = (int)((n_tok + a.pack - 1) / a.pack);
+    const long blocks = a.blocks + (n_kv_out ? (n_seq + 255) / 256 : 0);
     if (blocks == 0) return CDNA4_OK;
     DEVICE_SCOPE(ctx);
     if (k_cache->type == CDNA4_TYPE_BF16) hipLaunchKernelGGL(paged_store_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);

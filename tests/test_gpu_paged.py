@@ -282,6 +282,31 @@ def test_store(D, heads_kv, token_major, dtype, backend):
         np.testing.assert_array_equal(host(a), b)
 
 
+@pytest.mark.parametrize("D,heads_kv", [(64, 1), (64, 2), (64, 3), (128, 1), (128, 3), (64, 5), (256, 1), (256, 2), (64, 8), (128, 5)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_store_of_few_heads(D, heads_kv, dtype, backend):
+    """several tokens to a workgroup: sequences of none, one and many of them, tokens before the first and behind the last sequence, one token each"""
+    counts = [0, 0, 1, 70, 0, 3, 1, 1, 0, 17, 129, 0]
+    c = Case([5, 0, 16, 30, 1, -1, 15, 0, 7, 31, 3, 2], D=D, heads_kv=heads_kv, page=16, dtype=dtype, seed=D + heads_kv, junk=1.0, W=9)
+    for lead in (0, 3):
+        start = (np.concatenate([[0], np.cumsum(counts)]) + lead).astype(np.int32)
+        k, v = (c.rng.standard_normal((start[-1] + 5, heads_kv, D)).astype(np.float32) for _ in "kv")
+        n_past = np.arange(12, dtype=np.int32) * 11
+        weight, pos = c.slots(), c.slots(pos=True)
+        kh, vh, _, _ = c.host(); wh, ph = host(weight), host(pos)
+        want = ref.store(torch.from_numpy(k).to(dtype).double().numpy(), torch.from_numpy(v).to(dtype).double().numpy(), kh, vh, c.table, c.n_kv, start, n_past, wh, ph)
+        kc, vc, table, n_kv = c.dev()
+        got = backend.paged_store(g(k), g(v), kc, vc, table, n_kv, start=g(start), n_past=g(n_past), weight=weight, pos=pos)
+        np.testing.assert_array_equal(host(got), want)
+        for a, b in ((kc, kh), (vc, vh), (weight, wh), (pos, ph)):
+            np.testing.assert_array_equal(host(a), b)
+    k, v = (c.rng.standard_normal((12, heads_kv, D)).astype(np.float32) for _ in "kv")
+    kh, vh, _, _ = c.host()
+    want = ref.store(torch.from_numpy(k).to(dtype).double().numpy(), torch.from_numpy(v).to(dtype).double().numpy(), kh, vh, c.table, c.n_kv)
+    np.testing.assert_array_equal(host(backend.paged_store(g(k), g(v), kc, vc, table, n_kv)), want)
+    np.testing.assert_array_equal(host(kc), kh); np.testing.assert_array_equal(host(vc), vh)
+
+
 def test_store_one_token_each_with_inactive_rows_and_missing_pages(backend):
     c = Case([0, 15, 16, 40, 20, 47], junk=0.5, seed=3, W=3)
     c.n_kv[1] = -1; c.n_kv[5] = 48                                       # inactive; full
