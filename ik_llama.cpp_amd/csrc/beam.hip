@@ -2,7 +2,7 @@
 //
 // The logits are read once (4 bytes a candidate against a handful of operations: bound by that read).  A workgroup takes 8192 (2048) neighbouring logits of a row into registers and leaves
 // their maximum, the sum of their exponentials and their n_out best, sorted; a second launch joins a group's chunks: log sum exp of every beam, then the best of the sorted lists.
-// Measured: 256 rows of 128256 (131 MB), 32 groups of 8, 16 results: 29 us for the chunks (4.5 TB/s) and 9 us for the join; 4 rows of 32000: 4.1 and 4.9 us.
+// Measured: 256 rows of 128256 (131 MB), 32 groups of 8, 16 results: 24 us for the chunks (5.5 TB/s) and 9 us for the join; 4 rows of 32000: 4.1 and 4.9 us.
 //
 // Choosing the k best of many without sorting them: in a total order without ties, the k-th best of the threads' (or lanes' quads') own best elements is a bound that at least k elements
 // reach, and every element that reaches it belongs to one of the k owners whose best does -- so the collected list is never longer than k shares, whatever the values, and in random order
@@ -36,16 +36,19 @@ struct __attribute__((packed, aligned(4))) F4a4 { float x, y, z, w; };          
 
 // EPT logits a thread.  Owners of the bound: quads of lanes (64) for n_out <= 16, single threads above; the list holds n_out shares of either.
 // The bound is first taken on values alone, which costs a maximum and a comparison per logit (with keys of value and index all through, the launch was bound by its vector instructions:
-// 45 us for 256 rows of 128256, 131 MB).  Ties at the bound can make that list too long, and a bound of -inf says nothing: then the keys decide.
+// 45 us for 256 rows of 128256, 131 MB), and from every wave a quarter of n_out (one bound of the workgroup for 64 results took as long as the rest: 480 rows of 70000: 48 us, so 38).  Ties at
+// the bound can make that list too long, and a bound of -inf says nothing: then the keys decide.  A row's last chunk takes its logits one at a time, coalesced (as quads of which the last were
+// cut lane by lane, those chunks ended last: 29 us in all for the 131 MB, so 24).
 template <int EPT> __global__ void __launch_bounds__(256) beam_scan_kernel(BeamArgs a) {
     constexpr int CAP = BEAM_MAX_OUT * EPT;
-    __shared__ u64 s_own[256], s_list[CAP]; __shared__ float s_red[8]; __shared__ u64 s_bound; __shared__ int s_n;
+    __shared__ u64 s_own[256], s_list[CAP]; __shared__ float s_red[12]; __shared__ u64 s_bound; __shared__ int s_n;
     const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, base = blockIdx.x * 256 * EPT;
     const float *x = reinterpret_cast<const float *>(a.logits + (long)r * a.row) + base;
     const int n = min(256 * EPT, a.n_vocab - base);
-    auto index = [&](int e) { return (e / 4 * 256 + tid) * 4 + e % 4; };
+    const bool whole = n == 256 * EPT;          // (a cut chunk goes to the lanes one logit at a time, so that every wave has some)
+    auto index = [&](int e) { return whole ? (e / 4 * 256 + tid) * 4 + e % 4 : e * 256 + tid; };
     float v[EPT];
-    if (n == 256 * EPT) {
+    if (whole) {
 #pragma unroll
         for (int e = 0; e < EPT / 4; ++e) { const F4a4 f = reinterpret_cast<const F4a4 *>(x)[e * 256 + tid]; v[4 * e] = f.x; v[4 * e + 1] = f.y; v[4 * e + 2] = f.z; v[4 * e + 3] = f.w; }
     } else {
@@ -56,19 +59,25 @@ template <int EPT> __global__ void __launch_bounds__(256) beam_scan_kernel(BeamA
 #pragma unroll
     for (int e = 1; e < EPT; ++e) top = fmaxf(top, v[e]);
     const bool quads = a.n_out <= 16; const int owners = quads ? 64 : 256;
-    float ot = top;
-    if (quads) { ot = fmaxf(ot, fa_dpp<0xb1>(ot)); ot = fmaxf(ot, fa_dpp<0x4e>(ot)); }
-    if (!quads || (lane & 3) == 0) s_own[quads ? tid >> 2 : tid] = logit_key(ot, quads ? tid >> 2 : tid);
-    const float wm = wave_max(top);
-    if (lane == 0) s_red[wave] = wm;
+    // a quarter of n_out from every wave: the smallest of the waves' bounds is one that n_out elements reach (no barrier and a fourth of the comparisons of a bound over the workgroup)
+    float ot = top == top ? top : -INFINITY; int above = 0;
+    if (quads) {
+        ot = fmaxf(ot, fa_dpp<0xb1>(ot)); ot = fmaxf(ot, fa_dpp<0x4e>(ot));
+#pragma unroll
+        for (int i = 0; i < 64; i += 4) above += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ot), i)) > ot;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) above += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ot), i)) > ot;
+    }
+    const float wm = wave_max(top), wb = -wave_max(4 * above < a.n_out ? -ot : -INFINITY);          // (4 above < n_out: fewer than n_out / 4, rounded up, are before it)
+    if (lane == 0) { s_red[wave] = wm; s_red[8 + wave] = wb; }
     if (tid == 0) s_n = 0;
     __syncthreads();
-    const float m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-    if (tid < owners) {          // the owner with n_out - 1 better ones before it (owners differ in their index, so there is one)
-        const u64 mine = s_own[tid]; int rank = 0;
-#pragma unroll 8
-        for (int i = 0; i < owners; ++i) rank += s_own[i] > mine;
-        if (rank == a.n_out - 1) s_bound = mine;
+    const float m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3])), least = fminf(fminf(s_red[8], s_red[9]), fminf(s_red[10], s_red[11]));
+    bool by_keys = least == -INFINITY;
+    if (!by_keys) {
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) if (v[e] >= least) { const int p = atomicAdd(&s_n, 1); if (p < CAP) s_list[p] = logit_key(v[e], base + index(e)); }
     }
     float l = 0.f;
     if (m != -INFINITY) {
@@ -81,14 +90,7 @@ template <int EPT> __global__ void __launch_bounds__(256) beam_scan_kernel(BeamA
     l = wave_sum_dpp(l);
     if (lane == 0) s_red[4 + wave] = l;
     __syncthreads();
-    const float least = key_logit(s_bound);
-    bool by_keys = least == -INFINITY;
-    if (!by_keys) {
-#pragma unroll
-        for (int e = 0; e < EPT; ++e) if (v[e] >= least) { const int p = atomicAdd(&s_n, 1); if (p < CAP) s_list[p] = logit_key(v[e], base + index(e)); }
-        __syncthreads();
-        by_keys = s_n > CAP;
-    }
+    if (!by_keys) by_keys = s_n > CAP;
     if (by_keys) {          // (uniform)
         u64 own = 0;
 #pragma unroll
@@ -146,13 +148,15 @@ static __device__ __forceinline__ int rank_among(const Cand *s, int n, const Can
 constexpr int BEAM_LIST = BEAM_MAX_OUT * ((BEAM_MAX_LISTS + 255) / 256);
 struct JoinMem { Cand own[256], list[BEAM_LIST], bound; int n; };
 // The k best of get(0 .. n), sorted, into out (LDS); returns how many there are.  1024 threads: a quad of lanes to a candidate (ranking is the longest part: 128 + 136 comparisons of
-// 64 bits for a group of 8 beams and 16 results; with one lane to a candidate the launch took 18 us).  `first` is get(this lane's first index), n at most 256 times the share that JoinMem
-// is made for.
+// 64 bits for a group of 8 beams and 16 results; with one lane to a candidate the launch took 18 us).  `mine` are the lane's first OWN candidates, made by the caller so that their loads are
+// under way together; get(i) makes those behind them.  n is at most 256 times the share that JoinMem is made for.
 static __device__ __forceinline__ int first_of_lane() { return (int)(threadIdx.x >> 2) + 256 * (int)(threadIdx.x & 3); }
-template <typename F> static __device__ __forceinline__ int choose(int n, int k, const Cand &first, F get, Cand *out, JoinMem &mem) {
+template <int OWN, typename F> static __device__ __forceinline__ int choose(int n, int k, const Cand (&mine)[OWN], F get, Cand *out, JoinMem &mem) {
     const int quad = threadIdx.x >> 2; const bool lead = (threadIdx.x & 3) == 0;
-    Cand best = first;
-    for (int i = first_of_lane() + 1024; i < n; i += 1024) { const Cand q = get(i); if (before(q, best)) best = q; }
+    Cand best = mine[0];
+#pragma unroll
+    for (int p = 1; p < OWN; ++p) if (before(mine[p], best)) best = mine[p];
+    for (int i = first_of_lane() + OWN * 1024; i < n; i += 1024) { const Cand q = get(i); if (before(q, best)) best = q; }
 #pragma unroll
     for (int d = 1; d <= 2; ++d) { const Cand q = {quad_xor(best.value, d), quad_xor(best.rest, d)}; if (before(q, best)) best = q; }
     if (lead) mem.own[quad] = best;
@@ -167,7 +171,10 @@ template <typename F> static __device__ __forceinline__ int choose(int n, int k,
     if (lead && rank == k - 1) mem.bound = best;
     __syncthreads();
     const Cand bound = mem.bound;
-    for (int i = threadIdx.x; i < n; i += 1024) { const Cand q = get(i); if (q.rest && !before(bound, q)) mem.list[atomicAdd(&mem.n, 1)] = q; }
+    auto take = [&](const Cand &q) { if (q.rest && !before(bound, q)) mem.list[atomicAdd(&mem.n, 1)] = q; };
+#pragma unroll
+    for (int p = 0; p < OWN; ++p) take(mine[p]);
+    for (int i = first_of_lane() + OWN * 1024; i < n; i += 1024) take(get(i));
     __syncthreads();
     const int count = mem.n;
     for (int i = quad; i < count; i += 256) { const Cand q = mem.list[i]; const int r = rank_among(mem.list, count, q); if (lead && r < k) out[r] = q; }
@@ -176,12 +183,15 @@ template <typename F> static __device__ __forceinline__ int choose(int n, int k,
 }
 // One workgroup per group.  Only the n_out lists with the best heads can hold any of the n_out best, and of the list with rank r among them only its first n_out - r entries.
 // Bound by its chain of memory latencies (statistics, then the lists' entries): the heads are requested before the statistics.
-__global__ void __launch_bounds__(1024) beam_join_kernel(BeamArgs a) {
+// OWN: candidates of a group are at most that many times 1024 (1: up to 44 results; with 3 for all the small ones take 0.5 us more, the largest 1.2 us less).
+template <int OWN> __global__ void __launch_bounds__(1024) beam_join_kernel(BeamArgs a) {
     __shared__ float s_top[BEAM_MAX_BEAMS], s_score[BEAM_MAX_BEAMS]; __shared__ double s_lse[BEAM_MAX_BEAMS]; __shared__ int s_kind[BEAM_MAX_BEAMS];       // 0: logits, 1: finished, 2: nothing but -inf
     __shared__ JoinMem mem; __shared__ Cand s_heads[BEAM_MAX_OUT], s_best[BEAM_MAX_OUT];
     const int g = blockIdx.x, tid = threadIdx.x, k = a.n_out, lists = a.n_beam * a.chunks;
     const u64 *best = a.best + (long)g * lists * k;
-    const int l1 = min(first_of_lane(), lists - 1); const u64 head = best[(long)l1 * k];
+    u64 head[OWN];
+#pragma unroll
+    for (int p = 0; p < OWN; ++p) if (p * 1024 < lists) head[p] = best[(long)min(first_of_lane() + p * 1024, lists - 1) * k];
     for (int b0 = 0; b0 < a.n_beam; b0 += 64) {          // 16 lanes to a beam
         const int b = b0 + (tid >> 4), r = g * a.n_beam + min(b, a.n_beam - 1);
         const float2 *stat = a.stat + (long)r * a.chunks;
@@ -221,24 +231,35 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(BeamArgs a) {
         const int t = kind == 2 ? e : e == 0 ? a.pad : e - 1 < a.pad ? e - 1 : e;
         return made(kind == 1 && e == 0 ? (double)s_score[b] : -INFINITY, b, logit_key(-INFINITY, t));
     };
-    const int b1 = l1 / a.chunks;
-    const int heads = choose(lists, k, first_of_lane() < lists ? entry(b1, l1 - b1 * a.chunks, 0, head) : Cand{0, 0},
-                             [&](int i) { const int b = i / a.chunks; return entry(b, i - b * a.chunks, 0, best[(long)i * k]); }, s_heads, mem);
-    auto wanted = [&](int i) {          // i = r (r + 1) / 2 + e: entry e <= r of the list with rank k - 1 - r
+    Cand mine[OWN];
+#pragma unroll
+    for (int p = 0; p < OWN; ++p) {
+        mine[p] = {0, 0}; const int i = first_of_lane() + p * 1024;
+        if (p * 1024 < lists && i < lists) { const int b = i / a.chunks; mine[p] = entry(b, i - b * a.chunks, 0, head[p]); }
+    }
+    const int heads = choose(lists, k, mine, [&](int i) { const int b = i / a.chunks; return entry(b, i - b * a.chunks, 0, best[(long)i * k]); }, s_heads, mem);
+    // candidate i = r (r + 1) / 2 + e: entry e <= r of the list with rank h = k - 1 - r, which is entry e of chunk c of beam b; h -1: there is none
+    struct Place { int h, e, b, c; };
+    auto place = [&](int i) {
         int r = (int)((sqrtf(8.0f * i + 1.0f) - 1.0f) * 0.5f);
         while (r * (r + 1) / 2 > i) --r;
         while ((r + 1) * (r + 2) / 2 <= i) ++r;
-        const int e = i - r * (r + 1) / 2, h = k - 1 - r;
-        if (h < 0 || h >= heads) return Cand{0, 0};
-        const Cand q = s_heads[h];
-        if (e == 0) return q;
-        const int b = beam_of(q), c = s_kind[b] ? 0 : token_of(q) >> shift;          // (the chunk of a head is where its token lies)
-        return entry(b, c, e, best[(long)(b * a.chunks + c) * k + e]);
+        Place p = {k - 1 - r, i - r * (r + 1) / 2, 0, 0};
+        if (p.h < 0 || p.h >= heads) p.h = -1;
+        else { const Cand q = s_heads[p.h]; p.b = beam_of(q); p.c = s_kind[p.b] ? 0 : token_of(q) >> shift; }          // (the chunk of a head is where its token lies)
+        return p;
     };
-    const int total = k * (k + 1) / 2;
-    const Cand mine = first_of_lane() < total ? wanted(first_of_lane()) : Cand{0, 0};
+    const int total = k * (k + 1) / 2;          // (at most OWN * 1024)
+    Place at[OWN]; u64 key[OWN];
+#pragma unroll
+    for (int p = 0; p < OWN; ++p) if (p * 1024 < total) { at[p] = place(first_of_lane() + p * 1024); key[p] = at[p].h >= 0 && at[p].e ? best[(long)(at[p].b * a.chunks + at[p].c) * k + at[p].e] : 0; }
+#pragma unroll
+    for (int p = 0; p < OWN; ++p) {
+        mine[p] = {0, 0};
+        if (p * 1024 < total && at[p].h >= 0) mine[p] = at[p].e == 0 ? s_heads[at[p].h] : entry(at[p].b, at[p].c, at[p].e, key[p]);
+    }
     __syncthreads();          // (mem is free)
-    const int found = choose(total, k, mine, wanted, s_best, mem);
+    const int found = choose(total, k, mine, [](int) { return Cand{0, 0}; }, s_best, mem);
     for (int i = tid; i < found; i += 1024) {
         const Cand q = s_best[i]; const long o = (long)g * k + i;
         a.score_out[o] = (float)unordered(q.value); a.parent[o] = g * a.n_beam + beam_of(q); a.token[o] = token_of(q);
@@ -253,8 +274,9 @@ static int64_t beam_check(const cdna4_tensor *x, int n_beam, int n_out, int pad,
     OP_CHECK(n_out >= 1 && n_out <= BEAM_MAX_OUT && n_out <= x->ne[0] * n_beam, "beam_select: 1 <= n_out <= min(64, n_beam * n_vocab)");
     ARG_CHECK(pad >= 0 && pad < x->ne[0], "beam_select: pad is a token");
     a->logits = (const char *)x->data; a->row = x->nb[1]; a->n_vocab = (int)x->ne[0]; a->n_beam = n_beam; a->n_out = n_out; a->pad = pad;
-    // 2048 logits to a workgroup where 8192 would leave most of the chip idle (fewer than 256 workgroups)
-    a->chunk = x->ne[1] * ((x->ne[0] + BEAM_CHUNK - 1) / BEAM_CHUNK) < 256 ? BEAM_CHUNK / 4 : BEAM_CHUNK;
+    // 2048 logits to a workgroup where 8192 would leave most of the chip idle (fewer than 256 workgroups) or more than a fifth of its lanes (1000 rows of 4000: 20.2 -> 17.4 us)
+    const long whole = (x->ne[0] + BEAM_CHUNK - 1) / BEAM_CHUNK;
+    a->chunk = x->ne[1] * whole < 256 || whole * BEAM_CHUNK * 4 > x->ne[0] * 5 ? BEAM_CHUNK / 4 : BEAM_CHUNK;
     a->chunks = (a->n_vocab + a->chunk - 1) / a->chunk;
     return x->ne[1] * a->chunks * (8 + 8 * (int64_t)n_out);
 }
@@ -278,6 +300,8 @@ int cdna4_op_beam_select(cdna4_context *ctx, const cdna4_tensor *logits, const f
     if (a.chunk == BEAM_CHUNK) hipLaunchKernelGGL(beam_scan_kernel<32>, grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(beam_scan_kernel<8>, grid, dim3(256), 0, st, a);
     HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)(rows / n_beam)), dim3(1024), 0, st, a);
+    static_assert(BEAM_MAX_OUT * (BEAM_MAX_OUT + 1) / 2 <= 3 * 1024, "the candidates of a group are its lanes' own");
+    if (n_out * (n_out + 1) / 2 <= 1024) hipLaunchKernelGGL(beam_join_kernel<1>, dim3((unsigned)(rows / n_beam)), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL(beam_join_kernel<3>, dim3((unsigned)(rows / n_beam)), dim3(1024), 0, st, a);
     HIP_TRY(hipGetLastError()); return CDNA4_OK;
 }

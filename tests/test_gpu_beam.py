@@ -90,3 +90,15 @@ def test_repeats_bit_for_bit_and_in_a_graph(backend):
         assert all(torch.equal(a, b) for a, b in zip(outs, eager))
         if not i:
             assert all(torch.equal(a, b) for a, b in zip(outs, base))
+
+
+@pytest.mark.parametrize("n_group,n_beam,n_out,n_vocab", [(1, 256, 64, 20000), (1, 256, 50, 10000), (1, 200, 44, 14000), (2, 150, 45, 9000), (700, 1, 3, 4000), (3, 7, 23, 2049), (5, 3, 61, 2300), (300, 2, 17, 8193)])
+def test_many_lists_and_cut_chunks(n_group, n_beam, n_out, n_vocab, backend):
+    """more chunks of a group than the join has lanes, chunks with a few logits in them, waves without a finite one"""
+    r = np.random.default_rng(n_vocab)
+    x = (r.standard_normal((n_group * n_beam, n_vocab)) * 2).astype(np.float32); score = (-3 * r.random(n_group * n_beam)).astype(np.float32)
+    check(backend, x, score, n_beam, n_out)
+    x[:, n_vocab // 3:] = -np.inf; x[:, 5:300] = -np.inf; x[::2, :n_vocab // 3] = -np.inf; x[::2, -3:] = 1.0
+    check(backend, x, score, n_beam, n_out)
+    x[:] = np.round(r.standard_normal(x.shape)).astype(np.float32)                                                    # a few values, each many times
+    check(backend, x, np.zeros_like(score), n_beam, n_out)
