@@ -174,15 +174,13 @@ struct EvictArgs {
     int *moves;                                                                                                                           // [count, from[max], to[max]]
 };
 // sort key of a slot: larger = kept first.  Held slots above everything, then the order of the floats (-0 as 0, NaN as -inf)
-static __device__ __forceinline__ uint32_t evict_key(float w, int p, int sink, long recent_from) {
-    if (p < sink || (long)p >= recent_from) return 0xffffffffu;
-    if (w != w) w = -INFINITY;
-    const uint32_t b = __float_as_uint(w + 0.0f);
-    return b ^ ((b & 0x80000000u) ? 0xffffffffu : 0x80000000u);
+static __device__ __forceinline__ uint32_t evict_key(float w, int p, int sink, int recent_from) {
+    const uint32_t b = __float_as_uint(fmaxf(w + 0.0f, -INFINITY)), key = b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+    return p < sink || p >= recent_from ? 0xffffffffu : key;
 }
 // One workgroup per (sequence, KV head): a chain of dependent steps over n slots, so what counts is that weight and pos are read from memory once, that many of their bytes are under way at
 // a time and that the steps are few and short.
-// * The first pass (16 bytes a lane) turns weight and pos into keys in LDS (up to 32768; a longer row computes them again in every pass: 130000 slots cut to 100: 94 us) and copies what lies before the budget to
+// * The first pass (16 bytes a lane) turns weight and pos into keys in LDS (up to 32768; a longer row computes them again in every pass: 130000 slots cut to 100: 80 us) and copies what lies before the budget to
 //   weight_out / pos_out: of those slots the freed ones are written again by the moves.
 // * The budget-th largest key by digits of 11, 11 and 10 bits, the first counted while the keys are made.  Two copies of the histogram by lane parity: weights share few leading digits and
 //   adds to one address follow one another.  As soon as all keys of the bin in question are kept the search is over: with weights that differ, after the second digit.
@@ -190,8 +188,8 @@ static __device__ __forceinline__ uint32_t evict_key(float w, int p, int sink, l
 //   among equals are taken only if not all keys that equal the last kept one are kept.
 // * Few moves (`here`: at most EVICT_HERE a row, as when a cache is cut back after every few tokens) are made in the same launch from lists in LDS; otherwise the lists go to memory and a
 //   second launch moves the rows with the whole chip.
-// Measured: 128 rows of up to 4160 slots cut to 4096: one launch of 10.4 us (reading 3, digits 2.4, lists 2, moves 2).  32 rows of up to 32768 slots cut to 4096: 25 us (reading 6.4, digits
-// 5, lists 8: the instructions of 32 of the 256 CUs) and 25 us for the moves (108 MB, 4.3 TB/s).
+// Measured: 128 rows of up to 4160 slots cut to 4096: one launch of 10.2 us (reading 3, digits 2.4, lists 2, moves 2).  32 rows of up to 32768 slots cut to 4096: 24 us (reading 6, digits 5,
+// lists 7: the vector instructions of 32 of the 256 CUs, some 20 for every slot in each) and 25 us for the moves (108 MB, 4.3 TB/s).
 constexpr int EVICT_THREADS = 1024, EVICT_WAVES = 16, EVICT_KEYS = 32768, EVICT_HERE = 128, EVICT_BINS = 2048, EVICT_COPIES = 2;
 static __device__ __forceinline__ void evict_move(const EvictArgs &a, int s, int h, int from, int to, int sub) {          // 16 lanes to a row: K, V, weight and pos
     if (sub == 0) {
@@ -227,9 +225,9 @@ static __device__ __forceinline__ unsigned waves_before(const unsigned (&tot)[EV
 template <bool HERE> __global__ void __launch_bounds__(EVICT_THREADS) paged_evict_select_kernel(EvictArgs a) {
     extern __shared__ uint32_t s_key[];
     __shared__ unsigned hist[EVICT_BINS * EVICT_COPIES], tot[3][EVICT_WAVES], s_digit, s_rest, s_equal; __shared__ int s_moves[HERE ? 2 * EVICT_HERE : 1];
-    const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int raw = a.c.n_kv[s], n = paged_len(a.c, s), most = (a.list - 1) / 2;
-    const long recent_from = (long)a.n_past[s] - a.recent;
+    const int recent_from = (int)max((long)a.n_past[s] - a.recent, -(1l << 31));
     int *moves = HERE ? nullptr : a.moves + ((long)s * a.c.n_head_kv + h) * a.list;
     const float *w = slot_row<const float>(a.weight, s, h); const int *p = slot_row<const int>(a.pos, s, h);
     float *wo = slot_row<float>(a.weight_out, s, h); int *po = slot_row<int>(a.pos_out, s, h);
@@ -321,13 +319,14 @@ template <bool HERE> __global__ void __launch_bounds__(EVICT_THREADS) paged_evic
         unsigned t = tie0, found = 0, lane_holes = 0, lane_movers = 0;
         for (int b = j0; b < j1; b += 256) {
             const int j = b + 4 * lane; const uint4 k = keys4(min(j, (n - 1) & ~3)); const uint32_t x[4] = {k.x, k.y, k.z, k.w};
-            unsigned keep = 0, in = 0;
+            unsigned keep = 0, in = 15u;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { in |= (j + i < j1) << i; keep |= (x[i] >= prefix) << i; }
+            for (int i = 3; i >= 0; --i) keep = 2 * keep + (x[i] >= prefix);
+            if (b + 256 > j1) in = j1 >= j + 4 ? 15u : j1 <= j ? 0u : (1u << (j1 - j)) - 1;
             if (!all_equal) {
                 unsigned tie = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) tie |= (x[i] == prefix) << i;
+                for (int i = 3; i >= 0; --i) tie = 2 * tie + (x[i] == prefix);
                 tie &= in;
                 const unsigned mine = __popc(tie), upto = wave_scan(mine);
                 unsigned r = t + upto - mine;
@@ -335,7 +334,7 @@ template <bool HERE> __global__ void __launch_bounds__(EVICT_THREADS) paged_evic
                 for (int i = 0; i < 4; ++i) if ((tie >> i) & 1) { if (r >= rest) keep &= ~(1u << i); ++r; }
                 t += (unsigned)__builtin_amdgcn_readlane((int)upto, 63);
             }
-            const unsigned before = a.budget >= j + 4 ? 15u : a.budget <= j ? 0u : (1u << (a.budget - j)) - 1;      // the lane's slots before the budget
+            const unsigned before = b + 256 <= a.budget ? 15u : b >= a.budget ? 0u : a.budget >= j + 4 ? 15u : a.budget <= j ? 0u : (1u << (a.budget - j)) - 1;      // the lane's slots before the budget
             const unsigned hole = in & ~keep & before, mover = in & keep & ~before, c = __popc(hole) | (__popc(mover) << 16);
             if (!round) { lane_holes += c & 0xffffu; lane_movers += c >> 16; continue; }
             const unsigned upto = wave_scan(c), at = found + upto - c;
