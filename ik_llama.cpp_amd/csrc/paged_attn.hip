@@ -9,7 +9,7 @@
 // * f32 results from 16-bit operands: q and p are split into two f16 (2^-22; q scaled by a power of two, p by 2^8) or three bf16 (exactly 24 bits) terms, K and V are what the cache
 //   holds; products and sums are f32.  The extra matrix instructions stay far below the load time (32 or 48 of 16 clk per 16 KB and SIMD).
 // * Equal shares: all tiles of 128 slots of all (sequence, KV head) pairs are numbered through, and every workgroup takes an equal contiguous range of the numbers, from the lengths as
-//   they are on the device.  Groups of more than 16 query heads: the blocks of 16 have workgroups of their own, with the same ranges.  A long sequence in a batch of short ones spreads over the chip by itself; a workgroup that covers a unit alone writes its result, the others
+//   they are on the device.  Groups of more than 16 query heads: 32 to a wave, or blocks of 16 with workgroups of their own and the same ranges.  A long sequence in a batch of short ones spreads over the chip by itself; a workgroup that covers a unit alone writes its result, the others
 //   leave (max, sum, accumulator) for the join.
 //
 // Measured (8 KV heads of 128): 64 sequences of up to 8192 slots, f16, 32 query heads: 1.12 GB in 197 us + 6 us for the join, 5.5 TB/s; one of 131071, bf16, 64 query heads: 537 MB in 92 -
@@ -25,15 +25,15 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int TILE = 128, WAVES = 4, QH = 16;         // slots of a workgroup's tile (32 a wave), waves, query heads of a unit
+constexpr int TILE = 128, WAVES = 4, QH = 16;         // slots of a workgroup's tile (32 a wave), waves, query heads of a matrix instruction
 constexpr int ONE_LDS = 104 * 1024;                   // most dynamic LDS of a workgroup that has a unit to itself (and more than the others take)
 constexpr int ATTN_MAX_WG = 1024;                     // most workgroups of a launch; the size function, which knows no device, counts with it
 
 struct AttnArgs {
     PagedCache c; const char *q; long q_head, q_seq; char *dst; long d_head, d_seq; char *weight; long w_head, w_seq;
-    int group, n_head, blocks, n_wg; float scale, softcap, inv_softcap;          // blocks: of 16 query heads in a group; n_wg: workgroups that share the tiles of one block of every group
+    int group, n_head, lg, blocks, n_wg; float scale, softcap, inv_softcap;      // blocks: of 2^lg query heads in a group; n_wg: workgroups that share the tiles of one block of every group
     int *prefix;                // [n_seq + 1] tiles of a unit before sequence s
-    float *part;                // [blocks][n_wg][2][QH][D + 2]: what a workgroup leaves of its first / last unit (max, sum, accumulator of every head)
+    float *part;                // [blocks][n_wg][2][2^lg][D + 2]: what a workgroup leaves of its first / last unit (max, sum, accumulator of every head)
     float2 *stat;               // [n_seq][n_head] max and sum of a row (weight only)
     float *score; long score_row;   // [n_seq][n_head][score_row] scores in units of log 2 (weight only)
 };
@@ -108,10 +108,11 @@ struct Shares {
 };
 
 // ONE: a workgroup per unit (grid: units, sequences), for tables of few slots: no shares, nothing to join, and the weights are added from scores in LDS by the same launch.
-template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds__(256) paged_attn_kernel(AttnArgs a) {
-    constexpr int KC = D / 32, VW = D == 64 ? 4 : 8, VH = D == 256 ? 2 : 1, NS = Split<BF16>::N;      // K chunks of 32 elements; V elements of a lane and half; halves of 128
+// QB: blocks of 16 query heads that a wave takes.
+template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch_bounds__(256) paged_attn_kernel(AttnArgs a) {
+    constexpr int HEADS = QB * QH, KC = D / 32, VW = D == 64 ? 4 : 8, VH = D == 256 ? 2 : 1, NS = Split<BF16>::N;      // K chunks of 32 elements; V elements of a lane and half; halves of 128
     extern __shared__ int s_mem[];
-    __shared__ int s_tot[4]; __shared__ float s_m[WAVES][QH], s_l[WAVES][QH], s_row[2][QH];
+    __shared__ int s_tot[4]; __shared__ float s_m[WAVES][HEADS], s_l[WAVES][HEADS], s_row[2][HEADS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     int *pre = s_mem;                                                              // prefix sums (not ONE)
     float *s_o = reinterpret_cast<float *>(s_mem + (ONE ? 0 : (a.c.n_seq + 4) & ~3));       // [WAVES][heads][D + 4]
@@ -137,12 +138,15 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
             ntile = min(tiles - tile0, x_end - x);
             x += ntile;
         }
-        const int h0 = hk * a.group + blk * QH, heads = min(QH, (hk + 1) * a.group - h0);
-        // the queries: chunk c holds elements 32 c + 8 g ... + 7 of head `col`; requested before the cache rows, split under their way
-        const float *qr = reinterpret_cast<const float *>(a.q + (long)s * a.q_seq + (long)(h0 + min(col, heads - 1)) * a.q_head) + 8 * g;
-        float4 x0[KC], x1[KC];
+        const int h0 = hk * a.group + blk * HEADS, heads = min(HEADS, (hk + 1) * a.group - h0);
+        // the queries: chunk c holds elements 32 c + 8 g ... + 7 of head 16 b + col; requested before the cache rows, split under their way
+        float4 x0[QB][KC], x1[QB][KC];
 #pragma unroll
-        for (int c = 0; c < KC; ++c) { x0[c] = reinterpret_cast<const float4 *>(qr + 32 * c)[0]; x1[c] = reinterpret_cast<const float4 *>(qr + 32 * c)[1]; }
+        for (int b = 0; b < QB; ++b) {
+            const float *qr = reinterpret_cast<const float *>(a.q + (long)s * a.q_seq + (long)(h0 + min(QH * b + col, heads - 1)) * a.q_head) + 8 * g;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) { x0[b][c] = reinterpret_cast<const float4 *>(qr + 32 * c)[0]; x1[b][c] = reinterpret_cast<const float4 *>(qr + 32 * c)[1]; }
+        }
         const char *kb = a.c.k + (long)hk * a.c.k_head, *vb = a.c.v + (long)hk * a.c.v_head;
         const int *table = a.c.table + (long)s * a.c.table_row; const int in_page = (1 << a.c.page_shift) - 1;
         // 16 slots from j on lie in one page (pages are powers of two >= 16).  Its entry in the table (requested without a branch: the last one stands for those past the end), and the id that
@@ -178,79 +182,89 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
                     }
             }
         };
-        f4 o[VH][VW];
+        f4 o[QB][VH][VW]; float m[QB], l[QB];
 #pragma unroll
-        for (int hf = 0; hf < VH; ++hf)
+        for (int b = 0; b < QB; ++b) {
+            m[b] = -INFINITY; l[b] = 0.f;
 #pragma unroll
-            for (int i = 0; i < VW; ++i) o[hf][i] = (f4){0.f, 0.f, 0.f, 0.f};
-        float m = -INFINITY, l = 0.f;
+            for (int hf = 0; hf < VH; ++hf)
+#pragma unroll
+                for (int i = 0; i < VW; ++i) o[b][hf][i] = (f4){0.f, 0.f, 0.f, 0.f};
+        }
         int j = (tile0 * WAVES + wave) * 32; const int j_end = min((tile0 + ntile) * TILE, n);
-        const int hc = min(col, heads - 1);
-        float *score = !a.weight ? nullptr : ONE ? s_o + WAVES * heads * (D + 4) + hc * (int)a.score_row : a.score + ((long)s * a.n_head + h0 + hc) * a.score_row;
-        u4 q[NS][KC]; float unscale = 1.0f; int id0 = -1, id1 = -1, nx0 = -1, nx1 = -1;
+        float *score = !a.weight ? nullptr : ONE ? s_o + WAVES * heads * (D + 4) : a.score + ((long)s * a.n_head + h0) * a.score_row;          // of the unit's first head
+        u4 q[QB][NS][KC]; float unscale[QB]; int id0 = -1, id1 = -1, nx0 = -1, nx1 = -1;
         // One step: the tile in kr / vr.  MORE: the next tile is requested on the way, K as soon as its registers are read, V at the end.  (The last tile is a step of its own and not a
         // condition around the loads: behind a condition the compiler waits for V of the next tile before the first product of K.)
         auto step = [&](auto more) {
             constexpr bool MORE = decltype(more)::value;
-            f4 z[2];
+            f4 z[QB][2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                z[t] = (f4){0.f, 0.f, 0.f, 0.f};
+            for (int b = 0; b < QB; ++b)
 #pragma unroll
-                for (int c = 0; c < KC; ++c)
+                for (int t = 0; t < 2; ++t) {
+                    z[b][t] = (f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int k = NS - 1; k >= 0; --k) z[t] = mfma<BF16>(kr[t][c], q[k][c], z[t]);
-            }
+                    for (int c = 0; c < KC; ++c)
+#pragma unroll
+                        for (int k = NS - 1; k >= 0; --k) z[b][t] = mfma<BF16>(kr[t][c], q[b][k][c], z[b][t]);
+                }
             const int jn = j + TILE; int e0 = 0, e1 = 0;
             if constexpr (MORE) { load_k(jn, nx0, nx1); e0 = entry(jn + TILE); e1 = entry(jn + TILE + 16); }
             const bool whole = id0 >= 0 && id1 >= 0 && j + 32 <= n;          // (wave-uniform)
+            uint32_t p[QB][NS][4];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float v = z[t][r] * unscale;
-                    if constexpr (CAP) v = a.softcap * 1.44269504088896341f * tanh_of(v * a.inv_softcap);
-                    z[t][r] = v;
-                }
-            if (!whole) {
+            for (int b = 0; b < QB; ++b) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) if ((t ? id1 : id0) < 0 || j + 16 * t + 4 * g + r >= n) {
-                        z[t][r] = -INFINITY;
+                    for (int r = 0; r < 4; ++r) {
+                        float v = z[b][t][r] * unscale[b];
+                        if constexpr (CAP) v = a.softcap * 1.44269504088896341f * tanh_of(v * a.inv_softcap);
+                        z[b][t][r] = v;
+                    }
+                if (!whole) {
 #pragma unroll
-                        for (int hf = 0; hf < VH; ++hf)
+                    for (int t = 0; t < 2; ++t)
 #pragma unroll
-                            for (int i = 0; i < VW / 2; ++i) vr[4 * t + r][hf][i] = 0u;          // (0 times what an unused slot holds may be NaN)
+                        for (int r = 0; r < 4; ++r) if ((t ? id1 : id0) < 0 || j + 16 * t + 4 * g + r >= n) {
+                            z[b][t][r] = -INFINITY;
+                            if (b == 0) {
+#pragma unroll
+                                for (int hf = 0; hf < VH; ++hf)
+#pragma unroll
+                                    for (int i = 0; i < VW / 2; ++i) vr[4 * t + r][hf][i] = 0u;          // (0 times what an unused slot holds may be NaN)
+                            }
+                        }
+                }
+                if (score && QH * b + col < heads) {
+                    float *to = score + (long)(QH * b + col) * a.score_row + j + 4 * g;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) *reinterpret_cast<f4 *>(to + 16 * t) = z[b][t];
+                }
+                float top = fmaxf(fmaxf(fmaxf(z[b][0][0], z[b][0][1]), fmaxf(z[b][0][2], z[b][0][3])), fmaxf(fmaxf(z[b][1][0], z[b][1][1]), fmaxf(z[b][1][2], z[b][1][3])));
+                top = over_rows(top, [](float p, float r) { return fmaxf(p, r); });
+                // the reference value of the exponentials follows the maximum only when that has grown by 2^6: 2^8 p stays below 2^14 in f16
+                if (__ballot(top > m[b] + 6.0f)) {
+                    const float to = fmaxf(m[b], top), f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[b] - to);
+                    m[b] = to; l[b] *= f;
+#pragma unroll
+                    for (int hf = 0; hf < VH; ++hf)
+#pragma unroll
+                        for (int i = 0; i < VW; ++i) o[b][hf][i] *= f;
+                }
+                const float ref = m[b] == -INFINITY ? 0.f : m[b] - 8.0f;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; r += 2) {
+                        const float p0 = __builtin_amdgcn_exp2f(z[b][t][r] - ref), p1 = __builtin_amdgcn_exp2f(z[b][t][r + 1] - ref);
+                        l[b] += p0 + p1;
+                        uint32_t w[NS]; Split<BF16>::of(p0, p1, w);
+#pragma unroll
+                        for (int k = 0; k < NS; ++k) p[b][k][2 * t + r / 2] = w[k];
                     }
             }
-            if (score && col < heads) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t) *reinterpret_cast<f4 *>(score + j + 16 * t + 4 * g) = z[t];
-            }
-            float top = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])), fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
-            top = over_rows(top, [](float p, float r) { return fmaxf(p, r); });
-            // the reference value of the exponentials follows the maximum only when that has grown by 2^6: 2^8 p stays below 2^14 in f16
-            if (__ballot(top > m + 6.0f)) {
-                const float to = fmaxf(m, top), f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
-                m = to; l *= f;
-#pragma unroll
-                for (int hf = 0; hf < VH; ++hf)
-#pragma unroll
-                    for (int i = 0; i < VW; ++i) o[hf][i] *= f;
-            }
-            const float ref = m == -INFINITY ? 0.f : m - 8.0f;
-            uint32_t p[NS][4];
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; r += 2) {
-                    const float p0 = __builtin_amdgcn_exp2f(z[t][r] - ref), p1 = __builtin_amdgcn_exp2f(z[t][r + 1] - ref);
-                    l += p0 + p1;
-                    uint32_t w[NS]; Split<BF16>::of(p0, p1, w);
-#pragma unroll
-                    for (int k = 0; k < NS; ++k) p[k][2 * t + r / 2] = w[k];
-                }
 #pragma unroll
             for (int hf = 0; hf < VH; ++hf)
 #pragma unroll
@@ -260,7 +274,9 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
 #pragma unroll
                     for (int w = 0; w < 4; ++w) vt[w] = __builtin_amdgcn_perm(vr[2 * w + 1][hf][i / 2], vr[2 * w][hf][i / 2], sel);
 #pragma unroll
-                    for (int k = NS - 1; k >= 0; --k) o[hf][i] = mfma<BF16>(vt, (u4){p[k][0], p[k][1], p[k][2], p[k][3]}, o[hf][i]);
+                    for (int b = 0; b < QB; ++b)
+#pragma unroll
+                        for (int k = NS - 1; k >= 0; --k) o[b][hf][i] = mfma<BF16>(vt, (u4){p[b][k][0], p[b][k][1], p[b][k][2], p[b][k][3]}, o[b][hf][i]);
                 }
             if constexpr (MORE) { load_v(jn, nx0, nx1); id0 = nx0; id1 = nx1; nx0 = id_of(e0, jn + TILE); nx1 = id_of(e1, jn + TILE + 16); j = jn; }
         };
@@ -269,54 +285,65 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
             id0 = id_of(e0, j); id1 = id_of(e1, j + 16); nx0 = id_of(e2, j + TILE); nx1 = id_of(e3, j + TILE + 16);
             load_k(j, id0, id1); load_v(j, id0, id1);
             __builtin_amdgcn_sched_barrier(0);          // (V too is requested before the split of the queries)
-            float top = 0.f; const float pre_scale = CAP ? a.scale : a.scale * 1.44269504088896341f;
-            float up = 1.0f;
-            if constexpr (!BF16) {          // a power of two that puts the largest element into [2^10, 2^11): the f16 terms neither overflow nor lose bits to the smallest exponent
+            const float pre_scale = CAP ? a.scale : a.scale * 1.44269504088896341f;
 #pragma unroll
-                for (int c = 0; c < KC; ++c) top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(x0[c].x), fabsf(x0[c].y)), fmaxf(fabsf(x0[c].z), fabsf(x0[c].w))),
-                                                                   fmaxf(fmaxf(fabsf(x1[c].x), fabsf(x1[c].y)), fmaxf(fabsf(x1[c].z), fabsf(x1[c].w)))));
-                top = over_rows(top, [](float p, float r) { return fmaxf(p, r); });
-                const int e = top > 0.f ? min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100), 127) : 0;
-                up = __uint_as_float((uint32_t)(127 + 10 - e) << 23); unscale = __uint_as_float((uint32_t)(127 - 10 + e) << 23);
-            }
-            unscale *= pre_scale;
+            for (int b = 0; b < QB; ++b) {
+                float up = 1.0f; unscale[b] = pre_scale;
+                if constexpr (!BF16) {          // a power of two that puts the largest element into [2^10, 2^11): the f16 terms neither overflow nor lose bits to the smallest exponent
+                    float top = 0.f;
 #pragma unroll
-            for (int c = 0; c < KC; ++c) {
-                const float e[8] = {x0[c].x, x0[c].y, x0[c].z, x0[c].w, x1[c].x, x1[c].y, x1[c].z, x1[c].w};
+                    for (int c = 0; c < KC; ++c) top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(x0[b][c].x), fabsf(x0[b][c].y)), fmaxf(fabsf(x0[b][c].z), fabsf(x0[b][c].w))),
+                                                                       fmaxf(fmaxf(fabsf(x1[b][c].x), fabsf(x1[b][c].y)), fmaxf(fabsf(x1[b][c].z), fabsf(x1[b][c].w)))));
+                    top = over_rows(top, [](float p, float r) { return fmaxf(p, r); });
+                    const int e = top > 0.f ? min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100), 127) : 0;
+                    up = __uint_as_float((uint32_t)(127 + 10 - e) << 23); unscale[b] = __uint_as_float((uint32_t)(127 - 10 + e) << 23) * pre_scale;
+                }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { uint32_t t[NS]; Split<BF16>::of(e[2 * i] * up, e[2 * i + 1] * up, t);
+                for (int c = 0; c < KC; ++c) {
+                    const float e[8] = {x0[b][c].x, x0[b][c].y, x0[b][c].z, x0[b][c].w, x1[b][c].x, x1[b][c].y, x1[b][c].z, x1[b][c].w};
 #pragma unroll
-                    for (int k = 0; k < NS; ++k) q[k][c][i] = t[k]; }
+                    for (int i = 0; i < 4; ++i) { uint32_t t[NS]; Split<BF16>::of(e[2 * i] * up, e[2 * i + 1] * up, t);
+#pragma unroll
+                        for (int k = 0; k < NS; ++k) q[b][k][c][i] = t[k]; }
+                }
             }
             while (j + TILE < j_end) step(std::true_type());
             step(std::false_type());
         }
         // the four waves' results: (m, l) through LDS, then the accumulators on the common maximum
-        l = over_rows(l, [](float p, float r) { return p + r; });
-        if (m == -INFINITY && l != l) m = 0.f;                            // (scores that are all NaN: the maximum has passed them over, the result is NaN and not a row of nothing)
-        __syncthreads();                                                  // (the previous unit's reads of s_o are done)
-        if (g == 0) { s_m[wave][col] = m; s_l[wave][col] = l; }
-        __syncthreads();
-        const float m0 = s_m[0][col], m1 = s_m[1][col], m2 = s_m[2][col], m3 = s_m[3][col], M = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)), to = M == -INFINITY ? 0.f : M;
-        const float f = __builtin_amdgcn_exp2f(m - to);                   // (0 for a wave that had nothing)
-        if (wave == 0 && g == 0) {
-            s_row[0][col] = M;
-            s_row[1][col] = (s_l[0][col] * __builtin_amdgcn_exp2f(m0 - to) + s_l[1][col] * __builtin_amdgcn_exp2f(m1 - to)) +
-                            (s_l[2][col] * __builtin_amdgcn_exp2f(m2 - to) + s_l[3][col] * __builtin_amdgcn_exp2f(m3 - to));
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+            l[b] = over_rows(l[b], [](float p, float r) { return p + r; });
+            if (m[b] == -INFINITY && l[b] != l[b]) m[b] = 0.f;            // (scores that are all NaN: the maximum has passed them over, the result is NaN and not a row of nothing)
         }
-        if (col < heads) {
-            float *so = s_o + (wave * heads + col) * (D + 4);
+        __syncthreads();                                                  // (the previous unit's reads of s_o are done)
 #pragma unroll
-            for (int hf = 0; hf < VH; ++hf)
+        for (int b = 0; b < QB; ++b) if (g == 0) { s_m[wave][QH * b + col] = m[b]; s_l[wave][QH * b + col] = l[b]; }
+        __syncthreads();
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
+        for (int b = 0; b < QB; ++b) {
+            const int h = QH * b + col;
+            const float m0 = s_m[0][h], m1 = s_m[1][h], m2 = s_m[2][h], m3 = s_m[3][h], M = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)), to = M == -INFINITY ? 0.f : M;
+            const float f = __builtin_amdgcn_exp2f(m[b] - to);            // (0 for a wave that had nothing)
+            if (wave == 0 && g == 0) {
+                s_row[0][h] = M;
+                s_row[1][h] = (s_l[0][h] * __builtin_amdgcn_exp2f(m0 - to) + s_l[1][h] * __builtin_amdgcn_exp2f(m1 - to)) +
+                              (s_l[2][h] * __builtin_amdgcn_exp2f(m2 - to) + s_l[3][h] * __builtin_amdgcn_exp2f(m3 - to));
+            }
+            if (h < heads) {
+                float *so = s_o + (wave * heads + h) * (D + 4);
 #pragma unroll
-                    for (int i = 0; i < VW; i += 4)      // element 128 hf + VW (4 g + r) + i
-                        *reinterpret_cast<f4 *>(so + 128 * hf + VW * (4 * g + r) + i) = (f4){o[hf][i][r] * f, o[hf][i + 1][r] * f, o[hf][i + 2][r] * f, o[hf][i + 3][r] * f};
+                for (int hf = 0; hf < VH; ++hf)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int i = 0; i < VW; i += 4)      // element 128 hf + VW (4 g + r) + i
+                            *reinterpret_cast<f4 *>(so + 128 * hf + VW * (4 * g + r) + i) = (f4){o[b][hf][i][r] * f, o[b][hf][i + 1][r] * f, o[b][hf][i + 2][r] * f, o[b][hf][i + 3][r] * f};
+            }
         }
         __syncthreads();
         const bool alone = ONE || ntile == tiles;
-        float *part = ONE ? nullptr : a.part + ((long)blockIdx.x * 2 + (first ? 0 : 1)) * QH * (D + 2);
+        float *part = ONE ? nullptr : a.part + ((long)blockIdx.x * 2 + (first ? 0 : 1)) * HEADS * (D + 2);
         for (int e = threadIdx.x; e < heads * D / 4; e += 256) {
             const int h = e / (D / 4), d = (e - h * (D / 4)) * 4;
             const float Mh = s_row[0][h], L = s_row[1][h];
@@ -349,18 +376,19 @@ template <int D, bool BF16, bool CAP, bool ONE> __global__ void __launch_bounds_
 // where the partial results of a query head lie: those of `count` neighbouring workgroups, the first at base + other, the next at base + step ...  A workgroup's slot 0 is its first unit,
 // slot 1 a later (its last) one: only the first of the row's workgroups can have begun with another unit.  count 1: the row is done.
 template <int D> struct RowParts {
-    static constexpr long STEP = 2l * QH * (D + 2);
-    const float *base; long other; int count, tiles;
+    const float *base; long other, step; int count, tiles;
     __device__ RowParts(const AttnArgs &a, int h, int s) {
-        const int p0 = a.prefix[s]; tiles = a.prefix[s + 1] - p0; count = 0; base = nullptr; other = 0;
+        const int p0 = a.prefix[s]; tiles = a.prefix[s + 1] - p0; count = 0; base = nullptr; other = 0; step = (2l << a.lg) * (D + 2);
         if (!tiles) return;
         const Shares shares(a.prefix[a.c.n_seq] * a.c.n_head_kv, a.n_wg);
         const int hk = h / a.group, in = h - hk * a.group, x0 = p0 * a.c.n_head_kv + hk * tiles, w0 = shares.owner(x0);
         count = shares.owner(x0 + tiles - 1) - w0 + 1;
-        base = a.part + (((long)(in / QH) * a.n_wg + w0) * 2 * QH + in % QH) * (D + 2);
-        other = shares.first(w0) < x0 ? (long)QH * (D + 2) : 0;
+        base = a.part + w0 * step + offset(a, in);
+        other = shares.first(w0) < x0 ? step / 2 : 0;
     }
-    __device__ const float *at(int i) const { return base + i * STEP + (i ? 0 : other); }
+    __device__ const float *at(int i) const { return base + i * step + (i ? 0 : other); }
+    // of head `in` of a group behind the group's first
+    static __device__ long offset(const AttnArgs &a, int in) { const int b = in >> a.lg; return (((long)b * a.n_wg * 2 << a.lg) + (in - (b << a.lg))) * (D + 2); }
 };
 // weight[slot] += sum over the group of 2^(z - (m - 8)) / l for 1024 slots of a KV head, four to a thread, the heads in order.  The rows' m and l are joined here once more, 64 heads at a
 // time, 16 lanes to a head, which is cheaper than a third launch behind the join.  Nothing branches between the loads of the scores: 8 sequences of up to 4099 slots, 71 heads on one KV head of
@@ -373,7 +401,7 @@ template <int D> static __device__ __forceinline__ void add_weights(const AttnAr
     for (int h0 = 0; h0 < a.group; h0 += 64) {
         const int heads = min(64, a.group - h0);
         auto in = [&](int q) { return h0 + min(16 * q + ((int)threadIdx.x >> 4), heads - 1); };          // the lane's q-th head
-        auto at = [&](int q, int i) { return *reinterpret_cast<const float2 *>(row.at(i) + ((long)(in(q) / QH) * a.n_wg * 2 * QH + in(q) % QH) * (D + 2)); };
+        auto at = [&](int q, int i) { return *reinterpret_cast<const float2 *>(row.at(i) + RowParts<D>::offset(a, in(q))); };
         float2 first[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) if (16 * q < heads) first[q] = row.count == 1 ? a.stat[(long)s * a.n_head + hk * a.group + in(q)] : part < row.count ? at(q, part) : make_float2(-INFINITY, 0.f);
@@ -463,7 +491,7 @@ static int attn_check(const cdna4_tensor *q, const cdna4_tensor *k_cache, const 
     ARG_CHECK(q->ne[1] % a->c.n_head_kv == 0, "paged_attn: n_head a multiple of n_head_kv");
     OP_CHECK(q->ne[1] <= 16384, "paged_attn: at most 16384 query heads");
     if (weight && (rc = pg_slots_check("paged_attn", "weight", weight, CDNA4_TYPE_F32, a->c, true))) return rc;
-    a->n_head = (int)q->ne[1]; a->group = a->n_head / a->c.n_head_kv; a->blocks = (a->group + QH - 1) / QH;
+    a->n_head = (int)q->ne[1]; a->group = a->n_head / a->c.n_head_kv; a->lg = 4; a->blocks = (a->group + QH - 1) / QH;
     const long slots = (long)a->c.W << a->c.page_shift, tiles = (slots + TILE - 1) / TILE;
     OP_CHECK(tiles * a->c.n_seq < (1l << 31) / std::max(a->c.n_head_kv * a->blocks, 1) && tiles * a->c.n_head_kv < (1l << 26), "paged_attn: too many slots in all");
     a->score_row = tiles * TILE;
@@ -506,29 +534,36 @@ int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_t
     // With weights: if a KV head is one unit and its scores fit LDS.
     const size_t one_lds = merge + (weight ? (size_t)a.group * a.score_row * 4 : 0);
     const bool one = (row_tiles * a.c.D <= 640 || (row_tiles <= 16 && (long)a.c.n_seq * n_unit >= ctx->num_cu)) && (!weight || a.group <= QH) && one_lds <= ONE_LDS;
-#define ATTN(D_, B_, C_, O_, grid, lds) do { if ((lds) > 60 * 1024) HIP_TRY((pg_opt_in_lds<paged_attn_kernel<D_, B_, C_, O_>>(ctx->device, ONE_LDS))); \
-                                             hipLaunchKernelGGL((paged_attn_kernel<D_, B_, C_, O_>), grid, dim3(256), lds, st, a); } while (0)
-#define ATTN_D(D_, O_, grid, lds) do { if (bf) { if (cap) ATTN(D_, true, true, O_, grid, lds); else ATTN(D_, true, false, O_, grid, lds); } \
-                                       else { if (cap) ATTN(D_, false, true, O_, grid, lds); else ATTN(D_, false, false, O_, grid, lds); } HIP_TRY(hipGetLastError()); } while (0)
-#define ATTN_ALL(O_, grid, lds) do { if (a.c.D == 64) ATTN_D(64, O_, grid, lds); else if (a.c.D == 128) ATTN_D(128, O_, grid, lds); else ATTN_D(256, O_, grid, lds); } while (0)
+#define ATTN(D_, B_, C_, O_, Q_, grid, lds) do { if ((lds) > 60 * 1024) HIP_TRY((pg_opt_in_lds<paged_attn_kernel<D_, B_, C_, O_, Q_>>(ctx->device, ONE_LDS))); \
+                                                 hipLaunchKernelGGL((paged_attn_kernel<D_, B_, C_, O_, Q_>), grid, dim3(256), lds, st, a); } while (0)
+#define ATTN_D(D_, O_, Q_, grid, lds) do { if (bf) { if (cap) ATTN(D_, true, true, O_, Q_, grid, lds); else ATTN(D_, true, false, O_, Q_, grid, lds); } \
+                                           else { if (cap) ATTN(D_, false, true, O_, Q_, grid, lds); else ATTN(D_, false, false, O_, Q_, grid, lds); } HIP_TRY(hipGetLastError()); } while (0)
+#define ATTN_ALL(O_, grid, lds) do { if (a.c.D == 64) ATTN_D(64, O_, 1, grid, lds); else if (a.c.D == 128) ATTN_D(128, O_, 1, grid, lds); else ATTN_D(256, O_, 1, grid, lds); } while (0)
     if (one) {
         a.n_wg = 0; a.prefix = nullptr; a.part = nullptr; a.stat = nullptr; a.score = nullptr;
         ATTN_ALL(true, dim3((unsigned)n_unit, (unsigned)a.c.n_seq), one_lds);
         return CDNA4_OK;
     }
-    // Blocks of 16 heads that share a KV head read the same tiles at the same time: workgroups that are a multiple of 8 apart share an XCD and its L2, so much of the cache comes from memory
-    // once.  us with a numbering of all blocks one after the other / with this one (f16; sequences x slots, heads on KV heads): 64 x 8192, 32 on 1 of 128: 54.5 / 51.4, 160 on 8: 382 / 374;
-    // 1 x 130000, 20 on 1 of 256: 50.4 / 43.5, 80 on 4 of 64: 46.6 / 37.8; bf16, 128 on 1 of 128: 80.8 / 51.8.  (Registers leave two waves to a SIMD, so with every block the loads under way
-    // are of fewer different rows: 3 TB/s of them.)
-    long most_wg = std::min<long>((long)ctx->num_cu * (a.c.D == 256 ? 1 : 2), ATTN_MAX_WG) / a.blocks;          // (blocks: at most 1024, so blocks * n_wg is at most ATTN_MAX_WG)
+    // Groups of 17 to 32 heads over much cache: 32 heads to a wave, so that it is read once (heads of 64 and 128; for 256 there are not registers enough).  Two of those waves' registers do
+    // not fit a SIMD (heads of 128), so each of its steps is in the open: with fewer tiles than 16 to a CU, or rows of which the ends count, two blocks of 16 are faster.  us with blocks
+    // of 16 / 32 to a wave (f16, 20 heads a KV head; sequences x slots, KV heads): of 128: 64 x 8192, 8: 373 / 261, 32 x 8192, 4: 93 / 73, 64 x 8192, 1 (32 heads): 51.6 / 44.3, 16 x 4099, 8:
+    // 49.6 / 55.2, 4: 27.6 / 28.6, 1 x 3000, 1: 11.9 / 13.7; of 64: 64 x 8192, 8: 156 / 136, 16 x 4099, 8: 32.7 / 27.6, 1 x 130000, 4: 38.5 / 35.2, 1 (bf16): 18.8 / 20.6.
+    // Larger groups (and the others): blocks of 16 heads that read the same tiles at the same time: workgroups that are a multiple of 8 apart share an XCD and its L2, so much of the cache
+    // comes from memory once.  us with a numbering of all blocks one after the other / with this one: 64 x 8192, 32 on 1 of 128: 54.5 / 51.4, 1 x 130000, 20 on 1 of 256: 50.4 / 43.5; bf16,
+    // 128 on 1 of 128: 80.8 / 51.8; 48 on 1 of 128, 64 x 8192: 100 (32 to a wave: 121).
+    const bool two = a.group > QH && a.group <= 2 * QH && a.c.D <= 128 && tiles >= 16l * ctx->num_cu && row_tiles * TILE >= 64 * a.c.D;
+    if (two) { a.lg = 5; a.blocks = 1; }
+    const int qb = two ? 2 : 1, per_cu = a.c.D == 256 || (a.c.D == 128 && two) ? 1 : 2;          // (what the registers allow)
+    long most_wg = std::min<long>((long)ctx->num_cu * per_cu, ATTN_MAX_WG / qb) / a.blocks;       // (blocks: at most 1024)
     if (a.blocks > 1 && most_wg > 8) most_wg &= ~7l;
     a.n_wg = (int)std::max<long>(1, std::min(tiles, most_wg));
-    const AttnScratch sc = attn_scratch(a, weight != nullptr, a.n_wg * a.blocks);
+    const AttnScratch sc = attn_scratch(a, weight != nullptr, a.n_wg * a.blocks * qb);
     if ((rc = cdna4_ensure_ws(ctx, sc.total, st))) return rc;
     char *ws = (char *)ctx->ws;
     a.prefix = (int *)ws; a.part = (float *)(ws + sc.part); a.stat = weight ? (float2 *)(ws + sc.stat) : nullptr; a.score = weight ? (float *)(ws + sc.score) : nullptr;
-    const size_t lds = (size_t)((a.c.n_seq + 4) & ~3) * 4 + merge;          // (at most (8192 + 4) * 4 + 4 * 16 * 260 * 4 bytes)
-    ATTN_ALL(false, dim3((unsigned)(a.n_wg * a.blocks)), lds);
+    const size_t lds = (size_t)((a.c.n_seq + 4) & ~3) * 4 + (size_t)WAVES * std::min(QH * qb, a.group) * (a.c.D + 4) * 4;          // (at most (8192 + 4) * 4 + 4 * 32 * 132 * 4 bytes)
+    const dim3 grid((unsigned)(a.n_wg * a.blocks));
+    if (!two) ATTN_ALL(false, grid, lds); else if (a.c.D == 64) ATTN_D(64, false, 2, grid, lds); else ATTN_D(128, false, 2, grid, lds);
     const dim3 join((unsigned)(a.n_head + (weight ? a.c.n_head_kv * ((a.score_row + 1023) / 1024) : 0)), (unsigned)a.c.n_seq);
 #define JOIN(D_) do { if (weight) hipLaunchKernelGGL((paged_attn_join_kernel<D_, true>), join, dim3(256), 0, st, a); \
                       else hipLaunchKernelGGL((paged_attn_join_kernel<D_, false>), join, dim3(256), 0, st, a); } while (0)

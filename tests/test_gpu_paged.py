@@ -99,6 +99,20 @@ def test_attn_large_groups_over_long_tables(D, heads_kv, heads, dtype, weights, 
     check_attn(backend, c, heads, weight=c.slots() if weights else None, softcap=20.0 if D == 256 else 0.0)
 
 
+@pytest.mark.parametrize("D,heads_kv,heads,n_seq,dtype", [(64, 2, 40, 80, torch.float16), (64, 1, 32, 140, torch.bfloat16), (128, 1, 17, 66, torch.bfloat16), (128, 2, 62, 40, torch.float16), (128, 1, 31, 70, torch.float16)])
+@pytest.mark.parametrize("weights", [False, True])
+def test_attn_two_blocks_of_heads_to_a_wave(D, heads_kv, heads, n_seq, dtype, weights, backend):
+    """groups of 17 to 32 heads and tables of many slots, of which few are in use"""
+    W = 64 * D // 64 + 1
+    r = np.random.default_rng(heads)
+    lens = [int(x) for x in r.integers(0, 300, n_seq)]; lens[3] = 2100; lens[7] = 0; lens[8] = -1
+    c = Case([max(n, 0) for n in lens], D=D, heads_kv=heads_kv, page=64, dtype=dtype, seed=heads)
+    c.n_kv = np.array(lens, np.int32)
+    c.table = np.concatenate([c.table, np.full((n_seq, W - c.W), c.n_pages, np.int32)], axis=1); c.W = W          # (wider tables: nothing behind the lengths is mapped)
+    c.table[5, 0] = -1
+    check_attn(backend, c, heads, weight=c.slots() if weights else None, softcap=25.0 if D == 64 else 0.0)
+
+
 @pytest.mark.parametrize("heads_kv,heads", [(1, 1), (2, 2), (8, 8), (2, 6), (1, 8), (2, 14), (1, 16), (1, 17), (2, 40), (1, 71), (3, 12)])
 @pytest.mark.parametrize("weights", [False, True])
 def test_attn_groups(heads_kv, heads, weights, backend):
