@@ -8,6 +8,8 @@
 //   (16 bytes a lane, a row per 16 lanes) and becomes the other operand by v_perm, so the loop touches no LDS at all.
 // * f32 results from 16-bit operands: q and p are split into two f16 (2^-22; q scaled by a power of two, p by 2^8) or three bf16 (exactly 24 bits) terms, K and V are what the cache
 //   holds; products and sums are f32.  The extra matrix instructions stay far below the load time (32 or 48 of 16 clk per 16 KB and SIMD).
+// * Sums that finite values cannot take out of range: every step of 32 slots is summed on its own maximum and added to accumulators whose weights sum to at most 1, and partial rows are
+//   divided by their own sums before they are joined (bf16 values go up to the largest f32).
 // * Equal shares: all tiles of 128 slots of all (sequence, KV head) pairs are numbered through, and every workgroup takes an equal contiguous range of the numbers, from the lengths as
 //   they are on the device.  Groups of more than 16 query heads: 32 to a wave, or blocks of 16 with workgroups of their own and the same ranges.  A long sequence in a batch of short ones spreads over the chip by itself; a workgroup that covers a unit alone writes its result, the others
 //   leave (max, sum, accumulator) for the join.
@@ -33,8 +35,8 @@ struct AttnArgs {
     PagedCache c; const char *q; long q_head, q_seq; char *dst; long d_head, d_seq; char *weight; long w_head, w_seq;
     int group, n_head, lg, blocks, n_wg; float scale, softcap, inv_softcap;      // blocks: of 2^lg query heads in a group; n_wg: workgroups that share the tiles of one block of every group
     int *prefix;                // [n_seq + 1] tiles of a unit before sequence s
-    float *part;                // [blocks][n_wg][2][2^lg][D + 2]: what a workgroup leaves of its first / last unit (max, sum, accumulator of every head)
-    float2 *stat;               // [n_seq][n_head] max and sum of a row (weight only)
+    float *part;                // [blocks][n_wg][2][2^lg][D + 2]: what a workgroup leaves of its first / last unit (reference, sum, row divided by the sum of every head)
+    float2 *stat;               // [n_seq][n_head] reference and sum of a row (weight only)
     float *score; long score_row;   // [n_seq][n_head][score_row] scores in units of log 2 (weight only)
 };
 
@@ -111,6 +113,7 @@ struct Shares {
 // QB: blocks of 16 query heads that a wave takes.
 template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch_bounds__(256) paged_attn_kernel(AttnArgs a) {
     constexpr int HEADS = QB * QH, KC = D / 32, VW = D == 64 ? 4 : 8, VH = D == 256 ? 2 : 1, NS = Split<BF16>::N;      // K chunks of 32 elements; V elements of a lane and half; halves of 128
+    constexpr float P_SCALE = BF16 ? 1.0f / 32.0f : 256.0f;          // of a step's probabilities: 32 of 2^-5 sum to 1 in bf16
     extern __shared__ int s_mem[];
     __shared__ int s_tot[4]; __shared__ float s_m[WAVES][HEADS], s_l[WAVES][HEADS], s_row[2][HEADS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
@@ -182,10 +185,11 @@ template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch
                     }
             }
         };
-        f4 o[QB][VH][VW]; float m[QB], l[QB];
+        // o / l: the wave's sums of 2^(z - m) v and 2^(z - m); `held` of a head bounds the sum of 2^(z - m) over all its slots so far and stays at most 1 (see step)
+        f4 o[QB][VH][VW]; float m[QB], l[QB], held[QB];
 #pragma unroll
         for (int b = 0; b < QB; ++b) {
-            m[b] = -INFINITY; l[b] = 0.f;
+            m[b] = -INFINITY; l[b] = 0.f; held[b] = 0.f;
 #pragma unroll
             for (int hf = 0; hf < VH; ++hf)
 #pragma unroll
@@ -212,7 +216,7 @@ template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch
             const int jn = j + TILE; int e0 = 0, e1 = 0;
             if constexpr (MORE) { load_k(jn, nx0, nx1); e0 = entry(jn + TILE); e1 = entry(jn + TILE + 16); }
             const bool whole = id0 >= 0 && id1 >= 0 && j + 32 <= n;          // (wave-uniform)
-            uint32_t p[QB][NS][4];
+            uint32_t p[QB][NS][4]; float over[QB];
 #pragma unroll
             for (int b = 0; b < QB; ++b) {
 #pragma unroll
@@ -244,26 +248,32 @@ template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch
                 }
                 float top = fmaxf(fmaxf(fmaxf(z[b][0][0], z[b][0][1]), fmaxf(z[b][0][2], z[b][0][3])), fmaxf(fmaxf(z[b][1][0], z[b][1][1]), fmaxf(z[b][1][2], z[b][1][3])));
                 top = over_rows(top, [](float p, float r) { return fmaxf(p, r); });
-                // the reference value of the exponentials follows the maximum only when that has grown by 2^6: 2^8 p stays below 2^14 in f16
-                if (__ballot(top > m[b] + 6.0f)) {
-                    const float to = fmaxf(m[b], top), f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[b] - to);
-                    m[b] = to; l[b] *= f;
+                // A step's own maximum is the reference of its probabilities: their terms are as exact in every step, and f carries their sums over to the reference m of o and l.  m is not
+                // the maximum: it is raised (by 2^3 more than needed: a logarithmic number of times) where 2^top for each of the 32 slots would take `held` past 1.  A sum of 2^(z - m) v
+                // is then no larger than the largest |v|: bf16 values may be as large as f32's.
+                float f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - m[b]) * 32.0f;
+                if (__ballot(!(held[b] + f <= 1.0f))) {
+                    const float to = held[b] + f <= 1.0f ? m[b] : fmaxf(m[b], top + 5.0f) + 3.0f, down = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[b] - to);
+                    m[b] = to; l[b] *= down; held[b] *= down; f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - to) * 32.0f;
 #pragma unroll
                     for (int hf = 0; hf < VH; ++hf)
 #pragma unroll
-                        for (int i = 0; i < VW; ++i) o[b][hf][i] *= f;
+                        for (int i = 0; i < VW; ++i) o[b][hf][i] *= down;
                 }
-                const float ref = m[b] == -INFINITY ? 0.f : m[b] - 8.0f;
+                held[b] += f; over[b] = f * (1.0f / (32.0f * P_SCALE));
+                const float ref = top == -INFINITY ? 0.f : top;
+                float sum = 0.f;
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; r += 2) {
-                        const float p0 = __builtin_amdgcn_exp2f(z[b][t][r] - ref), p1 = __builtin_amdgcn_exp2f(z[b][t][r + 1] - ref);
-                        l[b] += p0 + p1;
+                        const float p0 = __builtin_amdgcn_exp2f(z[b][t][r] - ref) * P_SCALE, p1 = __builtin_amdgcn_exp2f(z[b][t][r + 1] - ref) * P_SCALE;
+                        sum += p0 + p1;
                         uint32_t w[NS]; Split<BF16>::of(p0, p1, w);
 #pragma unroll
                         for (int k = 0; k < NS; ++k) p[b][k][2 * t + r / 2] = w[k];
                     }
+                l[b] = fmaf(over[b], sum, l[b]);
             }
 #pragma unroll
             for (int hf = 0; hf < VH; ++hf)
@@ -274,9 +284,12 @@ template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch
 #pragma unroll
                     for (int w = 0; w < 4; ++w) vt[w] = __builtin_amdgcn_perm(vr[2 * w + 1][hf][i / 2], vr[2 * w][hf][i / 2], sel);
 #pragma unroll
-                    for (int b = 0; b < QB; ++b)
+                    for (int b = 0; b < QB; ++b) {
+                        f4 sum = (f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int k = NS - 1; k >= 0; --k) o[b][hf][i] = mfma<BF16>(vt, (u4){p[b][k][0], p[b][k][1], p[b][k][2], p[b][k][3]}, o[b][hf][i]);
+                        for (int k = NS - 1; k >= 0; --k) sum = mfma<BF16>(vt, (u4){p[b][k][0], p[b][k][1], p[b][k][2], p[b][k][3]}, sum);
+                        o[b][hf][i] += over[b] * sum;
+                    }
                 }
             if constexpr (MORE) { load_v(jn, nx0, nx1); id0 = nx0; id1 = nx1; nx0 = id_of(e0, jn + TILE); nx1 = id_of(e1, jn + TILE + 16); j = jn; }
         };
@@ -324,12 +337,10 @@ template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch
         for (int b = 0; b < QB; ++b) {
             const int h = QH * b + col;
             const float m0 = s_m[0][h], m1 = s_m[1][h], m2 = s_m[2][h], m3 = s_m[3][h], M = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)), to = M == -INFINITY ? 0.f : M;
-            const float f = __builtin_amdgcn_exp2f(m[b] - to);            // (0 for a wave that had nothing)
-            if (wave == 0 && g == 0) {
-                s_row[0][h] = M;
-                s_row[1][h] = (s_l[0][h] * __builtin_amdgcn_exp2f(m0 - to) + s_l[1][h] * __builtin_amdgcn_exp2f(m1 - to)) +
-                              (s_l[2][h] * __builtin_amdgcn_exp2f(m2 - to) + s_l[3][h] * __builtin_amdgcn_exp2f(m3 - to));
-            }
+            const float L = (s_l[0][h] * __builtin_amdgcn_exp2f(m0 - to) + s_l[1][h] * __builtin_amdgcn_exp2f(m1 - to)) +          // (0 for a wave that had nothing)
+                            (s_l[2][h] * __builtin_amdgcn_exp2f(m2 - to) + s_l[3][h] * __builtin_amdgcn_exp2f(m3 - to));
+            const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[b] - to) / L;            // (the rows are divided before they are added: see held)
+            if (wave == 0 && g == 0) { s_row[0][h] = M; s_row[1][h] = L; }
             if (h < heads) {
                 float *so = s_o + (wave * heads + h) * (D + 4);
 #pragma unroll
@@ -350,7 +361,6 @@ template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch
             const float *so = s_o + h * (D + 4) + d; const int next = heads * (D + 4);
             f4 v = (*reinterpret_cast<const f4 *>(so) + *reinterpret_cast<const f4 *>(so + next)) + (*reinterpret_cast<const f4 *>(so + 2 * next) + *reinterpret_cast<const f4 *>(so + 3 * next));
             if (alone) {
-                if (Mh == -INFINITY) v = (f4){0.f, 0.f, 0.f, 0.f}; else v /= L;          // (nothing to attend to: a row of zeros)
                 *reinterpret_cast<f4 *>(a.dst + (long)s * a.d_seq + (long)(h0 + h) * a.d_head + d * 4) = v;
                 if (!ONE && d == 0 && a.stat) a.stat[(long)s * a.n_head + h0 + h] = make_float2(Mh, L);
             } else {
@@ -366,7 +376,7 @@ template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch
                 float sum = 0.f;
                 for (int h = 0; h < heads; ++h) {
                     const float zi = z[h * (int)a.score_row + i];          // -inf: not attended to, whatever the row is
-                    if (zi != -INFINITY) sum += __builtin_amdgcn_exp2f(zi - (s_row[0][h] - 8.0f)) / s_row[1][h];
+                    if (zi != -INFINITY) sum += __builtin_amdgcn_exp2f(zi - s_row[0][h]) / s_row[1][h];
                 }
                 if (sum != 0.f) w[i] += sum;
             }
@@ -390,7 +400,7 @@ template <int D> struct RowParts {
     // of head `in` of a group behind the group's first
     static __device__ long offset(const AttnArgs &a, int in) { const int b = in >> a.lg; return (((long)b * a.n_wg * 2 << a.lg) + (in - (b << a.lg))) * (D + 2); }
 };
-// weight[slot] += sum over the group of 2^(z - (m - 8)) / l for 1024 slots of a KV head, four to a thread, the heads in order.  The rows' m and l are joined here once more, 64 heads at a
+// weight[slot] += sum over the group of 2^(z - m) / l for 1024 slots of a KV head, four to a thread, the heads in order.  The rows' m and l are joined here once more, 64 heads at a
 // time, 16 lanes to a head, which is cheaper than a third launch behind the join.  Nothing branches between the loads of the scores: 8 sequences of up to 4099 slots, 71 heads on one KV head of
 // 64: 38 us with a branch per head and 16 heads at a time, 17 us so.
 template <int D> static __device__ __forceinline__ void add_weights(const AttnArgs &a, int hk, int s, int chunk, float2 *s_row) {
@@ -431,7 +441,7 @@ template <int D> static __device__ __forceinline__ void add_weights(const AttnAr
             for (int i = 0; i < heads; ++i) {
                 const float2 st = s_row[i]; const f4 z = *reinterpret_cast<const f4 *>(z0 + i * a.score_row);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { const float p = __builtin_amdgcn_exp2f(z[e] - (st.x - 8.0f)) * st.y; sum[e] += z[e] != -INFINITY ? p : 0.0f; }          // (-inf: not attended to, whatever the row is)
+                for (int e = 0; e < 4; ++e) { const float p = __builtin_amdgcn_exp2f(z[e] - st.x) * st.y; sum[e] += z[e] != -INFINITY ? p : 0.0f; }          // (-inf: not attended to, whatever the row is)
             }
         }
     }
@@ -458,18 +468,19 @@ template <int D, bool WEIGHT> __global__ void __launch_bounds__(256) paged_attn_
     __syncthreads();
     M = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
     float L = 0.f;
-    for (int i = tid; i < count; i += 256) { const float m = s_f[i], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M); s_f[i] = f; L += f * part.at(i)[1]; }
+    for (int i = tid; i < count; i += 256) { const float m = s_f[i], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M) * part.at(i)[1]; s_f[i] = f; L += f; }
     L = wave_sum_dpp(L);
     if (lane == 0) s_red[4 + wave] = L;
     __syncthreads();
     L = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
+    const float share = M == -INFINITY ? 0.f : 1.0f / L;          // (nothing to attend to: a row of zeros)
     constexpr int TD = D / 4, ROWS = 256 / TD;
     const int d = (tid % TD) * 4, row = tid / TD;
     f4 v = (f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int i = row; i < count; i += ROWS) {
         const float *p = part.at(i) + 2 + d; const float2 lo = *reinterpret_cast<const float2 *>(p), hi = *reinterpret_cast<const float2 *>(p + 2);
-        const float f = s_f[i];
+        const float f = s_f[i] * share;          // the partial rows are divided by their own sums: what is added here is no larger than the largest value
         v[0] += lo.x * f; v[1] += lo.y * f; v[2] += hi.x * f; v[3] += hi.y * f;
     }
     s_v[tid] = v;
@@ -477,7 +488,6 @@ template <int D, bool WEIGHT> __global__ void __launch_bounds__(256) paged_attn_
     if (row) return;
 #pragma unroll
     for (int r = 1; r < ROWS; ++r) v += s_v[r * TD + tid];
-    if (M == -INFINITY) v = (f4){0.f, 0.f, 0.f, 0.f}; else v /= L;
     *reinterpret_cast<f4 *>(out + d) = v;
 }
 static int attn_check(const cdna4_tensor *q, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const cdna4_tensor *weight, const cdna4_tensor *dst, AttnArgs *a) {
