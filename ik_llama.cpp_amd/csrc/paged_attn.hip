@@ -6,8 +6,11 @@
 // * Matrix instructions, for any group size: 32 slots are one step of v_mfma_f32_16x16x32.  S^T = K Q^T puts a query head into every lane column and four slots into every lane, which is
 //   the operand layout that O^T = V^T P^T wants for P: the probabilities never leave their registers, and the running maximum and sum of a head are scalars of a lane.  V arrives as rows
 //   (16 bytes a lane, a row per 16 lanes) and becomes the other operand by v_perm, so the loop touches no LDS at all.
-// * f32 results from 16-bit operands: q and p are split into two f16 (2^-22; q scaled by a power of two, p by 2^8) or three bf16 (exactly 24 bits) terms, K and V are what the cache
-//   holds; products and sums are f32.  The extra matrix instructions stay far below the load time (32 or 48 of 16 clk per 16 KB and SIMD).
+// * f32 results from 16-bit operands: q and p are split into two f16 terms or three bf16 ones, K and V are what the cache holds; products and sums are f32.  bf16: exactly 24 bits.  f16: 22
+//   bits, rounded to nearest, down to 2^-28 of a row's largest element or a step's largest probability, the products of the second terms summed apart and scaled (a third term would change
+//   no result: the scores' own rounding is larger.  Root mean square error beside elementary 32-bit torch, scores of about 6, heads of 128: 2.3e-7 / 5.3e-7).  Without the scale the second
+//   terms ended at 2^-32 of the row's maximum: 8192 slots behind one that takes all but 10^-3 of the weight were off by 10^-5.  The extra matrix instructions stay far below the load time
+//   (32 or 48 of 16 clk per 16 KB and SIMD).
 // * Sums that finite values cannot take out of range: every step of 32 slots is summed on its own maximum and added to accumulators whose weights sum to at most 1, and partial rows are
 //   divided by their own sums before they are joined (bf16 values go up to the largest f32).
 // * Equal shares: all tiles of 128 slots of all (sequence, KV head) pairs are numbered through, and every workgroup takes an equal contiguous range of the numbers, from the lengths as
@@ -55,10 +58,12 @@ template <typename F> static __device__ __forceinline__ float over_rows(float v,
 template <bool BF16> struct Split;
 template <> struct Split<false> {
     static constexpr int N = 2;
+    static constexpr float UP = 4096.0f;          // the second term is the rounding error of the first times 2^12, in products of its own: for values up to 2^15 it is as far from overflow as
+                                                  // they are and keeps its 11 bits where the first keeps them (both down to 2^-14)
     static __device__ __forceinline__ void of(float a, float b, uint32_t (&t)[2]) {
-        t[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));          // towards zero: the remainders are exact and of the values' sign
-        const float ra = a - half_bits_to_float(t[0] & 0xffffu), rb = b - half_bits_to_float(t[0] >> 16);
-        t[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        const h2 first = {(_Float16)a, (_Float16)b}, rest = {(_Float16)((a - (float)first[0]) * UP), (_Float16)((b - (float)first[1]) * UP)};
+        t[0] = __builtin_bit_cast(uint32_t, first); t[1] = __builtin_bit_cast(uint32_t, rest);
     }
 };
 template <> struct Split<true> {
@@ -111,9 +116,10 @@ struct Shares {
 
 // ONE: a workgroup per unit (grid: units, sequences), for tables of few slots: no shares, nothing to join, and the weights are added from scores in LDS by the same launch.
 // QB: blocks of 16 query heads that a wave takes.
-template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch_bounds__(256) paged_attn_kernel(AttnArgs a) {
+// (Two waves a SIMD, 256 registers, wherever that is enough: with more the compiler puts a step's products into accumulation registers and moves every one of them out: 80 of 1300 instructions.)
+template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch_bounds__(256, (D * QB <= 128 ? 2 : 1)) paged_attn_kernel(AttnArgs a) {
     constexpr int HEADS = QB * QH, KC = D / 32, VW = D == 64 ? 4 : 8, VH = D == 256 ? 2 : 1, NS = Split<BF16>::N;      // K chunks of 32 elements; V elements of a lane and half; halves of 128
-    constexpr float P_SCALE = BF16 ? 1.0f / 32.0f : 256.0f;          // of a step's probabilities: 32 of 2^-5 sum to 1 in bf16
+    constexpr float P_SCALE = BF16 ? 1.0f / 32.0f : 32768.0f;          // of a step's probabilities: 32 of 2^-5 sum to 1 in bf16; f16 keeps the bits of those down to 2^-29 of the largest
     extern __shared__ int s_mem[];
     __shared__ int s_tot[4]; __shared__ float s_m[WAVES][HEADS], s_l[WAVES][HEADS], s_row[2][HEADS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
@@ -202,16 +208,19 @@ template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch
         // condition around the loads: behind a condition the compiler waits for V of the next tile before the first product of K.)
         auto step = [&](auto more) {
             constexpr bool MORE = decltype(more)::value;
-            f4 z[QB][2];
+            f4 z[QB][2], low[QB][2];          // (low: the products of the second f16 terms)
 #pragma unroll
             for (int b = 0; b < QB; ++b)
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    z[b][t] = (f4){0.f, 0.f, 0.f, 0.f};
+                    z[b][t] = low[b][t] = (f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int c = 0; c < KC; ++c)
+                    for (int c = 0; c < KC; ++c) {
+                        if constexpr (BF16) {
 #pragma unroll
-                        for (int k = NS - 1; k >= 0; --k) z[b][t] = mfma<BF16>(kr[t][c], q[b][k][c], z[b][t]);
+                            for (int k = NS - 1; k >= 0; --k) z[b][t] = mfma<BF16>(kr[t][c], q[b][k][c], z[b][t]);
+                        } else { z[b][t] = mfma<BF16>(kr[t][c], q[b][0][c], z[b][t]); low[b][t] = mfma<BF16>(kr[t][c], q[b][1][c], low[b][t]); }
+                    }
                 }
             const int jn = j + TILE; int e0 = 0, e1 = 0;
             if constexpr (MORE) { load_k(jn, nx0, nx1); e0 = entry(jn + TILE); e1 = entry(jn + TILE + 16); }
@@ -223,6 +232,7 @@ template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
+                        if constexpr (!BF16) z[b][t][r] = fmaf(low[b][t][r], 1.0f / Split<false>::UP, z[b][t][r]);
                         float v = z[b][t][r] * unscale[b];
                         if constexpr (CAP) v = a.softcap * 1.44269504088896341f * tanh_of(v * a.inv_softcap);
                         z[b][t][r] = v;
@@ -285,10 +295,10 @@ template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch
                     for (int w = 0; w < 4; ++w) vt[w] = __builtin_amdgcn_perm(vr[2 * w + 1][hf][i / 2], vr[2 * w][hf][i / 2], sel);
 #pragma unroll
                     for (int b = 0; b < QB; ++b) {
-                        f4 sum = (f4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int k = NS - 1; k >= 0; --k) sum = mfma<BF16>(vt, (u4){p[b][k][0], p[b][k][1], p[b][k][2], p[b][k][3]}, sum);
-                        o[b][hf][i] += over[b] * sum;
+                        auto product = [&](int k, f4 c) { return mfma<BF16>(vt, (u4){p[b][k][0], p[b][k][1], p[b][k][2], p[b][k][3]}, c); };
+                        const f4 zero = (f4){0.f, 0.f, 0.f, 0.f};
+                        if constexpr (BF16) o[b][hf][i] += over[b] * product(0, product(1, product(NS - 1, zero)));
+                        else o[b][hf][i] += over[b] * product(0, zero) + (over[b] * (1.0f / Split<false>::UP)) * product(1, zero);
                     }
                 }
             if constexpr (MORE) { load_v(jn, nx0, nx1); id0 = nx0; id1 = nx1; nx0 = id_of(e0, jn + TILE); nx1 = id_of(e1, jn + TILE + 16); j = jn; }
@@ -302,14 +312,14 @@ template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch
 #pragma unroll
             for (int b = 0; b < QB; ++b) {
                 float up = 1.0f; unscale[b] = pre_scale;
-                if constexpr (!BF16) {          // a power of two that puts the largest element into [2^10, 2^11): the f16 terms neither overflow nor lose bits to the smallest exponent
+                if constexpr (!BF16) {          // a power of two that puts the largest element into [2^14, 2^15): the f16 terms do not overflow, and elements down to 2^-28 of the largest keep their bits
                     float top = 0.f;
 #pragma unroll
                     for (int c = 0; c < KC; ++c) top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(x0[b][c].x), fabsf(x0[b][c].y)), fmaxf(fabsf(x0[b][c].z), fabsf(x0[b][c].w))),
                                                                        fmaxf(fmaxf(fabsf(x1[b][c].x), fabsf(x1[b][c].y)), fmaxf(fabsf(x1[b][c].z), fabsf(x1[b][c].w)))));
                     top = over_rows(top, [](float p, float r) { return fmaxf(p, r); });
                     const int e = top > 0.f ? min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100), 127) : 0;
-                    up = __uint_as_float((uint32_t)(127 + 10 - e) << 23); unscale[b] = __uint_as_float((uint32_t)(127 - 10 + e) << 23) * pre_scale;
+                    up = __uint_as_float((uint32_t)(127 + 14 - e) << 23); unscale[b] = __uint_as_float((uint32_t)(127 - 14 + e) << 23) * pre_scale;
                 }
 #pragma unroll
                 for (int c = 0; c < KC; ++c) {

@@ -88,6 +88,35 @@ def test_long_rows_are_as_close_as_32_bits(softcap, dtype, backend):
     check(backend, c, 8, queries(c, 8, 1.5), softcap=softcap, weights=True)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,n", [(64, 300), (128, 2048), (128, 8192), (256, 3000)])
+@pytest.mark.parametrize("share", [0.9, 0.999, 0.999999])
+def test_a_sink_of_no_value_leaves_the_others_their_digits(share, D, n, dtype, backend):
+    """one slot takes nearly all the weight and its value is zero: the rest is the sum of many small probabilities.  All of a row's elements share the error of the sink's score (16 to 32 in
+    units of log 2: up to four half steps of 2^-20, 2^-19 of the row): with values of both signs that is |sum p v| / sum p |v| ~ 1.25 / sqrt(n) of it"""
+    c = Case([n], D=D, heads_kv=2, dtype=dtype, page=16, seed=n)
+    q = queries(c, 4, 1.0)
+    at = int(c.table[0, 0])
+    for h in range(2):          # the first slot's key along the first of the head's two queries, as long as that share needs
+        d = q[0, 2 * h].astype(np.float64); z = np.log(share / (1 - share) * n)
+        c.k[at, h, 0] = g((d / (d @ d) * z * D ** 0.5).astype(np.float32)).to(dtype)
+        q[0, 2 * h + 1] = q[0, 2 * h] * np.float32(1.01)
+    c.v[at, :, 0] = 0.0
+    check(backend, c, 4, q, extra=2.0 ** -19 * 1.25 / n ** 0.5)
+    c.v[:] = 1.0; c.v[at, :, 0] = 0.0          # all others alike: what is always rounded one way adds up
+    check(backend, c, 4, q, extra=2.0 ** -19)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [200, 3000])
+def test_a_large_element_that_meets_zeros_leaves_the_others_their_digits(n, dtype, backend):
+    """a query with one very large element where all keys are zero"""
+    c = Case([n, 7], heads_kv=1, dtype=dtype, page=16, seed=n)
+    c.k[:, :, :, 5] = 0.0
+    q = queries(c, 4, 3.0); q[:, :, 5] = 1e7
+    check(backend, c, 4, q, weights=True)
+
+
 @pytest.mark.parametrize("form", ["unit", "shared", "blocks", "two"])
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("weights", [False, True])
