@@ -2,7 +2,8 @@
 //
 // The logits are read once (4 bytes a candidate against a handful of operations: bound by that read).  A workgroup takes 8192 (2048) neighbouring logits of a row into registers and leaves
 // their maximum, the sum of their exponentials and their n_out best, sorted; a second launch joins a group's chunks: log sum exp of every beam, then the best of the sorted lists.
-// Measured: 256 rows of 128256 (131 MB), 32 groups of 8, 16 results: 24 us for the chunks (5.5 TB/s) and 9 us for the join; 4 rows of 32000: 4.1 and 4.9 us.
+// The exponentials and their sums are 64 bits wide: candidates of different beams are ordered by values in which those sums stand, and 32 bits mixed up what differs by less than 10^-6
+// (32 bits took 35.3 us for 256 rows of 128256, 131 MB, 32 groups of 8, 16 results; so it takes 47.8).
 //
 // Choosing the k best of many without sorting them: in a total order without ties, the k-th best of the threads' (or lanes' quads') own best elements is a bound that at least k elements
 // reach, and every element that reaches it belongs to one of the k owners whose best does -- so the collected list is never longer than k shares, whatever the values, and in random order
@@ -15,10 +16,11 @@ typedef unsigned long long u64;
 constexpr int BEAM_MAX_OUT = 64, BEAM_MAX_BEAMS = 256, BEAM_CHUNK = 8192; constexpr long BEAM_MAX_CANDS = 1l << 26;
 constexpr int BEAM_MAX_LISTS = (int)(BEAM_MAX_CANDS / BEAM_CHUNK) + BEAM_MAX_BEAMS;
 
+struct BeamStat { double sum; float top; };
 struct BeamArgs {
     const char *logits; long row; const float *score; const int *done; int n_beam, n_out, pad, n_vocab, chunk, chunks;          // chunk: logits of a workgroup
     float *score_out; int *parent, *token;
-    float2 *stat; u64 *best;            // [rows][chunks] maximum and sum of exponentials; [rows][chunks][n_out] sorted keys (0: none)
+    struct BeamStat *stat; u64 *best;   // [rows][chunks] maximum and sum of exponentials; [rows][chunks][n_out] sorted keys (0: none)
 };
 // (logit descending, token ascending) as one number; NaN counts as -inf, both zeros are one
 static __device__ __forceinline__ u64 logit_key(float x, int t) {
@@ -32,6 +34,16 @@ static __device__ __forceinline__ u64 shfl_max(u64 k, int d) {
     const u64 o = ((u64)(uint32_t)__shfl_xor((int)(k >> 32), d, 64) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)k, d, 64);
     return o > k ? o : k;
 }
+// e^x of a difference of two f32 values, x <= 0, in 64 bits: 2^(k / 16) from a table of 16 in LDS (one bank pair each) with k >> 4 added to the exponent, times the Taylor polynomial of
+// 2^(r / 16), |r| <= 1/2, up to the fifth power (remainder (ln 2 / 32)^6 / 720 = 1.4 * 10^-13).  x below -700 counts as -700 (10^-304); NaN too, so the caller looks for those.
+static __device__ __forceinline__ double exp_below(double x, const double *pow16) {
+    constexpr double SCALE = 23.083120654223414, WHOLE = 6755399441055744.0, C = 0.043321698784996585;          // 16 / ln 2; 1.5 * 2^52 (adding it rounds to whole numbers, into the low bits); ln 2 / 16
+    x = __builtin_fmax(x, -700.0);
+    const double y = fma(x, SCALE, WHOLE), r = fma(x, SCALE, WHOLE - y);
+    const int k = (int)(uint32_t)__builtin_bit_cast(u64, y);
+    const double p = fma(r, fma(r, fma(r, fma(r, fma(r, C * C * C * C * C / 120, C * C * C * C / 24), C * C * C / 6), C * C / 2), C), 1.0);
+    return p * __builtin_bit_cast(double, __builtin_bit_cast(u64, pow16[k & 15]) + ((u64)(uint32_t)(k >> 4) << 52));
+}
 struct __attribute__((packed, aligned(4))) F4a4 { float x, y, z, w; };          // rows begin at any multiple of 4 bytes
 
 // EPT logits a thread.  Owners of the bound: quads of lanes (64) for n_out <= 16, single threads above; the list holds n_out shares of either.
@@ -41,7 +53,7 @@ struct __attribute__((packed, aligned(4))) F4a4 { float x, y, z, w; };          
 // cut lane by lane, those chunks ended last: 29 us in all for the 131 MB, so 24).
 template <int EPT> __global__ void __launch_bounds__(256) beam_scan_kernel(BeamArgs a) {
     constexpr int CAP = BEAM_MAX_OUT * EPT;
-    __shared__ u64 s_own[256], s_list[CAP]; __shared__ float s_red[12]; __shared__ u64 s_bound; __shared__ int s_n;
+    __shared__ u64 s_own[256], s_list[CAP]; __shared__ float s_red[8]; __shared__ double s_sum[4], s_pow[16]; __shared__ u64 s_bound; __shared__ int s_n;
     const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, base = blockIdx.x * 256 * EPT;
     const float *x = reinterpret_cast<const float *>(a.logits + (long)r * a.row) + base;
     const int n = min(256 * EPT, a.n_vocab - base);
@@ -70,25 +82,27 @@ template <int EPT> __global__ void __launch_bounds__(256) beam_scan_kernel(BeamA
         for (int i = 0; i < 64; ++i) above += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ot), i)) > ot;
     }
     const float wm = wave_max(top), wb = -wave_max(4 * above < a.n_out ? -ot : -INFINITY);          // (4 above < n_out: fewer than n_out / 4, rounded up, are before it)
-    if (lane == 0) { s_red[wave] = wm; s_red[8 + wave] = wb; }
+    if (lane == 0) { s_red[wave] = wm; s_red[4 + wave] = wb; }
+    if (tid < 16) s_pow[tid] = exp2(tid * 0.0625);
     if (tid == 0) s_n = 0;
     __syncthreads();
-    const float m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3])), least = fminf(fminf(s_red[8], s_red[9]), fminf(s_red[10], s_red[11]));
+    const float m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3])), least = fminf(fminf(s_red[4], s_red[5]), fminf(s_red[6], s_red[7]));
     bool by_keys = least == -INFINITY;
     if (!by_keys) {
 #pragma unroll
         for (int e = 0; e < EPT; ++e) if (v[e] >= least) { const int p = atomicAdd(&s_n, 1); if (p < CAP) s_list[p] = logit_key(v[e], base + index(e)); }
     }
-    float l = 0.f;
-    if (m != -INFINITY) {
+    double l = 0.0; bool nan = false;
 #pragma unroll
-        for (int e = 0; e < EPT; ++e) l += __builtin_amdgcn_exp2f((v[e] - m) * 1.44269504088896341f);
-    } else {
+    for (int e = 0; e < EPT; ++e) nan |= v[e] != v[e];
+    if (m != -INFINITY) {          // (nothing but -inf: 0)
 #pragma unroll
-        for (int e = 0; e < EPT; ++e) l += v[e] != v[e] ? v[e] : 0.f;       // (nothing but -inf and NaN: NaN stays in the sum)
+        for (int e = 0; e < EPT; ++e) l += exp_below((double)v[e] - (double)m, s_pow);
     }
-    l = wave_sum_dpp(l);
-    if (lane == 0) s_red[4 + wave] = l;
+    if (nan) l = __builtin_nan("");
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
+    if (lane == 0) s_sum[wave] = l;
     __syncthreads();
     if (!by_keys) by_keys = s_n > CAP;
     if (by_keys) {          // (uniform)
@@ -112,7 +126,7 @@ template <int EPT> __global__ void __launch_bounds__(256) beam_scan_kernel(BeamA
         __syncthreads();
     }
     const int count = s_n; const long row = (long)r * a.chunks + blockIdx.x;
-    if (tid == 0) a.stat[row] = make_float2(m, (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]));
+    if (tid == 0) a.stat[row] = BeamStat{(s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]), m};
     for (int i = tid; i < count; i += 256) {
         const u64 mine = s_list[i]; int rank = 0;
 #pragma unroll 4
@@ -194,22 +208,17 @@ template <int OWN> __global__ void __launch_bounds__(1024) beam_join_kernel(Beam
     for (int p = 0; p < OWN; ++p) if (p * 1024 < lists) head[p] = best[(long)min(first_of_lane() + p * 1024, lists - 1) * k];
     for (int b0 = 0; b0 < a.n_beam; b0 += 64) {          // 16 lanes to a beam
         const int b = b0 + (tid >> 4), r = g * a.n_beam + min(b, a.n_beam - 1);
-        const float2 *stat = a.stat + (long)r * a.chunks;
+        const BeamStat *stat = a.stat + (long)r * a.chunks;
         const float score = a.score[r]; const bool done = a.done && a.done[r];
-        float m = -INFINITY, l = 0.f;          // the lane's chunks, on their own maximum
-        for (int c = tid & 15; c < a.chunks; c += 16) {
-            const float2 s = stat[c]; const float to = fmaxf(m, s.x);
-            if (to != -INFINITY) l = l * __builtin_amdgcn_exp2f((m - to) * 1.44269504088896341f) + s.y * __builtin_amdgcn_exp2f((s.x - to) * 1.44269504088896341f); else l += s.y;
-            m = to;
-        }
+        float m = -INFINITY; double l = 0.0;          // the lane's chunks, on the row's maximum
+        for (int c = tid & 15; c < a.chunks; c += 16) m = fmaxf(m, stat[c].top);
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1) {
-            const float om = __shfl_xor(m, d, 64), ol = __shfl_xor(l, d, 64), to = fmaxf(m, om);
-            if (to != -INFINITY) l = l * __builtin_amdgcn_exp2f((m - to) * 1.44269504088896341f) + ol * __builtin_amdgcn_exp2f((om - to) * 1.44269504088896341f); else l += ol;
-            m = to;
-        }
+        for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+        for (int c = tid & 15; c < a.chunks; c += 16) { const BeamStat s = stat[c]; l += m == -INFINITY ? s.sum : s.sum * exp((double)s.top - (double)m); }
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) l += __shfl_xor(l, d, 64);
         if ((tid & 15) == 0 && b < a.n_beam) {
-            s_top[b] = m; s_lse[b] = log((double)l); s_score[b] = score;
+            s_top[b] = m; s_lse[b] = log(l); s_score[b] = score;
             const bool none = score != score || score == -INFINITY || (!done && (l != l || m == INFINITY || m == -INFINITY));
             s_kind[b] = none ? 2 : done ? 1 : 0;
         }
@@ -278,7 +287,7 @@ static int64_t beam_check(const cdna4_tensor *x, int n_beam, int n_out, int pad,
     const long whole = (x->ne[0] + BEAM_CHUNK - 1) / BEAM_CHUNK;
     a->chunk = x->ne[1] * whole < 256 || whole * BEAM_CHUNK * 4 > x->ne[0] * 5 ? BEAM_CHUNK / 4 : BEAM_CHUNK;
     a->chunks = (a->n_vocab + a->chunk - 1) / a->chunk;
-    return x->ne[1] * a->chunks * (8 + 8 * (int64_t)n_out);
+    return x->ne[1] * a->chunks * ((int64_t)sizeof(BeamStat) + 8 * (int64_t)n_out);
 }
 int64_t cdna4_beam_select_workspace(const cdna4_tensor *logits, int n_beam, int n_out, int pad) { PG_NORM(logits, 4) BeamArgs a; return beam_check(logits, n_beam, n_out, pad, &a); }
 int cdna4_op_beam_select(cdna4_context *ctx, const cdna4_tensor *logits, const float *score, const int32_t *done, int n_beam, int n_out, int pad, float *score_out, int32_t *parent, int32_t *token,
@@ -295,7 +304,7 @@ int cdna4_op_beam_select(cdna4_context *ctx, const cdna4_tensor *logits, const f
     a.score = score; a.done = done; a.score_out = score_out; a.parent = parent; a.token = token;
     DEVICE_SCOPE(ctx);
     const int rc = cdna4_ensure_ws(ctx, (size_t)bytes, (hipStream_t)stream); if (rc) return rc;
-    a.stat = (float2 *)ctx->ws; a.best = (u64 *)(a.stat + rows * a.chunks);
+    a.stat = (BeamStat *)ctx->ws; a.best = (u64 *)(a.stat + rows * a.chunks);
     hipStream_t st = (hipStream_t)stream; const dim3 grid((unsigned)a.chunks, (unsigned)rows);
     if (a.chunk == BEAM_CHUNK) hipLaunchKernelGGL(beam_scan_kernel<32>, grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(beam_scan_kernel<8>, grid, dim3(256), 0, st, a);
