@@ -2,6 +2,7 @@
 #pragma once
 #include "api_internal.h"
 #include <atomic>
+#include <initializer_list>
 
 #define OP_CHECK(cond, ...) do { if (!(cond)) return cdna4_set_err(CDNA4_E_UNSUPPORTED, __VA_ARGS__); } while (0)
 #define ARG_CHECK(cond, ...) do { if (!(cond)) return cdna4_set_err(CDNA4_E_INVALID, __VA_ARGS__); } while (0)
@@ -58,6 +59,19 @@ static inline bool pg_disjoint_elems(const cdna4_tensor *t, int esz) {
 }
 static inline bool pg_overlap(const void *a, long na, const void *b, long nb) { const char *x = (const char *)a, *y = (const char *)b; return x && y && x < y + nb && y < x + na; }
 static inline bool pg_overlap(const cdna4_tensor *a, int ea, const cdna4_tensor *b, int eb) { return pg_overlap(a->data, pg_extent(a, ea), b->data, pg_extent(b, eb)); }
+// memory of an argument: nothing that a call writes may share bytes with anything else that it reads or writes (the workgroups that write run beside those that read)
+struct PgRange { const char *name; const void *p; long n; bool written; };
+static inline PgRange pg_range(const char *name, const cdna4_tensor *t, int esz, bool written) { return PgRange{name, t && !pg_empty(t) ? t->data : nullptr, t && !pg_empty(t) ? pg_extent(t, esz) : 0, written}; }
+static inline PgRange pg_range(const char *name, const void *p, long n, bool written) { return PgRange{name, n > 0 ? p : nullptr, n, written}; }
+// pairs: i * 16 + j, i < j, of arguments that have a check of their own
+template <int N> static inline int pg_apart(const char *op, const PgRange (&r)[N], std::initializer_list<int> pairs = {}) {
+    for (int i = 0; i < N; ++i) for (int j = i + 1; j < N; ++j) {
+        if (!r[i].written && !r[j].written) continue;
+        bool own = false; for (const int x : pairs) own |= x == i * 16 + j;
+        ARG_CHECK(own || !pg_overlap(r[i].p, r[i].n, r[j].p, r[j].n), "%s: %s and %s share memory and one of them is written", op, r[i].name, r[j].name);
+    }
+    return CDNA4_OK;
+}
 static inline bool pg_same(const cdna4_tensor *a, const cdna4_tensor *b) {
     if (a->data != b->data) return false;
     for (int i = 0; i < 4; ++i) if (a->ne[i] != b->ne[i] || (a->ne[i] > 1 && a->nb[i] != b->nb[i])) return false;

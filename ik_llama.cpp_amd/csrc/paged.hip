@@ -97,9 +97,10 @@ int cdna4_op_paged_store(cdna4_context *ctx, const cdna4_tensor *k, const cdna4_
     if (n_seq == 0) return CDNA4_OK;
     ARG_CHECK(n_kv && (a.c.table || a.c.W == 0) && (n_tok == 0 || (k->data && v->data)) && (!pos || n_past), "paged_store: null data");
     ARG_CHECK((!weight || weight->data || a.c.W == 0) && (!pos || pos->data || a.c.W == 0), "paged_store: null data");
-    ARG_CHECK(!n_kv_out || (!pg_overlap(n_kv_out, n_seq * 4, n_kv, n_seq * 4) && !pg_overlap(n_kv_out, n_seq * 4, start, (n_seq + 1) * 4) && !pg_overlap(n_kv_out, n_seq * 4, n_past, n_seq * 4)),
-              "paged_store: n_kv_out overlaps an input");
-    ARG_CHECK(!weight || !pos || a.c.W == 0 || !pg_overlap(weight, 4, pos, 4), "paged_store: weight overlaps pos");
+    const PgRange args[] = {pg_range("k_cache", k_cache, 2, true), pg_range("v_cache", v_cache, 2, true), pg_range("weight", weight, 4, true), pg_range("pos", pos, 4, true),
+                            pg_range("n_kv_out", n_kv_out, n_seq * 4, true), pg_range("k", k, 4, false), pg_range("v", v, 4, false), pg_range("table", table, 4, false),
+                            pg_range("n_kv", n_kv, n_seq * 4, false), pg_range("start", start, (n_seq + 1) * 4, false), pg_range("n_past", n_past, n_seq * 4, false)};
+    if ((rc = pg_apart("paged_store", args, {0 * 16 + 1}))) return rc;
     a.k = (const char *)k->data; a.v = (const char *)v->data; a.k_head = k->nb[1]; a.v_head = v->nb[1]; a.k_tok = k->nb[2]; a.v_tok = v->nb[2];
     a.c.n_kv = n_kv; a.start = start; a.n_past = n_past; a.weight = slot_view(weight); a.pos = slot_view(pos); a.n_kv_out = n_kv_out; a.n_tok = (int)n_tok;
     const int units = 2 * a.c.n_head_kv * (a.c.D / 8);
@@ -156,12 +157,9 @@ int cdna4_op_paged_fork(cdna4_context *ctx, const cdna4_tensor *k_cache, const c
     OP_CHECK(n_out <= PAGED_MAX_SEQ, "paged_fork: at most %ld rows", PAGED_MAX_SEQ);
     if (n_out == 0) return CDNA4_OK;
     ARG_CHECK(n_seq > 0 && n_kv && parent && fresh && n_kv_out && ((a.c.table && table_out->data) || a.c.W == 0), "paged_fork: null data");
-    ARG_CHECK(!pg_overlap(n_kv_out, n_out * 4, n_kv, n_seq * 4) && !pg_overlap(n_kv_out, n_out * 4, parent, n_out * 4) && !pg_overlap(n_kv_out, n_out * 4, fresh, n_out * 4),
-              "paged_fork: n_kv_out overlaps an input");
-    if (a.c.W) {
-        ARG_CHECK(!pg_overlap(table_out, 4, table, 4) && !pg_overlap(table_out->data, pg_extent(table_out, 4), parent, n_out * 4) && !pg_overlap(table_out->data, pg_extent(table_out, 4), fresh, n_out * 4) &&
-                  !pg_overlap(table_out->data, pg_extent(table_out, 4), n_kv, n_seq * 4) && !pg_overlap(table_out->data, pg_extent(table_out, 4), n_kv_out, n_out * 4), "paged_fork: table_out overlaps another argument");
-    }
+    const PgRange args[] = {pg_range("k_cache", k_cache, 2, true), pg_range("v_cache", v_cache, 2, true), pg_range("table_out", table_out, 4, true), pg_range("n_kv_out", n_kv_out, n_out * 4, true),
+                            pg_range("table", table, 4, false), pg_range("n_kv", n_kv, n_seq * 4, false), pg_range("parent", parent, n_out * 4, false), pg_range("fresh", fresh, n_out * 4, false)};
+    if ((rc = pg_apart("paged_fork", args, {0 * 16 + 1}))) return rc;
     a.c.n_kv = n_kv; a.parent = parent; a.fresh = fresh; a.table_out = (int *)table_out->data; a.n_kv_out = n_kv_out; a.out_row = table_out->nb[1] / 4;
     DEVICE_SCOPE(ctx);
     hipLaunchKernelGGL(paged_fork_kernel, dim3((unsigned)a.c.n_head_kv, (unsigned)n_out), dim3(256), 0, (hipStream_t)stream, a);
@@ -396,11 +394,15 @@ int cdna4_op_paged_evict(cdna4_context *ctx, const cdna4_tensor *k_cache, const 
     if (a.c.n_seq == 0) return CDNA4_OK;
     const long n = a.c.n_seq;
     ARG_CHECK(n_kv && n_past && n_kv_out && (a.c.W == 0 || (a.c.table && weight->data && pos->data && weight_out->data && pos_out->data)), "paged_evict: null data");
-    ARG_CHECK(!pg_overlap(n_kv_out, n * 4, n_kv, n * 4) && !pg_overlap(n_kv_out, n * 4, n_past, n * 4), "paged_evict: n_kv_out overlaps an input");
+    const PgRange args[] = {pg_range("k_cache", k_cache, 2, true), pg_range("v_cache", v_cache, 2, true), pg_range("weight_out", weight_out, 4, true), pg_range("pos_out", pos_out, 4, true),
+                            pg_range("n_kv_out", n_kv_out, n * 4, true), pg_range("weight", weight, 4, false), pg_range("pos", pos, 4, false), pg_range("table", table, 4, false),
+                            pg_range("n_kv", n_kv, n * 4, false), pg_range("n_past", n_past, n * 4, false)};
+    int rc = pg_apart("paged_evict", args, {0 * 16 + 1, 2 * 16 + 5, 3 * 16 + 6});          // (in place or apart: evict_check)
+    if (rc) return rc;
     a.c.n_kv = n_kv; a.n_past = n_past; a.n_kv_out = n_kv_out;
     a.weight = slot_view(weight); a.pos = slot_view(pos); a.weight_out = slot_view(weight_out); a.pos_out = slot_view(pos_out);
     DEVICE_SCOPE(ctx);
-    int rc = cdna4_ensure_ws(ctx, (size_t)bytes, (hipStream_t)stream); if (rc) return rc;
+    if ((rc = cdna4_ensure_ws(ctx, (size_t)bytes, (hipStream_t)stream))) return rc;
     a.moves = (int *)ctx->ws;
     const long most = evict_most(a.c, budget);
     const dim3 grid((unsigned)a.c.n_head_kv, (unsigned)n); hipStream_t st = (hipStream_t)stream;

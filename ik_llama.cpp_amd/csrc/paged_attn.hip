@@ -538,7 +538,9 @@ int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_t
     AttnArgs a; int rc = attn_check(q, k_cache, v_cache, table, weight, dst, &a); if (rc) return rc;
     if (pg_empty(q)) return CDNA4_OK;
     ARG_CHECK(n_kv && q->data && dst->data && (a.c.W == 0 || (a.c.table && (!weight || weight->data))), "paged_attn: null data");
-    ARG_CHECK(!pg_overlap(q, 4, dst, 4) && (!weight || a.c.W == 0 || (!pg_overlap(weight, 4, dst, 4) && !pg_overlap(weight, 4, q, 4))), "paged_attn: q, dst and weight may not overlap");
+    const PgRange args[] = {pg_range("dst", dst, 4, true), pg_range("weight", weight, 4, true), pg_range("q", q, 4, false), pg_range("k_cache", k_cache, 2, false),
+                            pg_range("v_cache", v_cache, 2, false), pg_range("table", table, 4, false), pg_range("n_kv", n_kv, (long)a.c.n_seq * 4, false)};
+    if ((rc = pg_apart("paged_attn", args))) return rc;
     if (a.c.W == 0) { a.c.table = n_kv; a.c.table_row = 0; }          // (no slots: the entry that is read for a missing one is anything)
     a.c.n_kv = n_kv; a.scale = scale; a.softcap = softcap; a.inv_softcap = softcap != 0.0f ? 1.0f / softcap : 0.0f;
     a.q = (const char *)q->data; a.q_head = q->nb[1]; a.q_seq = q->nb[2]; a.dst = (char *)dst->data; a.d_head = dst->nb[1]; a.d_seq = dst->nb[2];
