@@ -82,6 +82,27 @@ static inline bool pg_sizes_ok(const cdna4_tensor *t) {                 // (no p
     return true;
 }
 
+// K and V caches that a call writes are apart: memory of their own, or views of one pool that take turns (pages of K beside pages of V, or rows inside a page)
+static inline bool pg_kv_apart(const cdna4_tensor *k, const cdna4_tensor *v) {
+    if (pg_empty(k) || !pg_overlap(k, 2, v, 2)) return true;
+    if (k->ne[3] > 1 && k->nb[3] == v->nb[3]) {          // in-page extents that both fit beside each other into the distance of two pages
+        cdna4_tensor kp = *k, vp = *v; kp.ne[3] = vp.ne[3] = 1;
+        const long step = k->nb[3], ek = pg_extent(&kp, 2), ev = pg_extent(&vp, 2), d = (((const char *)v->data - (const char *)k->data) % step + step) % step;
+        if (ek <= d && d + ev <= step) return true;
+    }
+    for (int i = 0; i < 4; ++i) if (k->ne[i] > 1 && k->nb[i] != v->nb[i]) return false;
+    // one tensor with a dimension of two for K and V: every stride steps over the extent of the smaller ones
+    const char *kd = (const char *)k->data, *vd = (const char *)v->data;
+    long ne[5] = {k->ne[0], k->ne[1], k->ne[2], k->ne[3], 2}, nb[5] = {k->nb[0], k->nb[1], k->nb[2], k->nb[3], vd > kd ? vd - kd : kd - vd}, need = 2;
+    for (int n = 0; n < 5; ++n) {
+        int least = -1; for (int i = 0; i < 5; ++i) if (ne[i] > 1 && (least < 0 || nb[i] < nb[least])) least = i;
+        if (least < 0) break;
+        if (nb[least] < need) return false;
+        need += nb[least] * (ne[least] - 1); ne[least] = 1;
+    }
+    return true;
+}
+
 // a descriptor whose dimensions of one element (or none) have the strides of a dense tensor: the caller's say nothing
 static inline cdna4_tensor pg_norm(const cdna4_tensor *t, int esz) {
     cdna4_tensor n = *t;

@@ -101,6 +101,7 @@ int cdna4_op_paged_store(cdna4_context *ctx, const cdna4_tensor *k, const cdna4_
                             pg_range("n_kv_out", n_kv_out, n_seq * 4, true), pg_range("k", k, 4, false), pg_range("v", v, 4, false), pg_range("table", table, 4, false),
                             pg_range("n_kv", n_kv, n_seq * 4, false), pg_range("start", start, (n_seq + 1) * 4, false), pg_range("n_past", n_past, n_seq * 4, false)};
     if ((rc = pg_apart("paged_store", args, {0 * 16 + 1}))) return rc;
+    ARG_CHECK(pg_kv_apart(k_cache, v_cache), "paged_store: K and V share rows");
     a.k = (const char *)k->data; a.v = (const char *)v->data; a.k_head = k->nb[1]; a.v_head = v->nb[1]; a.k_tok = k->nb[2]; a.v_tok = v->nb[2];
     a.c.n_kv = n_kv; a.start = start; a.n_past = n_past; a.weight = slot_view(weight); a.pos = slot_view(pos); a.n_kv_out = n_kv_out; a.n_tok = (int)n_tok;
     const int units = 2 * a.c.n_head_kv * (a.c.D / 8);
@@ -160,6 +161,7 @@ int cdna4_op_paged_fork(cdna4_context *ctx, const cdna4_tensor *k_cache, const c
     const PgRange args[] = {pg_range("k_cache", k_cache, 2, true), pg_range("v_cache", v_cache, 2, true), pg_range("table_out", table_out, 4, true), pg_range("n_kv_out", n_kv_out, n_out * 4, true),
                             pg_range("table", table, 4, false), pg_range("n_kv", n_kv, n_seq * 4, false), pg_range("parent", parent, n_out * 4, false), pg_range("fresh", fresh, n_out * 4, false)};
     if ((rc = pg_apart("paged_fork", args, {0 * 16 + 1}))) return rc;
+    ARG_CHECK(pg_kv_apart(k_cache, v_cache), "paged_fork: K and V share rows");
     a.c.n_kv = n_kv; a.parent = parent; a.fresh = fresh; a.table_out = (int *)table_out->data; a.n_kv_out = n_kv_out; a.out_row = table_out->nb[1] / 4;
     DEVICE_SCOPE(ctx);
     hipLaunchKernelGGL(paged_fork_kernel, dim3((unsigned)a.c.n_head_kv, (unsigned)n_out), dim3(256), 0, (hipStream_t)stream, a);
@@ -399,6 +401,7 @@ int cdna4_op_paged_evict(cdna4_context *ctx, const cdna4_tensor *k_cache, const 
                             pg_range("n_kv", n_kv, n * 4, false), pg_range("n_past", n_past, n * 4, false)};
     int rc = pg_apart("paged_evict", args, {0 * 16 + 1, 2 * 16 + 5, 3 * 16 + 6});          // (in place or apart: evict_check)
     if (rc) return rc;
+    ARG_CHECK(pg_kv_apart(k_cache, v_cache), "paged_evict: K and V share rows");
     a.c.n_kv = n_kv; a.n_past = n_past; a.n_kv_out = n_kv_out;
     a.weight = slot_view(weight); a.pos = slot_view(pos); a.weight_out = slot_view(weight_out); a.pos_out = slot_view(pos_out);
     DEVICE_SCOPE(ctx);

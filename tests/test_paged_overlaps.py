@@ -25,3 +25,8 @@ def run_case(script, tmp_path):
 def test_written_arguments_share_no_memory_with_others(tmp_path):
     out = run_case("paged_overlap_case.py", tmp_path)
     assert int(out.split("overlaps ok")[1]) >= 90
+
+
+def test_caches_that_are_written_share_no_rows(tmp_path):
+    accepted, refused = (int(x) for x in run_case("paged_kv_case.py", tmp_path).split("kv ok")[1].split())
+    assert accepted >= 9 and refused >= 80
