@@ -1,5 +1,6 @@
 """ctypes binding of include/ggml_hip_cdna4.h (the C-ABI drop-in boundary)."""
 import ctypes as C
+import operator
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -47,6 +48,14 @@ def act_row_size(vdt, k):
 class Cdna4Error(RuntimeError):
     def __init__(self, code, msg):
         super().__init__("cdna4 error %d: %s" % (code, msg)); self.code = code
+
+
+def _int32(name, x):
+    """a whole number for a C int: ctypes would cut what does not fit"""
+    x = operator.index(x)
+    if not -(1 << 31) <= x < 1 << 31:
+        raise Cdna4Error(-2, "%s: a whole number of 32 bits" % name)
+    return x
 
 
 def lib_path():
@@ -483,6 +492,7 @@ class Cdna4Backend:
     def paged_evict(self, k_cache, v_cache, table, n_kv, weight, pos, n_past, budget, n_sink=0, n_recent=0, weight_out=None, pos_out=None, n_kv_out=None):
         """cdna4_op_paged_evict: every (sequence, KV head) keeps `budget` slots, by position and gathered weight; weight_out / pos_out None: in place.  Returns the new n_kv."""
         d, vec, dev = self._desc, self._vec, self._dev
+        budget, n_sink, n_recent = _int32("budget", budget), _int32("n_sink", n_sink), _int32("n_recent", n_recent)
         td = d(table, "table", dev); n = table.shape[-2]
         if n_kv_out is None:
             n_kv_out = self._empty(table, 26, n)
@@ -495,6 +505,7 @@ class Cdna4Backend:
     def beam_select(self, logits, score, n_beam, n_out, done=None, pad=0, outs=None):
         """cdna4_op_beam_select: logits f32 [n_group * n_beam, n_vocab], score f32 [n_group * n_beam] -> (score f32, parent row int32, token int32), each [n_group, n_out]."""
         vec, dev = self._vec, self._dev
+        n_beam, n_out, pad = _int32("n_beam", n_beam), _int32("n_out", n_out), _int32("pad", pad)
         ld = self._desc(logits, "logits", dev)
         rows = logits.shape[-2]; n_group = rows // n_beam if n_beam > 0 else 0
         if outs is None:
@@ -527,11 +538,12 @@ class Cdna4Backend:
         """bytes of scratch that paged_evict takes"""
         d, dev = self._desc, self._dev
         w, p = d(weight, "weight", dev), d(pos, "pos", dev)
+        budget, n_sink, n_recent = _int32("budget", budget), _int32("n_sink", n_sink), _int32("n_recent", n_recent)
         return self._bytes(self.lib.cdna4_paged_evict_workspace(d(k_cache, "k_cache", dev), d(v_cache, "v_cache", dev), d(table, "table", dev), w, p, budget, n_sink, n_recent, w, p))
 
     def beam_workspace(self, logits, n_beam, n_out, pad=0):
         """bytes of scratch that beam_select takes"""
-        return self._bytes(self.lib.cdna4_beam_select_workspace(self._desc(logits, "logits", self._dev), n_beam, n_out, pad))
+        return self._bytes(self.lib.cdna4_beam_select_workspace(self._desc(logits, "logits", self._dev), _int32("n_beam", n_beam), _int32("n_out", n_out), _int32("pad", pad)))
 
     def _bytes(self, n):
         if n < 0:
