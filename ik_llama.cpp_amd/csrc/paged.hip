@@ -223,7 +223,7 @@ static __device__ __forceinline__ unsigned waves_before(const unsigned (&tot)[EV
     return b;
 }
 template <bool HERE> __global__ void __launch_bounds__(EVICT_THREADS) paged_evict_select_kernel(EvictArgs a) {
-    extern __shared__ uint32_t s_key[];
+    extern __shared__ __attribute__((aligned(16))) uint32_t s_key[];
     __shared__ unsigned hist[EVICT_BINS * EVICT_COPIES], tot[3][EVICT_WAVES], s_digit, s_rest, s_equal; __shared__ int s_moves[HERE ? 2 * EVICT_HERE : 1];
     const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int raw = a.c.n_kv[s], n = paged_len(a.c, s), most = (a.list - 1) / 2;

@@ -120,7 +120,7 @@ struct Shares {
 template <int D, bool BF16, bool CAP, bool ONE, int QB> __global__ void __launch_bounds__(256, (D * QB <= 128 ? 2 : 1)) paged_attn_kernel(AttnArgs a) {
     constexpr int HEADS = QB * QH, KC = D / 32, VW = D == 64 ? 4 : 8, VH = D == 256 ? 2 : 1, NS = Split<BF16>::N;      // K chunks of 32 elements; V elements of a lane and half; halves of 128
     constexpr float P_SCALE = BF16 ? 1.0f / 32.0f : 32768.0f;          // of a step's probabilities: 32 of 2^-5 sum to 1 in bf16; f16 keeps the bits of those down to 2^-29 of the largest
-    extern __shared__ int s_mem[];
+    extern __shared__ __attribute__((aligned(16))) int s_mem[];
     __shared__ int s_tot[4]; __shared__ float s_m[WAVES][HEADS], s_l[WAVES][HEADS], s_row[2][HEADS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     int *pre = s_mem;                                                              // prefix sums (not ONE)
