@@ -7,6 +7,7 @@ import hashlib
 import os
 import shutil
 import subprocess
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -107,15 +108,15 @@ def build_library(force=False, verbose=False, extra_flags=(), out=None, tag=None
     return LIB
 
 
-BINDING = os.path.join(HERE, "cdna4_args.so")
+BINDING = os.path.join(HERE, "cdna4_args" + sysconfig.get_config_var("EXT_SUFFIX"))          # (an interpreter of another ABI does not find it)
 
 
 def build_binding(force=False, verbose=False):
     """Compile the binding's C++ part (csrc/binding_args.cpp: torch tensors into descriptors; host code only) against the torch and Python of this interpreter.  Returns its path."""
-    import sysconfig
     import torch
     src = os.path.join(CSRC, "binding_args.cpp"); inc = os.path.join(os.path.dirname(torch.__file__), "include"); lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
+           '-DBUILT_WITH="%s"' % torch.__version__,
            "-I" + inc, "-I" + os.path.join(inc, "torch", "csrc", "api", "include"), "-I" + sysconfig.get_paths()["include"], src, "-o", BINDING + ".tmp",
            "-L" + lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
     h = hashlib.sha256((" ".join(cmd) + torch.__version__).encode()); h.update(open(src, "rb").read())

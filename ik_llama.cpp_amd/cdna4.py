@@ -191,12 +191,15 @@ def load_args():
     global _args
     if _args is None:
         import importlib.util
-        import torch  # noqa: F401  (its libraries are what the module is linked against)
-        p = os.path.join(HERE, "cdna4_args.so")
+        import sysconfig
+        import torch  # (its libraries are what the module is linked against)
+        p = os.path.join(HERE, "cdna4_args" + sysconfig.get_config_var("EXT_SUFFIX"))
         if not os.path.exists(p):
             raise FileNotFoundError("%s not found: build it with `python -m ik_llama.cpp_amd.build` / __graft_entry__.build()" % p)
         spec = importlib.util.spec_from_file_location("cdna4_args", p)
         m = importlib.util.module_from_spec(spec); spec.loader.exec_module(m)
+        if m.built_with != torch.__version__:          # (it reads torch's C++ objects: their layout is the version's)
+            raise RuntimeError("%s was built against torch %s, this is %s: build it again with `python -m ik_llama.cpp_amd.build` / __graft_entry__.build()" % (p, m.built_with, torch.__version__))
         m.set_error(Cdna4Error)
         _args = m
     return _args

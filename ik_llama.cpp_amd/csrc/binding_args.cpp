@@ -84,4 +84,8 @@ PyMethodDef methods[] = {{"desc", (PyCFunction)(void *)desc, METH_FASTCALL, "cdn
                          {"set_error", set_error, METH_O, "the class of what is raised"}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "cdna4_args", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 }
-PyMODINIT_FUNC PyInit_cdna4_args(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit_cdna4_args(void) {
+    PyObject *m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "built_with", BUILT_WITH) < 0) { Py_DECREF(m); return nullptr; }          // (the loader compares it with the torch that is there)
+    return m;
+}
