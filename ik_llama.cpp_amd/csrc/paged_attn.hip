@@ -551,8 +551,8 @@ int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_t
     hipStream_t st = (hipStream_t)stream;
     const size_t merge = (size_t)WAVES * std::min(QH, a.group) * (a.c.D + 4) * 4;
     // A workgroup per unit where a unit is little work, or where the units fill the chip and none is long.  Measured, us with a workgroup per unit / with equal shares and a join (f16, 32
-    // query heads and 8 KV heads of 128; sequences x slots): 1 x 100: 5.9 / 8.8, 1 x 640: 9.8 / 10.5, 1 x 1024: 13.0 / 10.6, 8 x 1024: 13.4 / 13.2, 32 x 1024: 16.9 / 23.2, 64 x 512: 16.7 /
-    // 24.4, 64 x 2048: 56 / 62, 256 x 2048: 204 / 223; bf16, 4 heads of 64, 1 x 768: 7.8 / 9.6; of 256, 1 x 512: 14.3 / 13.0, 128 x 2048: 111 / 110.
+    // query heads and 8 KV heads of 128; sequences x slots): 1 x 100: 6.2 / 9.2, 1 x 640: 10.2 / 11.2, 1 x 1024: 13.5 / 11.3, 8 x 1024: 14.2 / 14.7, 32 x 1024: 23.9 / 30.9, 64 x 512: 24.2 /
+    // 29.4, 64 x 2048: 94 / 100, 256 x 2048: 359 / 373; bf16, 4 heads of 64, 1 x 768: 8.3 / 10.0; of 256, 1 x 512: 14.9 / 13.8, 128 x 2048: 355 / 377.
     // With weights: if a KV head is one unit and its scores fit LDS.
     const size_t one_lds = merge + (weight ? (size_t)a.group * a.score_row * 4 : 0);
     const bool one = (row_tiles * a.c.D <= 640 || (row_tiles <= 16 && (long)a.c.n_seq * n_unit >= ctx->num_cu)) && (!weight || a.group <= QH) && one_lds <= ONE_LDS;
@@ -566,14 +566,15 @@ int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_t
         ATTN_ALL(true, dim3((unsigned)n_unit, (unsigned)a.c.n_seq), one_lds);
         return CDNA4_OK;
     }
-    // Groups of 17 to 32 heads over much cache: 32 heads to a wave, so that it is read once (heads of 64 and 128; for 256 there are not registers enough).  Two of those waves' registers do
-    // not fit a SIMD (heads of 128), so each of its steps is in the open: with fewer tiles than 16 to a CU, or rows of which the ends count, two blocks of 16 are faster.  us with blocks
-    // of 16 / 32 to a wave (f16, 20 heads a KV head; sequences x slots, KV heads): of 128: 64 x 8192, 8: 373 / 261, 32 x 8192, 4: 93 / 73, 64 x 8192, 1 (32 heads): 51.6 / 44.3, 16 x 4099, 8:
-    // 49.6 / 55.2, 4: 27.6 / 28.6, 1 x 3000, 1: 11.9 / 13.7; of 64: 64 x 8192, 8: 156 / 136, 16 x 4099, 8: 32.7 / 27.6, 1 x 130000, 4: 38.5 / 35.2, 1 (bf16): 18.8 / 20.6.
+    // Groups of 17 to 32 heads over much cache: 32 heads to a wave, so that it is read once (heads of 64, and of 128 in f16; for 256 there are not registers enough).  Two of those waves'
+    // registers do not fit a SIMD (heads of 128), so each of its steps is in the open: with fewer tiles than 16 to a CU, or rows of which the ends count, two blocks of 16 are faster, and in
+    // bf16, which has three terms for two, always.  us with blocks of 16 / 32 to a wave (sequences of up to as many slots, query heads on KV heads; f16): of 128: 64 x 8192, 160 on 8: 334 /
+    // 300 (bf16: 276 / 298), 32 x 8192, 80 on 4: 90.6 / 83.8 (75.3 / 82.6), 64 x 8192, 20 on 1: 50.1 / 47.8 (44.2 / 47.2), 16 x 4099, 160 on 8: 51.0 / 59.2, 1 x 3000, 20 on 1: 12.4 / 14.7;
+    // of 64: 64 x 8192, 160 on 8: 160 / 140 (157 / 139), 16 x 4099, 160 on 8: 34.2 / 29.3, 1 x 130000, 20 on 1: 19.4 / 21.7.
     // Larger groups (and the others): blocks of 16 heads that read the same tiles at the same time: workgroups that are a multiple of 8 apart share an XCD and its L2, so much of the cache
-    // comes from memory once.  us with a numbering of all blocks one after the other / with this one: 64 x 8192, 32 on 1 of 128: 54.5 / 51.4, 1 x 130000, 20 on 1 of 256: 50.4 / 43.5; bf16,
-    // 128 on 1 of 128: 80.8 / 51.8; 48 on 1 of 128, 64 x 8192: 100 (32 to a wave: 121).
-    const bool two = a.group > QH && a.group <= 2 * QH && a.c.D <= 128 && tiles >= 16l * ctx->num_cu && row_tiles * TILE >= 64 * a.c.D;
+    // comes from memory once.  (Before a step's sums were its own, us with a numbering of all blocks one after the other / with this one: 64 x 8192, 32 on 1 of 128: 54.5 / 51.4, 1 x 130000,
+    // 20 on 1 of 256: 50.4 / 43.5; bf16, 128 on 1 of 128: 80.8 / 51.8.)
+    const bool two = a.group > QH && a.group <= 2 * QH && (a.c.D == 64 || (a.c.D == 128 && !bf)) && tiles >= 16l * ctx->num_cu && row_tiles * TILE >= 64 * a.c.D;
     if (two) { a.lg = 5; a.blocks = 1; }
     const int qb = two ? 2 : 1, per_cu = a.c.D == 256 || (a.c.D == 128 && two) ? 1 : 2;          // (what the registers allow)
     long most_wg = std::min<long>((long)ctx->num_cu * per_cu, ATTN_MAX_WG / qb) / a.blocks;       // (blocks: at most 1024)
@@ -585,7 +586,9 @@ int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_t
     a.prefix = (int *)ws; a.part = (float *)(ws + sc.part); a.stat = weight ? (float2 *)(ws + sc.stat) : nullptr; a.score = weight ? (float *)(ws + sc.score) : nullptr;
     const size_t lds = (size_t)((a.c.n_seq + 4) & ~3) * 4 + (size_t)WAVES * std::min(QH * qb, a.group) * (a.c.D + 4) * 4;          // (at most (8192 + 4) * 4 + 4 * 32 * 132 * 4 bytes)
     const dim3 grid((unsigned)(a.n_wg * a.blocks));
-    if (!two) ATTN_ALL(false, grid, lds); else if (a.c.D == 64) ATTN_D(64, false, 2, grid, lds); else ATTN_D(128, false, 2, grid, lds);
+    if (!two) ATTN_ALL(false, grid, lds);
+    else if (a.c.D == 64) ATTN_D(64, false, 2, grid, lds);
+    else { if (cap) ATTN(128, false, true, false, 2, grid, lds); else ATTN(128, false, false, false, 2, grid, lds); HIP_TRY(hipGetLastError()); }
     const dim3 join((unsigned)(a.n_head + (weight ? a.c.n_head_kv * ((a.score_row + 1023) / 1024) : 0)), (unsigned)a.c.n_seq);
 #define JOIN(D_) do { if (weight) hipLaunchKernelGGL((paged_attn_join_kernel<D_, true>), join, dim3(256), 0, st, a); \
                       else hipLaunchKernelGGL((paged_attn_join_kernel<D_, false>), join, dim3(256), 0, st, a); } while (0)
