@@ -367,9 +367,11 @@ CDNA4_API int cdna4_op_moe_router_norm(cdna4_context *ctx, const cdna4_tensor *w
  *   weight, pos      : f32 / i32 [>= W * page, n_head_kv, n_seq]: per slot and KV head, the attention weight that the slot has gathered and the position of its token (the heads keep
  *                      different tokens after an eviction).
  * Attention does not depend on the order of the slots (K is rotated before it is stored), so evictions leave the slots of a sequence in disorder and pos says which token is where.
- * Strides of dimensions with one element do not count.  n_seq, W * page: at most 8192 and 2^30.  n_kv_out may not overlap an input.  Errors: CDNA4_E_INVALID null / inconsistent arguments, CDNA4_E_UNSUPPORTED shapes and types outside the
- * above, CDNA4_E_NOMEM a workspace that would have to grow during stream capture: reserve the largest cdna4_paged_*_workspace / cdna4_beam_select_workspace beforehand.  Those
- * functions run the same checks and return the bytes, or the error; they need no device. */
+ * Strides of dimensions with one element do not count.  n_seq, W * page: at most 8192 and 2^30.  What a call writes (caches, weight, pos, n_kv_out, dst ...) shares no memory with anything
+ * else that it reads or writes; written K and V caches may be views of one pool that take turns (pages beside pages, heads beside heads, rows beside rows).  Errors: CDNA4_E_INVALID null /
+ * inconsistent arguments, CDNA4_E_UNSUPPORTED shapes and types outside the above, CDNA4_E_NOMEM a workspace that would have to grow during stream capture: reserve the largest
+ * cdna4_paged_*_workspace / cdna4_beam_select_workspace beforehand.  Those functions return the bytes, or the error; they need no device and run the checks of shapes, types and strides
+ * (the calls also check addresses). */
 
 /* New tokens into the cache: token i of sequence s (start[s] <= i < start[s + 1]; start NULL: token i belongs to sequence i and n_tok == n_seq) goes to slot n_kv[s] + i - start[s]; its
  * f32 K and V rows ([D, n_head_kv, n_tok], after rope) are rounded once to the cache type, weight (or NULL) becomes 0 and pos (or NULL; needs n_past) n_past[s] + i - start[s] at the
@@ -380,7 +382,10 @@ CDNA4_API int cdna4_op_paged_store(cdna4_context *ctx, const cdna4_tensor *k, co
 /* Attention of one new token per sequence: q f32 [D, n_head, n_seq] -> dst f32 [D, n_head, n_seq]; n_head a multiple of n_head_kv.  scores = scale * q.k, softcap != 0:
  * softcap * tanh(scores / softcap); softmax over the mapped slots j < n_kv[s].  A sequence with nothing to attend to gets a row of zeros.  weight (or NULL): weight[s][hk][j] += the sum of
  * the slot's probabilities over the query heads of hk, every element by one thread in a fixed order.  Results do not depend on the run.  Slots that are not attended to may hold
- * anything (infinities and NaN included); those that are hold finite values. */
+ * anything (infinities and NaN included); those that are hold finite values, of any size.
+ * With T = W * page / 128, rounded up, and B = n_head / n_head_kv / 16, rounded up: T * n_seq * n_head_kv * B < 2^31, T * n_head_kv < 2^26, n_head <= 16384.  The scratch goes by the
+ * table's width and not by the lengths: with weight n_seq * n_head * T * 512 bytes (64 rows of 64 heads over tables of 131072 slots: 2.1 GB) and some MB without; the context keeps it.
+ * Hosts whose tables are much wider than the lengths pass the part of the table that is in use where they need the weights. */
 CDNA4_API int cdna4_op_paged_attn(cdna4_context *ctx, const cdna4_tensor *q, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const int32_t *n_kv,
                                   const cdna4_tensor *weight, const cdna4_tensor *dst, float scale, float softcap, void *stream);
 CDNA4_API int64_t cdna4_paged_attn_workspace(const cdna4_tensor *q, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const cdna4_tensor *weight,
@@ -388,7 +393,8 @@ CDNA4_API int64_t cdna4_paged_attn_workspace(const cdna4_tensor *q, const cdna4_
 /* Eviction by gathered attention weight: every (sequence, KV head) with more than `budget` slots keeps `budget` of them: first the held ones (pos < n_sink or
  * pos >= n_past[s] - n_recent; all alike), then by descending weight (NaN counts as -inf), ties to the lower slot.  Kept slots at budget and above move, in ascending order, into the freed slots
  * below, in ascending order: K and V rows in the cache, weight and pos into weight_out / pos_out (either the very tensors weight / pos, or memory apart from both; values of slots at
- * n_kv_out[s] and above are left as they were).  n_kv_out[s] = min(n_kv[s], budget).  budget >= 1, n_sink + n_recent <= budget.  The pages must belong to their sequence alone. */
+ * n_kv_out[s] and above are left as they were).  n_past counts every token so far, those just stored among them: the newest token's position is n_past[s] - 1.
+ * n_kv_out[s] = min(n_kv[s], budget).  budget >= 1, n_sink + n_recent <= budget.  The pages must belong to their sequence alone. */
 CDNA4_API int cdna4_op_paged_evict(cdna4_context *ctx, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const int32_t *n_kv, const cdna4_tensor *weight,
                                    const cdna4_tensor *pos, const int32_t *n_past, int budget, int n_sink, int n_recent, const cdna4_tensor *weight_out, const cdna4_tensor *pos_out,
                                    int32_t *n_kv_out, void *stream);
@@ -405,7 +411,7 @@ CDNA4_API int64_t cdna4_beam_select_workspace(const cdna4_tensor *logits, int n_
 /* Sequences go on from others: row i of table_out [W, n_out] = the pages of row parent[i] of table; if its last page is cut (n_kv % page != 0) the rows in use are copied into page
  * fresh[i], which takes its place, so that the rows that share a past append apart; entries behind are -1.  n_kv_out[i] = n_kv[parent[i]] (at most W * page).  A parent outside
  * [0, n_seq) or an inactive one gives an inactive row (-1 everywhere); a fresh page outside [0, n_pages) leaves the cut page unmapped.  Fresh pages are distinct and in no row of
- * table.  table_out may not overlap table. */
+ * table. */
 CDNA4_API int cdna4_op_paged_fork(cdna4_context *ctx, const cdna4_tensor *k_cache, const cdna4_tensor *v_cache, const cdna4_tensor *table, const int32_t *n_kv, const int32_t *parent,
                                   const int32_t *fresh, const cdna4_tensor *table_out, int32_t *n_kv_out, void *stream);
 
