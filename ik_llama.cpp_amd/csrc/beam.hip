@@ -3,7 +3,8 @@
 // The logits are read once (4 bytes a candidate against a handful of operations: bound by that read).  A workgroup takes 8192 (2048) neighbouring logits of a row into registers and leaves
 // their maximum, the sum of their exponentials and their n_out best, sorted; a second launch joins a group's chunks: log sum exp of every beam, then the best of the sorted lists.
 // The exponentials and their sums are 64 bits wide: candidates of different beams are ordered by values in which those sums stand, and 32 bits mixed up what differs by less than 10^-6
-// (32 bits took 35.3 us for 256 rows of 128256, 131 MB, 32 groups of 8, 16 results; so it takes 47.8).
+// (32 bits took 35.3 us for 256 rows of 128256, 131 MB, 32 groups of 8, 16 results; so it takes 47.8).  Medians of the launches: 39 us for the chunks, which are bound by 12 64-bit instructions
+// a logit, and 9 us for the join; 4 rows of 32000: 4.5 and 5.3 us.
 //
 // Choosing the k best of many without sorting them: in a total order without ties, the k-th best of the threads' (or lanes' quads') own best elements is a bound that at least k elements
 // reach, and every element that reaches it belongs to one of the k owners whose best does -- so the collected list is never longer than k shares, whatever the values, and in random order
@@ -50,7 +51,7 @@ struct __attribute__((packed, aligned(4))) F4a4 { float x, y, z, w; };          
 // The bound is first taken on values alone, which costs a maximum and a comparison per logit (with keys of value and index all through, the launch was bound by its vector instructions:
 // 45 us for 256 rows of 128256, 131 MB), and from every wave a quarter of n_out (one bound of the workgroup for 64 results took as long as the rest: 480 rows of 70000: 48 us, so 38).  Ties at
 // the bound can make that list too long, and a bound of -inf says nothing: then the keys decide.  A row's last chunk takes its logits one at a time, coalesced (as quads of which the last were
-// cut lane by lane, those chunks ended last: 29 us in all for the 131 MB, so 24).
+// cut lane by lane, those chunks ended last: 29 us in all for the 131 MB, so 24).  (These figures: with sums of 32 bits.)
 template <int EPT> __global__ void __launch_bounds__(256) beam_scan_kernel(BeamArgs a) {
     constexpr int CAP = BEAM_MAX_OUT * EPT;
     __shared__ u64 s_own[256], s_list[CAP]; __shared__ float s_red[8]; __shared__ double s_sum[4], s_pow[16]; __shared__ u64 s_bound; __shared__ int s_n;

@@ -188,8 +188,8 @@ static __device__ __forceinline__ uint32_t evict_key(float w, int p, int sink, i
 //   among equals are taken only if not all keys that equal the last kept one are kept.
 // * Few moves (`here`: at most EVICT_HERE a row, as when a cache is cut back after every few tokens) are made in the same launch from lists in LDS; otherwise the lists go to memory and a
 //   second launch moves the rows with the whole chip.
-// Measured: 128 rows of up to 4160 slots cut to 4096: one launch of 10.2 us (reading 3, digits 2.4, lists 2, moves 2).  32 rows of up to 32768 slots cut to 4096: 24 us (reading 6, digits 5,
-// lists 7: the vector instructions of 32 of the 256 CUs, some 20 for every slot in each) and 25 us for the moves (108 MB, 4.3 TB/s).
+// Measured: 128 rows of up to 4160 slots cut to 4096: one launch of 10.2 us (reading 3, digits 2.4, lists 2, moves 2).  32 rows of up to 32768 slots cut to 4096: 23 us (reading 6, digits 5,
+// lists 7: the vector instructions of 32 of the 256 CUs, some 20 for every slot in each) and 26 - 27 us for the moves (108 MB, 4.1 TB/s).
 constexpr int EVICT_THREADS = 1024, EVICT_WAVES = 16, EVICT_KEYS = 32768, EVICT_HERE = 128, EVICT_BINS = 2048, EVICT_COPIES = 2;
 static __device__ __forceinline__ void evict_move(const EvictArgs &a, int s, int h, int from, int to, int sub) {          // 16 lanes to a row: K, V, weight and pos
     if (sub == 0) {

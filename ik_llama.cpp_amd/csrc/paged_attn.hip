@@ -4,7 +4,7 @@
 // operator is bound by that read (4 D bytes a slot and KV head against 4 D flops a query head).  Three things follow:
 //
 // * Matrix instructions, for any group size: 32 slots are one step of v_mfma_f32_16x16x32.  S^T = K Q^T puts a query head into every lane column and four slots into every lane, which is
-//   the operand layout that O^T = V^T P^T wants for P: the probabilities never leave their registers, and the running maximum and sum of a head are scalars of a lane.  V arrives as rows
+//   the operand layout that O^T = V^T P^T wants for P: the probabilities never leave their registers, and the running reference and sum of a head are scalars of a lane.  V arrives as rows
 //   (16 bytes a lane, a row per 16 lanes) and becomes the other operand by v_perm, so the loop touches no LDS at all.
 // * f32 results from 16-bit operands: q and p are split into two f16 terms or three bf16 ones, K and V are what the cache holds; products and sums are f32.  bf16: exactly 24 bits.  f16: 22
 //   bits, rounded to nearest, down to 2^-28 of a row's largest element or a step's largest probability, the products of the second terms summed apart and scaled (a third term would change
@@ -15,10 +15,10 @@
 //   divided by their own sums before they are joined (bf16 values go up to the largest f32).
 // * Equal shares: all tiles of 128 slots of all (sequence, KV head) pairs are numbered through, and every workgroup takes an equal contiguous range of the numbers, from the lengths as
 //   they are on the device.  Groups of more than 16 query heads: 32 to a wave, or blocks of 16 with workgroups of their own and the same ranges.  A long sequence in a batch of short ones spreads over the chip by itself; a workgroup that covers a unit alone writes its result, the others
-//   leave (max, sum, accumulator) for the join.
+//   leave (reference, sum, row divided by it) for the join.
 //
-// Measured (8 KV heads of 128): 64 sequences of up to 8192 slots, f16, 32 query heads: 1.12 GB in 197 us + 6 us for the join, 5.5 TB/s; one of 131071, bf16, 64 query heads: 537 MB in 92 -
-// 105 us + 5 us; one of 301 slots: 6.8 us.  The first form, a wave per slot and a workgroup per KV head, took 10.7 ms, 336 ms and 192 us.
+// Measured (8 KV heads of 128, medians): 64 sequences of up to 8192 slots, f16, 32 query heads: 1.12 GB in 199 us + 7 us for the join, 5.4 TB/s; one of 131071, bf16, 64 query heads: 537 MB in
+// 106 us + 5 us; one of 301 slots: 7.4 us.  The first form, a wave per slot and a workgroup per KV head, took 10.7 ms, 336 ms and 192 us.
 #include "paged.cuh"
 #include "fa_decode.cuh"
 #include <algorithm>
