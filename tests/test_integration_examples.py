@@ -1,4 +1,5 @@
-"""The paged decode step of INTEGRATION.md, run on a backend that notes its calls: what the eviction holds as recent counts the token that the step stored (no GPU)."""
+"""The paged decode step of the documentation for hosts, run on a backend that notes its calls: what the eviction holds as recent counts the token that the step stored (no GPU)."""
+import glob
 import os
 import re
 
@@ -32,8 +33,9 @@ class Torch:
 
 
 def test_the_paged_decode_step():
-    text = open(os.path.join(ROOT, "INTEGRATION.md")).read()
-    section = text[text.index("### Many sequences in one pool of pages"):]
+    heading = "### Many sequences in one pool of pages"
+    (text,) = [t for t in (open(p).read() for p in glob.glob(os.path.join(ROOT, "*.md"))) if heading in t]
+    section = text[text.index(heading):]
     code = re.search(r"```python\n(.*?)```", section, re.S).group(1)
     past = torch.tensor([7, 100], dtype=torch.int32)
     names = dict(Cdna4Backend=Notes, torch=Torch, n_pages=3, n_head_kv=2, k=None, v=None, q=None, past=past, weight=None, pos=None, n_kv=torch.tensor([7, 90], dtype=torch.int32))
